@@ -16,7 +16,9 @@ it does, and needs ``dionw_b200/lib/libdionw_b200.so``
 from dionw_b200._keys import (
     FRACTION_KEY, MOMENTUM_FORM_KEY, NEWTON_SCHULZ_KEY, NUM_HEADS_KEY, ROUTE_KEY, ROW_NORMALIZATION_KEY,
 )
+from dionw_b200.adamw8 import adamw8_state, adamw8_step
 from dionw_b200.ema import EMAConfig, EMADevice, EMASchedule, IntegratedEMAOptimizer
+from dionw_b200.float8 import Float8Linear, Float8Matrix, float8_linear, float8_product, quantize_rows, quantize_tiles
 from dionw_b200.matrix_update import DION3_UPDATE, MUON_UPDATE, MatrixUpdate, MomentumForm, RowNormalization
 from dionw_b200.newton_schulz import NewtonSchulz
 from dionw_b200.optimizer import Dion
@@ -29,7 +31,8 @@ __version__ = "0.1.0"
 __all__ = [
     "DION3_UPDATE", "FRACTION_KEY", "MOMENTUM_FORM_KEY", "MUON_UPDATE", "NEWTON_SCHULZ_KEY", "NUM_HEADS_KEY",
     "ROUTE_KEY", "ROW_NORMALIZATION_KEY", "Dion", "EMAConfig", "EMADevice", "EMASchedule",
-    "IntegratedEMAOptimizer", "MatrixUpdate", "MomentumForm", "NewtonSchulz", "ParamGroups", "Route",
+    "Float8Linear", "Float8Matrix", "IntegratedEMAOptimizer", "MatrixUpdate", "MomentumForm", "NewtonSchulz", "ParamGroups", "Route",
     "RouteKind", "RouteProvider", "RouteReason", "RoutedParameter", "RoutingReport", "RowNormalization",
-    "__version__", "param_groups",
+    "__version__", "adamw8_state", "adamw8_step", "float8_linear", "float8_product", "param_groups", "quantize_rows",
+    "quantize_tiles",
 ]

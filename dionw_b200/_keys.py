@@ -23,6 +23,8 @@ MOMENTUM_KEY = "momentum"               # matrix momentum / error-feedback decay
 MUON_BETA2_KEY = "muon_beta2"           # NorMuon EMA decay of squared rows
 ROW_NORMALIZATION_KEY = "row_normalization"
 MOMENTUM_FORM_KEY = "momentum_form"
+# AdamW groups whose moments are held in 8 bits have this entry (8); the others have none.
+ADAMW_STATE_BITS_KEY = "adamw_state_bits"
 # A checkpoint is refused when one of these differs from the optimizer's groups.
 STRUCTURAL_KEYS = (
     ROUTE_KEY, FRACTION_KEY, NUM_HEADS_KEY, NEWTON_SCHULZ_KEY, ROW_NORMALIZATION_KEY, MOMENTUM_FORM_KEY,
@@ -33,6 +35,9 @@ MOMENTUM_STATE = "momentum"
 VARIANCE_STATE = "variance"
 EXP_AVG_STATE = "exp_avg"
 EXP_AVG_SQ_STATE = "exp_avg_sq"
+# of moments held in 8 bits: fp32 scales, one for 128 consecutive elements
+EXP_AVG_SCALE_STATE = "exp_avg_scale"
+EXP_AVG_SQ_SCALE_STATE = "exp_avg_sq_scale"
 # torch's load_state_dict moves an entry called "step" to the CPU; this name keeps it on the device.
 ADAMW_STEP_STATE = "adamw_step"
 

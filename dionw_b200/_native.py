@@ -9,7 +9,7 @@ current CUDA stream of the tensors' device.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint32, c_void_p
 from pathlib import Path
 from typing import Any, Sequence
 
@@ -97,6 +97,15 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "dionw_adamw_multi": (
         c_int, (_PP, _PP, _PP, _PP, _PP, _I64P, c_int, c_float, c_float, c_float, c_float, c_float, c_void_p,
                 c_void_p)),
+    "dionw_adamw8_multi": (
+        c_int, (_PP, _PP, c_int, _PP, _PP, _PP, _PP, _PP, _I64P, c_int, c_float, c_double, c_double, c_float, c_float,
+                c_uint32, c_void_p, c_void_p)),
+    "dionw_float8_quantize": (
+        c_int, (c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                c_int64, c_void_p, c_int64, c_void_p)),
+    "dionw_float8_product": (
+        c_int, (c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64,
+                c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_void_p)),
     "dionw_ema_multi": (c_int, (_PP, _PP, _I64P, c_int, c_int, c_float, c_int, c_void_p)),
     "dionw_ema_stage_pack": (c_int, (_PP, _I64P, _I64P, c_int, c_int, c_void_p, c_void_p)),
     "dionw_cpu_ema_job_start": (c_void_p, (_PP, _PP, _I64P, POINTER(c_uint8), c_int, c_float, c_void_p, c_int)),
@@ -369,6 +378,36 @@ def batched_gemm(a: Tensor, b: Tensor, out: Tensor, *, b_is_nk: bool, cin: Tenso
 
 
 # ---------------------------------------------------------------------------
+# 8-bit products
+# ---------------------------------------------------------------------------
+def _leading(t: Tensor) -> int:
+    """Leading dimension; of a single row, whose stride means nothing, its length."""
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def float8_quantize(x: Tensor, *, tiles: bool, q: Tensor | None, scales: Tensor | None, qt: Tensor | None,
+                    scales_t: Tensor | None) -> None:
+    """``q`` and ``qt`` are ``[rows, ld]`` and ``[cols, ld]`` codes; scales as the ABI stores them, two-dimensional."""
+    def ld(t: Tensor | None) -> int:
+        return 0 if t is None else _leading(t)
+
+    rows, cols = x.shape
+    _check(library().dionw_float8_quantize(
+        x.data_ptr(), dtype_code(x.dtype), rows, cols, _leading(x), int(tiles), _ptr(q), ld(q), _ptr(scales), ld(scales),
+        _ptr(qt), ld(qt), _ptr(scales_t), ld(scales_t), _stream(x)))
+
+
+def float8_product(a: Tensor, a_scales: Tensor, a_tiles: bool, b: Tensor, b_scales: Tensor, b_tiles: bool, out: Tensor,
+                   *, bias: Tensor | None, accumulate: bool) -> None:
+    """``a`` ``[m, k]``, ``b`` ``[n, k]`` codes; scales ``[rows or tile rows, blocks]`` of any strides."""
+    (m, k), n = a.shape, b.shape[0]
+    _check(library().dionw_float8_product(
+        a.data_ptr(), _leading(a), a_scales.data_ptr(), *a_scales.stride(), int(a_tiles), b.data_ptr(), _leading(b),
+        b_scales.data_ptr(), *b_scales.stride(), int(b_tiles), _ptr(bias), 0 if bias is None else dtype_code(bias.dtype),
+        out.data_ptr(), _leading(out), dtype_code(out.dtype), int(accumulate), m, n, k, _stream(out)))
+
+
+# ---------------------------------------------------------------------------
 # NorMuon and apply
 # ---------------------------------------------------------------------------
 def row_sumsq_bf16(o: Tensor, cols: int, s: Tensor) -> None:
@@ -463,6 +502,20 @@ def adamw_multi(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
     _check(library().dionw_adamw_multi(
         _ptr_array(params), _ptr_array(grads), _ptr_array(exp_avg), _ptr_array(exp_avg_sq), _ptr_array(steps),
         _i64_array([p.numel() for p in params]), len(params), lr, beta1, beta2, weight_decay, eps,
+        _ptr(hyper_device), _stream(params[0])))
+
+
+def adamw8_multi(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[Tensor],
+                 exp_avg_sq: Sequence[Tensor], exp_avg_scale: Sequence[Tensor], exp_avg_sq_scale: Sequence[Tensor],
+                 steps: Sequence[Tensor], *, lr: float, beta1: float, beta2: float, weight_decay: float, eps: float,
+                 seed: int, hyper_device: Tensor | None = None) -> None:
+    """``adamw_multi`` with 8-bit moments; gradients of one dtype per call, ``seed`` below 2**32."""
+    if not params:
+        return
+    _check(library().dionw_adamw8_multi(
+        _ptr_array(params), _ptr_array(grads), dtype_code(grads[0].dtype), _ptr_array(exp_avg), _ptr_array(exp_avg_sq),
+        _ptr_array(exp_avg_scale), _ptr_array(exp_avg_sq_scale), _ptr_array(steps),
+        _i64_array([p.numel() for p in params]), len(params), lr, beta1, beta2, weight_decay, eps, seed,
         _ptr(hyper_device), _stream(params[0])))
 
 

@@ -1,0 +1,115 @@
+"""AdamW with moments held in 8 bits, as one fused step over many tensors.
+
+The moments of a parameter are an e4m3 and an e5m2 tensor of its shape, and a
+fp32 scale for every 128 consecutive elements of each: 2.1 bytes per element
+where fp32 moments take 8, and 16.1 bytes of memory traffic a step instead of 28.
+They are updated in fp32 and rounded stochastically for the next step, by a hash
+of the seed, the step and the element's place: the same call gives the same bits.
+``Dion(..., adamw_state_bits=8)`` uses it for every AdamW-routed parameter.
+
+The reference keeps its moments in fp32 (src/dionw/_adamw.py:18-61).
+"""
+
+from __future__ import annotations
+
+import math
+from collections.abc import Sequence
+from typing import Any
+
+import torch
+from torch import Tensor
+
+from dionw_b200 import _native
+from dionw_b200._keys import (
+    ADAMW_STEP_STATE, EXP_AVG_SCALE_STATE, EXP_AVG_SQ_SCALE_STATE, EXP_AVG_SQ_STATE, EXP_AVG_STATE,
+)
+
+BLOCK = 128                        # consecutive elements that share a scale
+MEAN_DTYPE = torch.float8_e4m3fn
+SQUARE_DTYPE = torch.float8_e5m2
+_GRAD_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def adamw8_state(param: Tensor) -> dict[str, Tensor]:
+    """The state before the first step, under the keys a ``Dion`` state entry has."""
+    blocks = -(-param.numel() // BLOCK)
+    device = param.device
+    return {
+        EXP_AVG_STATE: torch.zeros(param.shape, dtype=MEAN_DTYPE, device=device),
+        EXP_AVG_SQ_STATE: torch.zeros(param.shape, dtype=SQUARE_DTYPE, device=device),
+        EXP_AVG_SCALE_STATE: torch.zeros(blocks, dtype=torch.float32, device=device),
+        EXP_AVG_SQ_SCALE_STATE: torch.zeros(blocks, dtype=torch.float32, device=device),
+        ADAMW_STEP_STATE: torch.zeros((), dtype=torch.float32, device=device),
+    }
+
+
+def dequantize_moments(entry: dict[str, Any]) -> tuple[Tensor, Tensor]:
+    """The fp32 moments that a state entry stands for, in the parameter's shape."""
+    def values(codes: Tensor, scales: Tensor) -> Tensor:
+        return (codes.float().view(-1) * scales.repeat_interleave(BLOCK)[:codes.numel()]).view(codes.shape)
+
+    return (values(entry[EXP_AVG_STATE], entry[EXP_AVG_SCALE_STATE]),
+            values(entry[EXP_AVG_SQ_STATE], entry[EXP_AVG_SQ_SCALE_STATE]))
+
+
+@torch.no_grad()
+def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[Tensor],
+                exp_avg_sq: Sequence[Tensor], exp_avg_scale: Sequence[Tensor], exp_avg_sq_scale: Sequence[Tensor],
+                steps: Sequence[Tensor], *, lr: float, betas: tuple[float, float] = (0.9, 0.95),
+                weight_decay: float = 0.0, eps: float = 1e-8, seed: int = 0,
+                hyper_device: Tensor | None = None) -> None:
+    """One decoupled-decay, bias-corrected AdamW step of every parameter, in place.
+
+    Args:
+        params: fp32 CUDA tensors of one device, contiguous, each once.
+        grads: Their gradients, of one dtype (float32, float16 or bfloat16), contiguous.
+        exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, steps: The state, as ``adamw8_state`` makes
+            it.  Every step counter goes up by one.
+        lr, betas, weight_decay, eps: As in ``Dion``.
+        seed: Of the stochastic rounding, below 2**32.
+        hyper_device: Two fp32 on the device, ``{lr, weight_decay}``, read instead of the two arguments.
+
+    A block of 128 elements in which a moment becomes infinite or NaN is NaN from then on.
+
+    Raises:
+        ValueError: On lists or tensors that do not fit one another, hyperparameters out of range, or a
+            tensor off CUDA or on another device.
+        TypeError: On a dtype other than the ones above.
+    """
+    lists = (grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, steps)
+    if any(len(values) != len(params) for values in lists):
+        raise ValueError(f"adamw8_step: {len(params)} parameters, {[len(values) for values in lists]} of the others")
+    beta1, beta2 = betas
+    if not (0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0):
+        raise ValueError(f"adamw8_step: betas must be in [0, 1), got {betas}")
+    if not (eps > 0.0 and lr >= 0.0 and weight_decay >= 0.0 and math.isfinite(lr + weight_decay + eps)):
+        raise ValueError("adamw8_step: lr and weight_decay must be >= 0 and eps > 0")
+    if not 0 <= seed < 1 << 32:
+        raise ValueError(f"adamw8_step: seed must be in [0, 2**32), got {seed}")
+    if not params:
+        return
+    device, grad_dtype = params[0].device, grads[0].dtype
+    if device.type != "cuda":
+        raise ValueError(f"adamw8_step runs on CUDA devices, got a parameter on {device}")
+    if grad_dtype not in _GRAD_DTYPES:
+        raise TypeError(f"adamw8_step takes float32, float16 or bfloat16 gradients, got {grad_dtype}")
+    for p, g, m, v, ms, vs, step in zip(params, *lists):
+        n = p.numel()
+        if (p.dtype is not torch.float32 or g.dtype is not grad_dtype or m.dtype is not MEAN_DTYPE
+                or v.dtype is not SQUARE_DTYPE or ms.dtype is not torch.float32 or vs.dtype is not torch.float32
+                or step.dtype is not torch.float32):
+            raise TypeError(f"adamw8_step: dtypes {[t.dtype for t in (p, g, m, v, ms, vs, step)]}")
+        blocks = -(-n // BLOCK)
+        if not (g.numel() == m.numel() == v.numel() == n and ms.numel() == vs.numel() == blocks and step.numel() == 1):
+            raise ValueError(f"adamw8_step: {[t.numel() for t in (p, g, m, v, ms, vs, step)]} elements")
+        for t in (p, g, m, v, ms, vs, step):
+            if t.device != device or not t.is_contiguous():
+                raise ValueError("adamw8_step needs contiguous tensors of one device")
+    if len({p.data_ptr() for p in params if p.numel()}) != sum(1 for p in params if p.numel()):
+        raise ValueError("adamw8_step: a parameter is given twice")
+    if len({step.data_ptr() for step in steps}) != len(steps):
+        raise ValueError("adamw8_step: a step counter is given twice")
+    with torch.cuda.device(device):
+        _native.adamw8_multi(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, steps, lr=lr,
+                             beta1=beta1, beta2=beta2, weight_decay=weight_decay, eps=eps, seed=seed,
+                             hyper_device=hyper_device)

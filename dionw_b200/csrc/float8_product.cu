@@ -1,0 +1,96 @@
+// Host side of the 8-bit products (float8_sm100.cuh): tensor maps, tile shapes, launches.
+#include <atomic>
+
+#include "float8_sm100.cuh"
+#include "products.cuh"
+
+namespace dionw {
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+template <int kTileN, bool kSwap>
+int launch(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  using S = float8::Shape<kTileN>;
+  static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = float8::product_kernel<kTileN, kSwap>;
+  static std::atomic<bool> configured[kMaxDevices];   // the attribute is per device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
+  if (!configured[device].load(std::memory_order_acquire)) {
+    DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmemBytes)));
+    configured[device].store(true, std::memory_order_release);
+  }
+  CUtensorMap map_a{}, map_b{};
+  if (p.k > 0) {
+    int st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
+    if (st != DIONW_OK) return st;
+    st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, kTileN);
+    if (st != DIONW_OK) return st;
+  }
+  p.tiles_m = (p.m + float8::kBM - 1) / float8::kBM;
+  p.tiles_n = (p.n + kTileN - 1) / kTileN;
+  const long long total = (long long)p.tiles_m * p.tiles_n;
+  DIONW_REQUIRE(total <= 0x7FFFFFFFll, "float8_product: too many tiles");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(total < sm_count() ? total : sm_count()));
+  config.blockDim = dim3(float8::kThreads);
+  config.dynamicSmemBytes = S::kSmemBytes;
+  config.stream = stream;
+  cudaLaunchAttribute attribute;
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = use_dependent_launch() ? 1 : 0;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
+}
+
+}  // namespace
+}  // namespace dionw
+
+using namespace dionw;
+
+extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int64_t a_row_stride,
+                                    int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
+                                    const float* b_scales, int64_t b_row_stride, int64_t b_block_stride, int b_tiles,
+                                    const void* bias, int bias_dtype, void* out, int64_t ldo, int out_dtype,
+                                    int accumulate, int64_t m, int64_t n, int64_t k, void* stream_ptr) {
+  DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= 0x7FFFFF00ll && n <= 0x7FFFFF00ll && k <= 0x7FFFFF00ll,
+                "float8_product: bad shape %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
+  DIONW_REQUIRE(out_dtype >= DIONW_F32 && out_dtype <= DIONW_BF16, "float8_product: bad output dtype");
+  DIONW_REQUIRE(bias == nullptr || (bias_dtype >= DIONW_F32 && bias_dtype <= DIONW_BF16), "float8_product: bad bias dtype");
+  if (m == 0 || n == 0) return DIONW_OK;
+  DIONW_REQUIRE(out != nullptr && ldo >= n, "float8_product: leading dimension %lld of %lld columns", (long long)ldo,
+                (long long)n);
+  if (k > 0) {
+    DIONW_REQUIRE(a != nullptr && b != nullptr && a_scales != nullptr && b_scales != nullptr, "float8_product: null operand");
+    DIONW_REQUIRE(aligned16(a) && aligned16(b) && (lda % 16 == 0 || m == 1) && (ldb % 16 == 0 || n == 1) && lda >= k && ldb >= k,
+                  "float8_product: rows of codes must start on 16-byte boundaries (leading dimensions %lld, %lld)",
+                  (long long)lda, (long long)ldb);
+  }
+  float8::Params p{};
+  p.a = {a_scales, a_row_stride, a_block_stride, a_tiles ? 7 : 0};
+  p.b = {b_scales, b_row_stride, b_block_stride, b_tiles ? 7 : 0};
+  p.out = out;
+  p.ldo = ldo;
+  p.bias = bias;
+  p.out_dtype = out_dtype;
+  p.bias_dtype = bias_dtype;
+  p.accumulate = accumulate;
+  p.m = int(m);
+  p.n = int(n);
+  p.k = int(k);
+  p.status = device_status_word();
+  p.wait_ns = gemm::kWaitLimitNs;
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (m <= 64) {
+    // A few tokens: the weights are the 128 rows of a tile.
+    std::swap(p.a, p.b);
+    std::swap(p.m, p.n);
+    if (m <= 16) return launch<16, true>(b, ldb, a, lda, p, stream);
+    if (m <= 32) return launch<32, true>(b, ldb, a, lda, p, stream);
+    return launch<64, true>(b, ldb, a, lda, p, stream);
+  }
+  return launch<128, false>(a, lda, b, ldb, p, stream);
+}

@@ -77,6 +77,34 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t inner, int64
   return DIONW_OK;
 }
 
+}  // namespace
+
+// 2-D map over a row-major matrix of bytes: (inner, rows).
+int make_byte_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, uint32_t box_inner,
+                  uint32_t box_rows) {
+  EncodeFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from this driver");
+    return DIONW_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(rows)};
+  // a single row has no next one: any legal stride will do
+  cuuint64_t strides[1] = {rows == 1 ? cuuint64_t((inner + 15) / 16 * 16) : cuuint64_t(ld)};
+  cuuint32_t box[2] = {box_inner, box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult res = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with code %d (inner=%lld rows=%lld ld=%lld)", int(res), (long long)inner,
+              (long long)rows, (long long)ld);
+    return DIONW_ERR_CUDA;
+  }
+  return DIONW_OK;
+}
+
+namespace {
+
 constexpr int kMaxDevices = 64;
 
 // Ordinal of the current device, clamped into the per-device tables.

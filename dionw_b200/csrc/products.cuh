@@ -1,6 +1,8 @@
 // Batched tensor-core products as the host describes them (gemm.cu runs them).
 #pragma once
 
+#include <cuda.h>
+
 #include "common.cuh"
 
 namespace dionw {
@@ -62,5 +64,9 @@ struct ChainSlot {
 int on_chip_pairs(int64_t blocks, int64_t m, int64_t n);
 int run_on_chip(const Product* list, const int* chain_length, const ChainSlot* slots, int n_slots, bool tall, int pairs,
                 cudaStream_t stream);
+
+// Tensor map over a row-major matrix of bytes (rows `ld` apart, 16-byte aligned), 128-byte swizzled boxes.
+int make_byte_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, uint32_t box_inner,
+                  uint32_t box_rows);
 
 }  // namespace dionw

@@ -1,0 +1,248 @@
+"""8-bit products for training beside the optimizer: e4m3 codes with a fp32 scale for each block of 128.
+
+``Dion`` steps fp32 master weights; the forward and backward passes between two steps may run in
+fewer bits.  ``quantize_rows`` gives activations and gradients a scale for each 1 x 128 block,
+``quantize_tiles`` weights one for each 128 x 128 tile, ``float8_product`` multiplies two such
+matrices on the tensor cores with fp32 sums, and ``Float8Linear`` is a linear layer made of the
+three: forward, gradient of the input, and the gradient of the weight in fp32, as the step takes it.
+
+There is no counterpart in the reference.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Any
+
+import torch
+from torch import Tensor, nn
+
+from dionw_b200 import _native
+
+BLOCK = 128
+CODES = torch.float8_e4m3fn
+_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _padded(n: int) -> int:
+    """Leading dimension of a matrix of codes: rows start on 16-byte boundaries."""
+    return (n + 15) // 16 * 16
+
+
+@dataclass(frozen=True)
+class Float8Matrix:
+    """A ``[rows, cols]`` matrix of e4m3 codes and its fp32 scales.
+
+    ``scales`` is ``[rows, ceil(cols / 128)]``, one for each 1 x 128 block, or
+    ``[ceil(rows / 128), ceil(cols / 128)]``, one for each tile; of any strides.  An element is its code
+    times its block's scale.  Rows of codes start on 16-byte boundaries, a multiple of 16 bytes apart.
+
+    Raises:
+        TypeError: On other dtypes.
+        ValueError: On shapes, strides or devices that do not fit.
+    """
+
+    values: Tensor
+    scales: Tensor
+
+    def __post_init__(self) -> None:
+        values, scales = self.values, self.scales
+        if values.dtype is not CODES or scales.dtype is not torch.float32:
+            raise TypeError(f"Float8Matrix needs float8_e4m3fn codes and float32 scales, got {values.dtype}, {scales.dtype}")
+        if values.ndim != 2 or scales.ndim != 2 or values.device != scales.device:
+            raise ValueError(
+                f"Float8Matrix needs two matrices on one device, got shapes {tuple(values.shape)} on {values.device} and "
+                f"{tuple(scales.shape)} on {scales.device}")
+        rows, cols = values.shape
+        if scales.shape[1] != _blocks(cols) or scales.shape[0] not in (rows, _blocks(rows)):
+            raise ValueError(f"scales {tuple(scales.shape)} fit neither the rows nor the tiles of {tuple(values.shape)} codes")
+        if rows and cols and ((cols > 1 and values.stride(1) != 1) or values.data_ptr() % 16
+                              or (rows > 1 and (values.stride(0) % 16 or values.stride(0) < cols))):
+            raise ValueError(f"rows of codes must start on 16-byte boundaries, got strides {values.stride()}")
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.values.shape
+
+    @property
+    def tiles(self) -> bool:
+        """Whether 128 rows share a scale."""
+        return self.scales.shape[0] != self.values.shape[0]
+
+    def dequantize(self) -> Tensor:
+        """The fp32 matrix."""
+        rows, cols = self.values.shape
+        scales = self.scales.repeat_interleave(BLOCK, 0)[:rows] if self.tiles else self.scales
+        return self.values.float() * scales.repeat_interleave(BLOCK, 1)[:, :cols]
+
+
+def _quantize(x: Tensor, tiles: bool, straight: bool, transposed: bool) -> list[Float8Matrix]:
+    if x.ndim != 2:
+        raise ValueError(f"expected a matrix, got shape {tuple(x.shape)}")
+    if not x.is_cuda:
+        raise ValueError(f"dionw_b200 quantizes on CUDA devices only, got a matrix on {x.device}")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"dionw_b200 quantizes float32, float16 and bfloat16, got {x.dtype}")
+    x = x.detach()
+    rows, cols = x.shape
+    if (cols > 1 and x.stride(1) != 1) or (rows > 1 and x.stride(0) < cols):
+        x = x.contiguous()
+    made: list[tuple[Tensor, Tensor, Float8Matrix]] = []
+    for wanted, high, wide in ((straight, rows, cols), (transposed, cols, rows)):
+        if not wanted:
+            continue
+        codes = torch.empty(high, _padded(wide), dtype=CODES, device=x.device)
+        if tiles:
+            scales = torch.empty(_blocks(high), _blocks(wide), dtype=torch.float32, device=x.device)
+            made.append((codes, scales, Float8Matrix(codes[:, :wide], scales)))
+        else:   # the scales of a block column lie together, as the product and the quantizer go through them
+            scales = torch.empty(_blocks(wide), high, dtype=torch.float32, device=x.device)
+            made.append((codes, scales, Float8Matrix(codes[:, :wide], scales.T)))
+    if rows and cols:
+        first = made[0] if straight else (None, None, None)
+        second = made[-1] if transposed else (None, None, None)
+        with torch.cuda.device(x.device):
+            _native.float8_quantize(x, tiles=tiles, q=first[0], scales=first[1], qt=second[0], scales_t=second[1])
+    return [matrix for _, _, matrix in made]
+
+
+def quantize_rows(x: Tensor, *, transposed: bool = False) -> Any:
+    """``x`` ``[rows, cols]`` with a scale for each 1 x 128 block of its rows.
+
+    Codes are rounded to nearest even; a scale is the least power of two that keeps its block in range.
+    With ``transposed=True`` returns a pair: the matrix and its transpose (scales along ``x``'s columns),
+    from one read.
+
+    Raises:
+        ValueError: If ``x`` is not a CUDA matrix.
+        TypeError: If it is not float32, float16 or bfloat16.
+    """
+    found = _quantize(x, False, True, transposed)
+    return tuple(found) if transposed else found[0]
+
+
+def quantize_tiles(x: Tensor, *, transposed: bool = False) -> Any:
+    """``quantize_rows`` with a scale for each 128 x 128 tile; the transpose has the same codes and scales."""
+    found = _quantize(x, True, True, transposed)
+    return tuple(found) if transposed else found[0]
+
+
+@torch.no_grad()
+def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = None, out: Tensor | None = None,
+                   accumulate: bool = False, out_dtype: torch.dtype | None = None) -> Tensor:
+    """``a @ b.T`` (``a`` ``[m, k]``, ``b`` ``[n, k]``), plus ``bias`` ``[n]``, summed in fp32 and rounded once.
+
+    Args:
+        out: ``[m, n]`` result (float32, float16 or bfloat16), rows contiguous; made if None.
+        accumulate: Add to what ``out`` holds.
+        out_dtype: Of the result that is made (bfloat16 if None); must be ``out``'s where both are given.
+
+    Raises:
+        ValueError: On shapes, strides or devices that do not fit, or ``accumulate`` without ``out``.
+        TypeError: On other dtypes.
+    """
+    (m, k), (n, other) = a.shape, b.shape
+    device = a.values.device
+    if k != other:
+        raise ValueError(f"float8_product: {tuple(a.shape)} and {tuple(b.shape)} differ in their columns")
+    if device.type != "cuda" or b.values.device != device:
+        raise ValueError(f"float8_product needs operands on one CUDA device, got {device} and {b.values.device}")
+    if out is None:
+        if accumulate:
+            raise ValueError("float8_product: accumulate needs out")
+        out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        if out_dtype not in _DTYPES:
+            raise TypeError(f"float8_product gives float32, float16 or bfloat16, not {out_dtype}")
+        out = torch.empty(m, n, dtype=out_dtype, device=device)
+    if out.dtype not in _DTYPES or out_dtype not in (None, out.dtype):
+        raise TypeError(f"float8_product: out is {out.dtype}, out_dtype {out_dtype}")
+    if out.shape != (m, n) or out.device != device or (m and n and ((n > 1 and out.stride(1) != 1)
+                                                                    or (m > 1 and out.stride(0) < n))):
+        raise ValueError(f"float8_product: out must be a [{m}, {n}] matrix with contiguous rows on {device}, "
+                         f"got {tuple(out.shape)} with strides {out.stride()} on {out.device}")
+    if bias is not None:
+        if bias.dtype not in _DTYPES:
+            raise TypeError(f"float8_product: bias is {bias.dtype}")
+        if bias.shape != (n,) or bias.device != device:
+            raise ValueError(f"float8_product: bias must have {n} elements on {device}, got {tuple(bias.shape)} on {bias.device}")
+        bias = bias.contiguous()
+    if m and n:
+        with torch.cuda.device(device):
+            _native.float8_product(a.values, a.scales, a.tiles, b.values, b.scales, b.tiles, out, bias=bias,
+                                   accumulate=accumulate)
+    return out
+
+
+class _Linear(torch.autograd.Function):
+    """``x @ weight.T`` on 8-bit products; every operand is quantized along the side that is summed over."""
+
+    @staticmethod
+    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
+        need_x, need_w = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        rows = _quantize(x, False, True, need_w)
+        tiles = _quantize(weight, True, True, need_x)
+        # What the backward pass needs: the transposed codes, a byte an element.
+        saved: list[Tensor | None] = [None] * 4
+        if need_w:
+            saved[:2] = rows[1].values, rows[1].scales
+        if need_x:
+            saved[2:] = tiles[1].values, tiles[1].scales
+        ctx.save_for_backward(*saved)
+        ctx.dtypes = x.dtype, weight.dtype, None if bias is None else bias.dtype
+        return float8_product(rows[0], tiles[0], bias=bias, out_dtype=x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx: Any, grad: Tensor) -> tuple[Tensor | None, ...]:
+        need_x, need_w, need_b = ctx.needs_input_grad
+        x_dtype, w_dtype, b_dtype = ctx.dtypes
+        x_codes, x_scales, w_codes, w_scales = ctx.saved_tensors
+        dx = dw = db = None
+        found = _quantize(grad, False, need_x, need_w) if need_x or need_w else []
+        if need_x:
+            dx = float8_product(found[0], Float8Matrix(w_codes, w_scales), out_dtype=x_dtype)
+        if need_w:
+            dw = float8_product(found[-1], Float8Matrix(x_codes, x_scales), out_dtype=w_dtype)
+        if need_b:
+            db = grad.float().sum(0).to(b_dtype)
+        return dx, dw, db
+
+
+def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
+    """``torch.nn.functional.linear`` with its three products in 8 bits.
+
+    ``x`` is ``[..., inputs]``, ``weight`` ``[outputs, inputs]`` (an fp32 master weight, or 2 bytes), the result has
+    ``x``'s dtype, and the weight's gradient the weight's.  Activations and output gradients get a scale for each 1 x 128
+    block along the side that is summed over, the weight one for each 128 x 128 tile.
+
+    Raises:
+        ValueError: On shapes that do not fit, or tensors off CUDA or on different devices.
+        TypeError: If a dtype is not float32, float16 or bfloat16.
+    """
+    if weight.ndim != 2 or x.ndim < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"float8_linear: x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
+    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype not in _DTYPES:
+            raise TypeError(f"float8_linear takes float32, float16 and bfloat16, {name} is {t.dtype}")
+        if t is not None and (not t.is_cuda or t.device != x.device):
+            raise ValueError(f"float8_linear needs its tensors on one CUDA device, {name} is on {t.device}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"float8_linear: bias {tuple(bias.shape)} does not fit a weight {tuple(weight.shape)}")
+    flat = x.reshape(-1, x.shape[-1])
+    return _Linear.apply(flat, weight, bias).view(*x.shape[:-1], weight.shape[0])
+
+
+class Float8Linear(nn.Linear):
+    """``nn.Linear`` on ``float8_linear``: fp32 master weight and bias, the result in the input's dtype.
+
+    ``param_groups`` routes its weight as any linear layer's; under autocast the input is cast first.
+    """
+
+    def forward(self, x: Tensor) -> Tensor:
+        if torch.is_autocast_enabled("cuda"):
+            x = x.to(torch.get_autocast_dtype("cuda"))
+        return float8_linear(x, self.weight, self.bias)

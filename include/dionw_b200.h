@@ -255,6 +255,35 @@ int dionw_batched_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, i
                        int64_t blocks, int64_t m, int64_t n, int64_t kdim, int in_dtype,
                        int out_dtype, void* stream);
 
+/* ---- 8-bit products -------------------------------------------------------- */
+/* (No counterpart in the reference, whose products are those of the optimizer step.) */
+
+/* A matrix x [rows, ldx] of any of the three dtypes into e4m3 codes with a fp32 scale for each
+ * block: 1 x 128 along the rows (tiles = 0) or 128 x 128 (tiles = 1); codes * scale are x,
+ * rounded to nearest even.  A scale is the least power of two that keeps the block's largest
+ * magnitude at most 448; 1 for a block of zeros, NaN for one with an infinity or a NaN.
+ * q (nullable) is [rows, ldq], qt (nullable) the transposed matrix [cols, ldqt]; both start on
+ * 16-byte boundaries and have leading dimensions that are multiples of 16 (codes between the
+ * matrix and the next multiple of 8 may be overwritten, with zeros).  The scale of (row r,
+ * block c) is scales[c * lds + r], of (tile row r, tile column c) scales[r * lds + c]; scales_t
+ * (ldst) is the same for the transposed matrix. */
+int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                          int tiles, void* q, int64_t ldq, float* scales, int64_t lds,
+                          void* qt, int64_t ldqt, float* scales_t, int64_t ldst, void* stream);
+
+/* out[i, j] = sum over blocks b of 128 k's of sa[i, b] sb[j, b] sum over k in b of a[i, k] b[j, k],
+ * + bias[j] (nullable), + out[i, j] (accumulate != 0); sums in fp32, rounded once to out_dtype.
+ * a [m, lda] and b [n, ldb] are e4m3 codes, rows on 16-byte boundaries; the scale of row i in
+ * block b is a_scales[i * a_row_stride + b * a_block_stride], with i / 128 in the place of i
+ * where a_tiles != 0 (b likewise).  out must not overlap an operand.  Results do not depend on
+ * anything but the operands: sums are taken in a fixed order. */
+int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int64_t a_row_stride,
+                         int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
+                         const float* b_scales, int64_t b_row_stride, int64_t b_block_stride,
+                         int b_tiles, const void* bias, int bias_dtype, void* out, int64_t ldo,
+                         int out_dtype, int accumulate, int64_t m, int64_t n, int64_t k,
+                         void* stream);
+
 /* ---- NorMuon and the weight update -------------------------------------- */
 
 /* s[b*k + r] = sum_c o[b, r, c]^2 for a bf16 batch [blocks, k, ldo] (used where
@@ -354,6 +383,22 @@ int dionw_adamw_multi(void* const* params, const void* const* grads, void* const
                       int n_tensors, float lr, float beta1, float beta2, float weight_decay,
                       float eps, const float* hyper_device, void* stream);
 /* hyper_device (nullable): {lr, weight_decay} read from device memory instead. */
+
+/* The same step with moments held in 8 bits: exp_avg[i] holds numels[i] e4m3 codes,
+ * exp_avg_sq[i] e5m2 codes, and every 128 consecutive elements share a fp32 scale in
+ * exp_avg_scale[i] and exp_avg_sq_scale[i] (ceil(numels[i] / 128) each).  A moment is its
+ * code times its scale; zeros everywhere are the state before the first step.  Moments are
+ * updated in fp32 and rounded, for the next step, to a code below or above with the
+ * probability of the distance to the other: by a hash of `seed`, the step and the element's
+ * index, so that the same call gives the same bits.  A second moment that is not zero keeps
+ * a code that is not zero.  A block in which a moment becomes infinite or NaN gets the scale
+ * NaN.  grads are of any of the three dtypes, params fp32; any alignment (16 bytes, and 4 of
+ * the codes, are the fast ones).  The reference keeps moments in fp32 (src/dionw/_adamw.py:18-61). */
+int dionw_adamw8_multi(void* const* params, const void* const* grads, int grad_dtype,
+                       void* const* exp_avg, void* const* exp_avg_sq, void* const* exp_avg_scale,
+                       void* const* exp_avg_sq_scale, void* const* steps, const int64_t* numels,
+                       int n_tensors, float lr, double beta1, double beta2, float weight_decay,
+                       float eps, uint32_t seed, const float* hyper_device, void* stream);
 
 /* shadow <- source (first = 1) or shadow += weight * (source - shadow) for
  * every tensor (weight = 1 - decay < 0.5 form of torch.lerp; else
