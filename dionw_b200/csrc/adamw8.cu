@@ -129,8 +129,10 @@ __device__ __forceinline__ void update(Piece& x, const Factors& f, const uint32_
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float g = x.g[i];
-    m[i] = fmaf(f.beta1, m[i] * x.m_scale, f.omb1 * g);
-    v[i] = fmaf(f.beta2, v[i] * x.v_scale, f.omb2 * (g * g));
+    // every operation rounded by itself: two evaluations of the moments in fp32 are the same bit for bit, and a
+    // difference in the last bit, rounded to the next code, would be one of a tenth in the steps to come
+    m[i] = __fadd_rn(__fmul_rn(f.beta1, __fmul_rn(m[i], x.m_scale)), __fmul_rn(f.omb1, g));
+    v[i] = __fadd_rn(__fmul_rn(f.beta2, __fmul_rn(v[i], x.v_scale)), __fmul_rn(f.omb2, __fmul_rn(g, g)));
     float root;
     asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v[i]));
     x.p[i] = fmaf(-f.keep, x.p[i], x.p[i]) - __fdividef(f.rate * m[i], fmaf(root, f.inv_root2, f.eps));
@@ -143,7 +145,7 @@ __device__ __forceinline__ void update(Piece& x, const Factors& f, const uint32_
   const float nan = __uint_as_float(0x7FFFFFFFu);
   x.m_scale = m_largest < INFINITY ? fmaxf(m_largest * (1.0f / kMeanMax), kSmallestScale) : nan;
   x.v_scale = v_largest < INFINITY ? fmaxf(v_largest * (1.0f / kSquareMax), kSmallestScale) : nan;
-  const float m_inv = __fdividef(1.0f, x.m_scale), v_inv = __fdividef(1.0f, x.v_scale);
+  const float m_inv = __frcp_rn(x.m_scale), v_inv = __frcp_rn(x.v_scale);
   x.m = x.v = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

@@ -1,6 +1,7 @@
 // Host side of the 8-bit products (float8_sm100.cuh): tensor maps, tile shapes, launches.
 #include <atomic>
 
+#include "float8_pair_sm100.cuh"
 #include "float8_sm100.cuh"
 #include "products.cuh"
 
@@ -42,6 +43,48 @@ int launch(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Param
   attribute.val.programmaticStreamSerializationAllowed = 1;
   config.attrs = &attribute;
   config.numAttrs = use_dependent_launch() ? 1 : 0;
+  count_launch();
+  return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
+}
+
+// 256 x 256 tiles on SM pairs.
+template <bool kRowScales>
+int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  namespace pair = float8::pair;
+  static_assert(pair::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = pair::product_kernel<kRowScales>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
+  if (!configured[device].load(std::memory_order_acquire)) {
+    DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(pair::kSmemBytes)));
+    configured[device].store(true, std::memory_order_release);
+  }
+  CUtensorMap map_a{}, map_b{};
+  if (p.k > 0) {
+    int st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
+    if (st != DIONW_OK) return st;
+    st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, pair::kPairN / 2);
+    if (st != DIONW_OK) return st;
+  }
+  p.tiles_m = (p.m + pair::kPairM - 1) / pair::kPairM;
+  p.tiles_n = (p.n + pair::kPairN - 1) / pair::kPairN;
+  const long long total = (long long)p.tiles_m * p.tiles_n, pairs_max = sm_count() / 2;
+  DIONW_REQUIRE(total <= 0x7FFFFFFFll, "float8_product: too many tiles");
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(unsigned(2 * (total < pairs_max ? total : pairs_max)));
+  config.blockDim = dim3(pair::kThreads);
+  config.dynamicSmemBytes = pair::kSmemBytes;
+  config.stream = stream;
+  cudaLaunchAttribute attributes[2];
+  attributes[0].id = cudaLaunchAttributeClusterDimension;
+  attributes[0].val.clusterDim.x = 2;
+  attributes[0].val.clusterDim.y = 1;
+  attributes[0].val.clusterDim.z = 1;
+  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[1].val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = attributes;
+  config.numAttrs = use_dependent_launch() ? 2 : 1;
   count_launch();
   return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
 }
@@ -92,5 +135,8 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
     if (m <= 32) return launch<32, true>(b, ldb, a, lda, p, stream);
     return launch<64, true>(b, ldb, a, lda, p, stream);
   }
+  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
+  if (pair_tiles >= sm_count() / 2)
+    return b_tiles ? launch_pairs<false>(a, lda, b, ldb, p, stream) : launch_pairs<true>(a, lda, b, ldb, p, stream);
   return launch<128, false>(a, lda, b, ldb, p, stream);
 }

@@ -140,6 +140,17 @@ def test_product(m, n, k, b_tiles) -> None:
         _close(dionw.float8_product(a, b, out_dtype=dtype), a64, b64)
 
 
+@pytest.mark.parametrize("m,n,k", [(2500, 1900, 300), (513, 9500, 1153), (4096, 1280, 127), (2304, 2305, 4100)])
+@pytest.mark.parametrize("b_tiles", [False, True])
+def test_product_of_many_tiles(m, n, k, b_tiles) -> None:
+    """Enough tiles for a pair of SMs each, several for some."""
+    a, a64 = _operand(m, k, False, 1)
+    b, b64 = _operand(n, k, b_tiles, 2, "rows")
+    held = torch.randn(m, n, generator=torch.Generator().manual_seed(3))
+    _close(dionw.float8_product(a, b), a64, b64)
+    _close(dionw.float8_product(a, b, out=held.to(DEV), accumulate=True), a64, b64, held.double())
+
+
 @pytest.mark.parametrize("m", [40, 200])
 def test_product_with_weights_on_the_left(m) -> None:
     a, a64 = _operand(m, 700, True, 3)
