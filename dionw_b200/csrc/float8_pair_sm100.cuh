@@ -3,11 +3,9 @@
 // its 128 rows: 128 fp32 sums a thread, in pairs (fma.rn.f32x2).
 //
 // The bound: a block of 128 is 512 cycles of MMA for 32 KB of codes a CTA.  In that time its eight summing warps read 128 x
-// 256 accumulators from TMEM (32 of 128 bytes each cycle and sub-partition: 256 cycles) and add them (64 packed
+// 256 accumulators from TMEM (128 bytes each cycle and sub-partition: 256 cycles) and add them (64 packed
 // multiply-adds a thread, 128 issue cycles; twice that where each row of B has a scale of its own).  Two
 // accumulators of 256 columns are all of TMEM, so the warps give one back as soon as it is in registers.
-//
-// Warps 0 to 3: TMA, MMA (leader), scales, idle; 4 to 11: sums and output.  Scales have a ring of their own, in each CTA.
 #pragma once
 
 #include "float8_sm100.cuh"
@@ -18,15 +16,18 @@ namespace float8 {
 namespace pair {
 
 constexpr int kPairM = 256, kPairN = 256;
-constexpr int kThreads = 384;
-constexpr int kStages = 5;
-constexpr int kScaleStages = 8;
-constexpr uint32_t kStageBytes = 2 * kABytes;          // 128 rows of A, 128 of B
-constexpr int kScaleFloats = kBM + kPairN;
-constexpr uint32_t kStagingBytes = kSumWarps * 32 * 128;
-constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + kScaleStages * kScaleFloats * 4 + 256 + 1024;
+constexpr int kThreads = 384;            // warp 0: TMA, warp 1: MMA + TMEM owner, warps 4-11: sums and output
 // Registers: 384 threads are launched with 168 each; 128 * 56 + 256 * 224 = 384 * 168.
 constexpr int kHelperRegisters = 56, kSumRegisters = 224;
+constexpr int kStages = 5;
+constexpr int kColumns = kPairN / 2;     // of a summing warp
+constexpr uint32_t kStageBytes = 2 * kABytes;          // 128 rows of A, 128 of B
+constexpr uint32_t kStagingBytes = kSumWarps * 32 * 128;
+template <bool kRowScales>
+using Queue = ScaleQueue<kRowScales ? kColumns : 0, kRowScales ? 4 : 8>;
+template <bool kRowScales>
+constexpr size_t kSmemBytes =
+    size_t(kStages) * kStageBytes + kStagingBytes + kSumWarps * Queue<kRowScales>::kBytes + 256 + 1024;
 
 __device__ __forceinline__ void tma_load_pair(uint32_t smem_dst, const CUtensorMap* map, uint32_t leader_bar, int c0, int c1) {
   asm volatile(
@@ -47,43 +48,20 @@ __device__ __forceinline__ void umma2_f8(uint32_t tmem_d, uint64_t desc_a, uint6
       : "memory");
 }
 
-// Two floats as one register pair.
-__device__ __forceinline__ uint64_t two(uint32_t lo, uint32_t hi) {
-  uint64_t v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
-  return v;
-}
-__device__ __forceinline__ uint64_t two(float lo, float hi) { return two(__float_as_uint(lo), __float_as_uint(hi)); }
-__device__ __forceinline__ float2 apart(uint64_t v) {
-  uint32_t lo, hi;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
-  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
-}
-__device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
-  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(a), "l"(b));
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t v;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
-
 // kRowScales: each row of B has its own scales; otherwise 128 share one.
-template <bool kRowScales>
+template <typename T, bool kRowScales>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   using namespace gemm;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + size_t(kStages) * kStageBytes;
-  float* scale_ring = reinterpret_cast<float*>(staging + kStagingBytes);
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(scale_ring + kScaleStages * kScaleFloats);  // leader's: both CTAs' codes landed
+  uint8_t* queues = staging + kStagingBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(queues + kSumWarps * Queue<kRowScales>::kBytes);  // leader's: both CTAs' codes landed
   uint64_t* empty_bar = full_bar + kStages;            // both: the pair's MMAs on this stage completed
   uint64_t* acc_full = empty_bar + kStages;            // [2] both
   uint64_t* acc_empty = acc_full + 2;                  // [2] leader's: both CTAs have read it
-  uint64_t* scale_full = acc_empty + 2;                // [kScaleStages] own
-  uint64_t* scale_empty = scale_full + kScaleStages;   // [kScaleStages] own
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(scale_empty + kScaleStages);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -100,10 +78,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     for (int a = 0; a < 2; ++a) {
       mbar_init(&acc_full[a], 1);
       mbar_init(&acc_empty[a], 2 * kSumWarps);
-    }
-    for (int s = 0; s < kScaleStages; ++s) {
-      mbar_init(&scale_full[s], 32);
-      mbar_init(&scale_empty[s], kSumWarps);
     }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -126,33 +100,33 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, p.wait_ns)) != 0;
   };
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegisters));
-    if (warp == 0) {
-      // ---------------------------------------------------------- TMA producer (both CTAs)
-      int s = 0;
-      uint32_t released = 1;
-      bool ok = true;
-      const uint32_t ring = smem_u32(smem), leader_full = peer_address(full_bar, 0);
-      for (int t = first_tile; t < total_tiles && ok; t += pairs) {
-        int tm, tn;
-        tile_at(t, p, tm, tn);
-        const int m0 = tm * kPairM + int(rank) * kBM, n0 = tn * kPairN + int(rank) * (kPairN / 2);
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!warp_wait(&empty_bar[s], released)) { ok = false; break; }
-          if (gemm2::elect_one()) {
-            const uint32_t dst = ring + uint32_t(s) * kStageBytes;
-            const uint32_t landed = leader_full + uint32_t(s) * uint32_t(sizeof(uint64_t));
-            // The peer's bytes may land before the leader announces them: the phase cannot complete before its arrive.
-            if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
-            tma_load_pair(dst, &map_a, landed, kb * kBK, m0);
-            tma_load_pair(dst + kABytes, &map_b, landed, kb * kBK, n0);
-          }
-          __syncwarp();
-          if (++s == kStages) s = 0, released ^= 1u;
+  if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegisters));
+  if (warp == 0) {
+    // ---------------------------------------------------------- TMA producer (both CTAs)
+    int s = 0;
+    uint32_t released = 1;
+    bool ok = true;
+    const uint32_t ring = smem_u32(smem), leader_full = peer_address(full_bar, 0);
+    for (int t = first_tile; t < total_tiles && ok; t += pairs) {
+      int tm, tn;
+      tile_at(t, p, tm, tn);
+      const int m0 = tm * kPairM + int(rank) * kBM, n0 = tn * kPairN + int(rank) * (kPairN / 2);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        if (!warp_wait(&empty_bar[s], released)) { ok = false; break; }
+        if (gemm2::elect_one()) {
+          const uint32_t dst = ring + uint32_t(s) * kStageBytes;
+          const uint32_t landed = leader_full + uint32_t(s) * uint32_t(sizeof(uint64_t));
+          // The peer's bytes may land before the leader announces them: the phase cannot complete before its arrive.
+          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * kStageBytes);
+          tma_load_pair(dst, &map_a, landed, kb * kBK, m0);
+          tma_load_pair(dst + kABytes, &map_b, landed, kb * kBK, n0);
         }
+        __syncwarp();
+        if (++s == kStages) s = 0, released ^= 1u;
       }
-    } else if (warp == 1 && rank == 0) {
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {   // the second CTA's MMA warp has nothing to issue
       // ---------------------------------------------------------- MMA issuer (leader)
       constexpr uint32_t idesc = make_idesc(kPairM, kPairN);
       int s = 0;
@@ -178,124 +152,50 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
           if (++s == kStages) s = 0, loaded ^= 1u;
         }
       }
-    } else if (warp == 2) {
-      // ---------------------------------------------------------- scales (both CTAs)
-      int s = 0;
-      uint32_t released = 1;
-      bool ok = true;
-      for (int t = first_tile; t < total_tiles && ok; t += pairs) {
-        int tm, tn;
-        tile_at(t, p, tm, tn);
-        const int m0 = tm * kPairM + int(rank) * kBM, n0 = tn * kPairN;
-        const float* a_at[kBM / 32];
-        const float* b_at[kRowScales ? kPairN / 32 : 1];
-        bool a_there[kBM / 32], b_there[kRowScales ? kPairN / 32 : 1];
-#pragma unroll
-        for (int i = 0; i < kBM / 32; ++i) {
-          const int row = m0 + 32 * i + lane;
-          a_there[i] = row < p.m;
-          a_at[i] = p.a.base + (a_there[i] ? int64_t(row >> p.a.shift) * p.a.row_stride : 0);
-        }
-#pragma unroll
-        for (int i = 0; i < (kRowScales ? kPairN / 32 : 1); ++i) {
-          const int row = n0 + (kRowScales ? 32 * i + lane : 128 * (lane & 1));
-          b_there[i] = row < p.n;
-          b_at[i] = p.b.base + (b_there[i] ? int64_t(row >> p.b.shift) * p.b.row_stride : 0);
-        }
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!warp_wait(&scale_empty[s], released)) { ok = false; break; }
-          float* dst = scale_ring + s * kScaleFloats;
-          const int64_t a_block = kb * p.a.block_stride, b_block = kb * p.b.block_stride;
-#pragma unroll
-          for (int i = 0; i < kBM / 32; ++i) copy4(dst + 32 * i + lane, a_at[i] + (a_there[i] ? a_block : 0), a_there[i]);
-          if (kRowScales) {
-#pragma unroll
-            for (int i = 0; i < kPairN / 32; ++i)
-              copy4(dst + kBM + 32 * i + lane, b_at[kRowScales ? i : 0] + (b_there[kRowScales ? i : 0] ? b_block : 0),
-                    b_there[kRowScales ? i : 0]);
-          } else if (lane < 2) {
-            copy4(dst + kBM + lane, b_at[0] + (b_there[0] ? b_block : 0), b_there[0]);
-          }
-          copies_arrive(&scale_full[s]);
-          if (++s == kScaleStages) s = 0, released ^= 1u;
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-  } else {
+  } else if (warp >= 4) {
     // ------------------------------------------------------------ sums and output (both CTAs)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSumRegisters));
-    constexpr int kColumns = kPairN / 2;
     const int sub = warp & 3, half = (warp - 4) >> 2;
     uint8_t* stage_out = staging + (warp - 4) * 32 * 128;
-    const bool vec = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
     const uint32_t tmem_mine = tmem_base + uint32_t(half * kColumns) + (uint32_t(sub * 32) << 16);
     const uint32_t leader_empty = peer_address(acc_empty, 0);
-    int s = 0;
-    uint32_t filled = 0, it = 0;
+    Queue<kRowScales> queue(queues + (warp - 4) * Queue<kRowScales>::kBytes, lane);
+    const int row_in_tile = int(rank) * kBM + sub * 32, col_in_tile = half * kColumns;
+    uint32_t it = 0;
     bool ok = true;
-    for (int t = first_tile; t < total_tiles && ok; t += pairs) {
+    int tm, tn;
+    if (first_tile < total_tiles) {
+      tile_at(first_tile, p, tm, tn);
+      queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks);
+    }
+    for (int t = first_tile; t < total_tiles; t += pairs) {
       uint64_t sum[kColumns / 2];
 #pragma unroll
       for (int c = 0; c < kColumns / 2; ++c) sum[c] = 0;
       for (int kb = 0; kb < k_blocks; ++kb, ++it) {
         const uint32_t acc = it & 1u;
-        if (!warp_wait(&scale_full[s], filled)) { ok = false; break; }
-        const float* scales = scale_ring + s * kScaleFloats;
-        const float row_scale = scales[sub * 32 + lane];
-        const ulonglong2* column_scales = reinterpret_cast<const ulonglong2*>(scales + kBM + half * kColumns);
-        const float factor = kRowScales ? row_scale : row_scale * scales[kBM + half];
-        const uint64_t factors = two(factor, factor);
+        const float* slot = queue.take();
         if (!warp_wait(&acc_full[acc], (it >> 1) & 1u)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t from = tmem_mine + acc * uint32_t(kPairN);
-#pragma unroll
-        for (int c0 = 0; c0 < kColumns; c0 += 32) {
-          uint32_t v[32];
-          tmem_load<32>(from + c0, v);
-          tmem_wait<32>(v);
-          if (c0 + 32 == kColumns) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
-          }
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            if constexpr (kRowScales) {
-              const ulonglong2 f = column_scales[(c0 + c) / 4];
-              fma2(sum[(c0 + c) / 2], two(v[c], v[c + 1]), mul2(factors, f.x));
-              fma2(sum[(c0 + c) / 2 + 1], two(v[c + 2], v[c + 3]), mul2(factors, f.y));
-            } else {
-              fma2(sum[(c0 + c) / 2], two(v[c], v[c + 1]), factors);
-              fma2(sum[(c0 + c) / 2 + 1], two(v[c + 2], v[c + 3]), factors);
-            }
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&scale_empty[s]);
-        if (++s == kScaleStages) s = 0, filled ^= 1u;
+        add_block<kColumns, 16, kRowScales>(tmem_mine + acc * uint32_t(kPairN), slot, lane, sum, [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
+        });
       }
       if (!ok) break;
-      int tm, tn;
-      tile_at(t, p, tm, tn);
-      const int row0 = tm * kPairM + int(rank) * kBM + sub * 32, col0 = tn * kPairN + half * kColumns;
-#pragma unroll
-      for (int c0 = 0; c0 < kColumns; c0 += 32) {
-        __syncwarp();
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float2 x = apart(sum[c0 / 2 + 2 * u]), y = apart(sum[c0 / 2 + 2 * u + 1]);
-          *reinterpret_cast<float4*>(stage_out + lane * 128 + ((u ^ (lane & 7)) << 4)) = make_float4(x.x, x.y, y.x, y.y);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int r = i * 4 + (lane >> 3), u = lane & 7;
-          const float4 f = *reinterpret_cast<const float4*>(stage_out + r * 128 + ((u ^ (r & 7)) << 4));
-          put4(p, row0 + r, col0 + c0 + 4 * u, f, vec);
-        }
+      const int row0 = tm * kPairM + row_in_tile, col0 = tn * kPairN + col_in_tile;
+      if (t + pairs < total_tiles) {   // the next tile's first scales come while this one's sums go out
+        tile_at(t + pairs, p, tm, tn);
+        queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks);
       }
+      write_sums<T, kColumns>(p, stage_out, row0, col0, lane, [&](int c) {
+        const float2 f = apart(sum[c / 2]);
+        return (c & 1) != 0 ? f.y : f.x;
+      });
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   // ------------------------------------------------------------ teardown

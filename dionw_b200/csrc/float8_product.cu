@@ -10,11 +10,11 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 
-template <int kTileN, bool kSwap>
-int launch(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
-  using S = float8::Shape<kTileN>;
+template <typename T, int kTileN, bool kSwap, bool kRowScales>
+int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  using S = float8::Shape<kTileN, kRowScales>;
   static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = float8::product_kernel<kTileN, kSwap>;
+  auto kernel = float8::product_kernel<T, kTileN, kSwap, kRowScales>;
   static std::atomic<bool> configured[kMaxDevices];   // the attribute is per device
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
@@ -47,17 +47,23 @@ int launch(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Param
   return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
 }
 
+template <typename T, int kTileN, bool kSwap>
+int launch(const void* a, int64_t lda, const void* b, int64_t ldb, const float8::Params& p, cudaStream_t stream) {
+  return p.b.shift != 0 ? launch_single<T, kTileN, kSwap, false>(a, lda, b, ldb, p, stream)
+                        : launch_single<T, kTileN, kSwap, true>(a, lda, b, ldb, p, stream);
+}
+
 // 256 x 256 tiles on SM pairs.
-template <bool kRowScales>
+template <typename T, bool kRowScales>
 int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
   namespace pair = float8::pair;
-  static_assert(pair::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = pair::product_kernel<kRowScales>;
+  static_assert(pair::kSmemBytes<kRowScales> <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = pair::product_kernel<T, kRowScales>;
   static std::atomic<bool> configured[kMaxDevices];
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
   if (!configured[device].load(std::memory_order_acquire)) {
-    DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(pair::kSmemBytes)));
+    DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(pair::kSmemBytes<kRowScales>)));
     configured[device].store(true, std::memory_order_release);
   }
   CUtensorMap map_a{}, map_b{};
@@ -74,7 +80,7 @@ int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8:
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(2 * (total < pairs_max ? total : pairs_max)));
   config.blockDim = dim3(pair::kThreads);
-  config.dynamicSmemBytes = pair::kSmemBytes;
+  config.dynamicSmemBytes = pair::kSmemBytes<kRowScales>;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -87,6 +93,24 @@ int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8:
   config.numAttrs = use_dependent_launch() ? 2 : 1;
   count_launch();
   return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
+}
+
+// The kernel for a product of this shape.
+template <typename T>
+int run(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  const int m = p.m;
+  if (m <= 64) {
+    // A few tokens: the weights are the 128 rows of a tile.
+    std::swap(p.a, p.b);
+    std::swap(p.m, p.n);
+    if (m <= 16) return launch<T, 16, true>(b, ldb, a, lda, p, stream);
+    if (m <= 32) return launch<T, 32, true>(b, ldb, a, lda, p, stream);
+    return launch<T, 64, true>(b, ldb, a, lda, p, stream);
+  }
+  const long long pair_tiles = ((p.m + 255ll) / 256) * ((p.n + 255ll) / 256);
+  if (pair_tiles >= sm_count() / 2)
+    return p.b.shift != 0 ? launch_pairs<T, false>(a, lda, b, ldb, p, stream) : launch_pairs<T, true>(a, lda, b, ldb, p, stream);
+  return launch<T, 128, false>(a, lda, b, ldb, p, stream);
 }
 
 }  // namespace
@@ -118,7 +142,6 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
   p.out = out;
   p.ldo = ldo;
   p.bias = bias;
-  p.out_dtype = out_dtype;
   p.bias_dtype = bias_dtype;
   p.accumulate = accumulate;
   p.m = int(m);
@@ -127,16 +150,7 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
   p.status = device_status_word();
   p.wait_ns = gemm::kWaitLimitNs;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (m <= 64) {
-    // A few tokens: the weights are the 128 rows of a tile.
-    std::swap(p.a, p.b);
-    std::swap(p.m, p.n);
-    if (m <= 16) return launch<16, true>(b, ldb, a, lda, p, stream);
-    if (m <= 32) return launch<32, true>(b, ldb, a, lda, p, stream);
-    return launch<64, true>(b, ldb, a, lda, p, stream);
-  }
-  const int64_t pair_tiles = ((m + 255) / 256) * ((n + 255) / 256);
-  if (pair_tiles >= sm_count() / 2)
-    return b_tiles ? launch_pairs<false>(a, lda, b, ldb, p, stream) : launch_pairs<true>(a, lda, b, ldb, p, stream);
-  return launch<128, false>(a, lda, b, ldb, p, stream);
+  if (out_dtype == DIONW_F32) return run<float>(a, lda, b, ldb, p, stream);
+  if (out_dtype == DIONW_F16) return run<__half>(a, lda, b, ldb, p, stream);
+  return run<__nv_bfloat16>(a, lda, b, ldb, p, stream);
 }

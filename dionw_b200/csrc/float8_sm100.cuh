@@ -4,8 +4,8 @@
 //
 // The tensor cores sum one block of 128 (four MMAs of 32) into an accumulator of its own in TMEM; eight warps read it
 // back, scale it by its row's and its column's factor and add it in fp32 registers, while the tensor cores work on the next
-// blocks in the other accumulators.  Scales travel with their block: the producer warp brings the 128-byte rows of both operands
-// by TMA and the block's scales by 4-byte asynchronous copies (any strides) into the same stage of the ring.
+// blocks in the other accumulators.  The codes come by TMA; each summing warp fetches the scales it needs itself, a few blocks
+// ahead, by 4-byte asynchronous copies (any strides) into a queue of its own.
 //
 // A is [m, k], B is [n, k], both with rows of k codes: 128 of A times kTileN of B make a tile.  With kSwap A holds the
 // weights and B a few tokens, and `out` is the transposed tile.
@@ -14,6 +14,7 @@
 #pragma once
 
 #include "cluster.cuh"
+#include "gemm2_sm100.cuh"
 #include "gemm_sm100.cuh"
 
 namespace dionw {
@@ -21,7 +22,7 @@ namespace float8 {
 
 constexpr int kBM = 128;
 constexpr int kBK = 128;                 // codes, and bytes, of a block
-constexpr int kThreads = 320;            // warp 0: TMA and scales, warp 1: MMA + TMEM owner, warps 2-9: sums and output
+constexpr int kThreads = 320;            // warp 0: TMA, warp 1: MMA + TMEM owner, warps 2-9: sums and output
 constexpr int kSumWarps = 8;
 constexpr uint32_t kABytes = kBM * kBK;  // 16 KB
 constexpr int kAccumulators = 4;
@@ -38,24 +39,12 @@ struct Params {
   void* out;
   int64_t ldo;
   const void* bias;                      // nullable: one for each column of `out`
-  int out_dtype, bias_dtype;             // DIONW_F32, _F16, _BF16
+  int bias_dtype;                        // DIONW_F32, _F16, _BF16
   int accumulate;                        // add to what `out` holds
   int m, n, k;                           // rows of A, rows of B, summed length
   int tiles_m, tiles_n;
   int* status;
   uint64_t wait_ns;
-};
-
-template <int kTileN>
-struct Shape {
-  static constexpr int kColumns = kTileN / 2;                      // of a summing warp: half of the tile's
-  static constexpr uint32_t kBBytes = kTileN * kBK;
-  static constexpr uint32_t kScaleBytes = (kBM + kTileN) * 4;
-  static constexpr uint32_t kStageBytes = (kABytes + kBBytes + kScaleBytes + 1023) / 1024 * 1024;
-  static constexpr int kStages = kTileN == 128 ? 5 : 8;
-  static constexpr uint32_t kTmemCols = kAccumulators * kTileN < 32 ? 32 : kAccumulators * kTileN;
-  static constexpr uint32_t kStagingBytes = kTileN == 128 ? kSumWarps * 32 * 128 : 0;   // 32 rows of 32 floats a warp
-  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + 256 + 1024;
 };
 
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
@@ -70,11 +59,6 @@ __device__ __forceinline__ void copy4(void* smem_dst, const float* src, bool the
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
                ::"r"(gemm::smem_u32(smem_dst)), "l"(src), "r"(there ? 4 : 0) : "memory");
 }
-// Arrives on `bar` once this thread's asynchronous copies so far are there.
-__device__ __forceinline__ void copies_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(gemm::smem_u32(bar)) : "memory");
-}
-
 __device__ __forceinline__ void umma_f8(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
                                         uint32_t accumulate) {
   asm volatile(
@@ -130,45 +114,236 @@ __device__ __forceinline__ void tmem_wait(uint32_t* v) {
                       "+r"(v[i + 6]), "+r"(v[i + 7]));
 }
 
-// One value in each of the three types.
-__device__ __forceinline__ float load_as(const void* base, int64_t at, int dtype) {
-  if (dtype == DIONW_F32) return static_cast<const float*>(base)[at];
-  if (dtype == DIONW_F16) return __half2float(static_cast<const __half*>(base)[at]);
-  return __bfloat162float(static_cast<const __nv_bfloat16*>(base)[at]);
-}
-__device__ __forceinline__ void store_as(void* base, int64_t at, int dtype, float v) {
-  if (dtype == DIONW_F32) static_cast<float*>(base)[at] = v;
-  else if (dtype == DIONW_F16) static_cast<__half*>(base)[at] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(base)[at] = __float2bfloat16_rn(v);
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ float bias_at(const Params& p, int at) {
+  if (p.bias_dtype == DIONW_F32) return static_cast<const float*>(p.bias)[at];
+  if (p.bias_dtype == DIONW_F16) return __half2float(static_cast<const __half*>(p.bias)[at]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p.bias)[at]);
 }
 
-// Four values at out[row, col ..]: bias and what is there are added in fp32, the sum is rounded once.
-__device__ __forceinline__ void put4(const Params& p, int row, int col, float4 v, bool vec) {
-  const int cols = p.n;
-  if (row >= p.m || col >= cols) return;
-  float f[4] = {v.x, v.y, v.z, v.w};
-  const int64_t at = int64_t(row) * p.ldo + col;
+// The 32 x kColumns sums of a warp (lane l: row row0 + l, columns col0 ..; get(c) is the sum of column c) into `out`, through
+// 4 KB of the warp's shared memory: 128 bytes of each row at a time, kept at unit ^ (row % 8) of 16 bytes, so that
+// neither the rows on the way in nor the lines on the way out meet in a bank.  Eight lanes then write 128 bytes of a row.
+// Bias and what is there are added to the fp32 sums, which are rounded once.
+template <typename T, int kColumns, typename Get>
+__device__ __forceinline__ void write_sums(const Params& p, uint8_t* stage, int row0, int col0, int lane, Get&& get) {
+  T* out = static_cast<T*>(p.out);
+  constexpr int kUnit = 16 / sizeof(T);
+  const bool aligned = (p.ldo & (kUnit - 1)) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  const bool whole = aligned && row0 + 32 <= p.m && col0 + kColumns <= p.n;
+  uint8_t* const my_row = stage + lane * 128;
+  const int turn = lane & 7;
+  const int r0 = lane >> 3, u = lane & 7;
+  if (whole && p.bias == nullptr && p.accumulate == 0) {
+    constexpr int kPass = 128 / sizeof(T);
+    T* const at = out + int64_t(row0 + r0) * p.ldo + col0 + u * kUnit;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (col + i >= cols) continue;
-    if (p.bias != nullptr) f[i] += load_as(p.bias, col + i, p.bias_dtype);
-    if (p.accumulate) f[i] += load_as(p.out, at + i, p.out_dtype);
-  }
-  if (vec && col + 4 <= cols) {
-    if (p.out_dtype == DIONW_F32) {
-      *reinterpret_cast<float4*>(static_cast<float*>(p.out) + at) = make_float4(f[0], f[1], f[2], f[3]);
-    } else if (p.out_dtype == DIONW_F16) {
-      *reinterpret_cast<uint2*>(static_cast<__half*>(p.out) + at) =
-          make_uint2(gemm::pack2<__half>(f[0], f[1]), gemm::pack2<__half>(f[2], f[3]));
-    } else {
-      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + at) =
-          make_uint2(gemm::pack2<__nv_bfloat16>(f[0], f[1]), gemm::pack2<__nv_bfloat16>(f[2], f[3]));
+    for (int c0 = 0; c0 < kColumns; c0 += kPass) {
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        uint4 w;
+        if constexpr (sizeof(T) == 4) {
+          w = make_uint4(__float_as_uint(get(c0 + 4 * i)), __float_as_uint(get(c0 + 4 * i + 1)),
+                         __float_as_uint(get(c0 + 4 * i + 2)), __float_as_uint(get(c0 + 4 * i + 3)));
+        } else {
+          w = make_uint4(gemm::pack2<T>(get(c0 + 8 * i), get(c0 + 8 * i + 1)), gemm::pack2<T>(get(c0 + 8 * i + 2), get(c0 + 8 * i + 3)),
+                         gemm::pack2<T>(get(c0 + 8 * i + 4), get(c0 + 8 * i + 5)), gemm::pack2<T>(get(c0 + 8 * i + 6), get(c0 + 8 * i + 7)));
+        }
+        *reinterpret_cast<uint4*>(my_row + ((i ^ turn) << 4)) = w;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 4 * i + r0;
+        *reinterpret_cast<uint4*>(at + int64_t(4 * i) * p.ldo + c0) = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+      }
     }
     return;
   }
+  const bool add = p.accumulate != 0;
+  const bool vec = aligned && (col0 & 3) == 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i < cols) store_as(p.out, at + i, p.out_dtype, f[i]);
+  for (int c0 = 0; c0 < kColumns; c0 += 32) {
+    const int col = col0 + c0 + 4 * u;
+    const bool inside = vec && col + 4 <= p.n;
+    float bias[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (p.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bias[j] = col + j < p.n ? bias_at(p, col + j) : 0.0f;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      *reinterpret_cast<float4*>(my_row + ((i ^ turn) << 4)) =
+          make_float4(get(c0 + 4 * i), get(c0 + 4 * i + 1), get(c0 + 4 * i + 2), get(c0 + 4 * i + 3));
+    __syncwarp();
+#pragma unroll 4
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + r0, row = row0 + r;
+      if (row >= p.m) continue;
+      const float4 v = *reinterpret_cast<const float4*>(stage + r * 128 + ((u ^ (r & 7)) << 4));
+      float f[4] = {v.x + bias[0], v.y + bias[1], v.z + bias[2], v.w + bias[3]};
+      T* at = out + int64_t(row) * p.ldo + col;
+      if (inside) {
+        if constexpr (sizeof(T) == 4) {
+          float4* q = reinterpret_cast<float4*>(at);
+          if (add) {
+            const float4 held = *q;
+            f[0] += held.x; f[1] += held.y; f[2] += held.z; f[3] += held.w;
+          }
+          *q = make_float4(f[0], f[1], f[2], f[3]);
+        } else {
+          uint2* q = reinterpret_cast<uint2*>(at);
+          if (add) {
+            const uint2 held = *q;
+            const float2 a = gemm::unpack2<T>(held.x), b = gemm::unpack2<T>(held.y);
+            f[0] += a.x; f[1] += a.y; f[2] += b.x; f[3] += b.y;
+          }
+          *q = make_uint2(gemm::pack2<T>(f[0], f[1]), gemm::pack2<T>(f[2], f[3]));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (col + j >= p.n) continue;
+          at[j] = from_float<T>(add ? f[j] + to_float<T>(at[j]) : f[j]);
+        }
+      }
+    }
+  }
+}
+
+// The scales that a summing warp needs: one for each of its 32 rows, and kColumnScales for its columns (0: one for all of
+// them), block after block, fetched kDepth - 1 blocks ahead into a queue in shared memory that only this warp uses.  (A ring
+// filled by a warp of its own, released and awaited through barriers, cost each block some 400 cycles of barrier traffic:
+// 8192 x 14336 x 4096 on SM pairs took 590 us with it, 466 without any scales.)
+template <int kColumnScales, int kDepth>
+struct ScaleQueue {
+  static constexpr int kFloats = 32 + (kColumnScales == 0 ? 4 : kColumnScales);
+  static constexpr uint32_t kBytes = kDepth * kFloats * 4;
+  static constexpr int kCopies = (kColumnScales + 31) / 32;
+
+  float* slots;
+  const float* row_at;         // of the next block to fetch
+  const float* column_at;
+  int64_t row_step, column_step, column_apart;
+  int left;                    // blocks to fetch
+  int columns_there;           // of this warp, from its first one
+  bool row_there;
+  int lane;
+  uint32_t next_in, next_out;
+
+  __device__ __forceinline__ ScaleQueue(void* at, int lane_)
+      : slots(static_cast<float*>(at)), lane(lane_), next_in(0), next_out(0) {}
+
+  __device__ __forceinline__ void fetch() {
+    if (left > 0) {
+      float* slot = slots + next_in * kFloats;
+      copy4(slot + lane, row_at, row_there);
+      row_at += row_there ? row_step : 0;
+      if constexpr (kColumnScales == 0) {
+        if (lane == 0) copy4(slot + 32, column_at, columns_there > 0);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int c = 32 * i + lane;
+          const bool there = c < columns_there;
+          if (kColumnScales % 32 == 0 || c < kColumnScales) copy4(slot + 32 + c, there ? column_at + i * column_apart : row_at, there);
+        }
+      }
+      column_at += column_step;
+      --left;
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    next_in = next_in + 1 == kDepth ? 0 : next_in + 1;
+  }
+
+  // The first blocks of a tile whose rows and columns start at row0 and col0 for this warp.
+  __device__ __forceinline__ void start(const Params& p, int row0, int col0, int blocks) {
+    const int row = row0 + lane;
+    row_there = row < p.m;
+    row_at = p.a.base + (row_there ? int64_t(row >> p.a.shift) * p.a.row_stride : 0);
+    row_step = p.a.block_stride;
+    columns_there = p.n - col0;
+    const int column = kColumnScales == 0 ? col0 : col0 + lane;
+    column_at = p.b.base + (columns_there > 0 ? int64_t(column >> p.b.shift) * p.b.row_stride : 0);
+    column_apart = 32 * p.b.row_stride;
+    column_step = columns_there > 0 ? p.b.block_stride : 0;
+    left = blocks;
+    next_out = next_in;
+    __syncwarp();              // nobody reads the last tile's any more
+#pragma unroll
+    for (int i = 0; i < kDepth - 1; ++i) fetch();
+  }
+
+  // The slot of the next block, in the order of fetching; the one before it is fetched into.
+  __device__ __forceinline__ const float* take() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
+    __syncwarp();              // every lane's copies are there, and the slot before has been read
+    fetch();
+    const float* slot = slots + next_out * kFloats;
+    next_out = next_out + 1 == kDepth ? 0 : next_out + 1;
+    return slot;
+  }
+};
+
+// Two floats as one register pair.
+__device__ __forceinline__ uint64_t two(uint32_t lo, uint32_t hi) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+  return v;
+}
+__device__ __forceinline__ float2 apart(uint64_t v) {
+  uint32_t lo, hi;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+  return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ void fma2(uint64_t& sum, uint64_t a, uint64_t b) {
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(a), "l"(b));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+// Adds a block's sums, times their factors, to this lane's kColumns sums (in pairs): from the accumulator at `taddr`, kChunk
+// columns on their way while the ones before are added.  `slot` holds the block's scales.  Calls `release` once the
+// accumulator is in registers.
+template <int kColumns, int kChunk, bool kRowScales, typename Release>
+__device__ __forceinline__ void add_block(uint32_t taddr, const float* slot, int lane, uint64_t (&sum)[kColumns / 2],
+                                          Release&& release) {
+  const float factor = kRowScales ? slot[lane] : slot[lane] * slot[32];
+  const uint64_t factors = two(__float_as_uint(factor), __float_as_uint(factor));
+  const ulonglong2* column_scales = reinterpret_cast<const ulonglong2*>(slot + 32);
+  uint32_t v[2][kChunk];
+  tmem_load<kChunk>(taddr, v[0]);
+#pragma unroll
+  for (int c0 = 0; c0 < kColumns; c0 += kChunk) {
+    uint32_t (&now)[kChunk] = v[(c0 / kChunk) & 1];
+    tmem_wait<kChunk>(now);
+    if (c0 + kChunk < kColumns) tmem_load<kChunk>(taddr + c0 + kChunk, v[(c0 / kChunk + 1) & 1]);
+    else release();
+#pragma unroll
+    for (int c = 0; c < kChunk; c += 4) {
+      if constexpr (kRowScales) {
+        const ulonglong2 f = column_scales[(c0 + c) / 4];
+        fma2(sum[(c0 + c) / 2], two(now[c], now[c + 1]), mul2(factors, f.x));
+        fma2(sum[(c0 + c) / 2 + 1], two(now[c + 2], now[c + 3]), mul2(factors, f.y));
+      } else {
+        fma2(sum[(c0 + c) / 2], two(now[c], now[c + 1]), factors);
+        fma2(sum[(c0 + c) / 2 + 1], two(now[c + 2], now[c + 3]), factors);
+      }
+    }
+  }
 }
 
 // Tiles in groups of eight tile rows that sweep the columns: a wave of CTAs shares its operands in L2.
@@ -181,18 +356,31 @@ __device__ __forceinline__ void tile_at(int t, const Params& p, int& tm, int& tn
   tn = r / rows_here;
 }
 
-template <int kTileN, bool kSwap>
+template <int kTileN, bool kRowScales>
+struct Shape {
+  static constexpr int kColumns = kTileN / 2;                      // of a summing warp: half of the tile's
+  static constexpr uint32_t kStageBytes = kABytes + kTileN * kBK;
+  static constexpr int kStages = kTileN == 128 ? 5 : 8;
+  static constexpr uint32_t kTmemCols = kAccumulators * kTileN < 32 ? 32 : kAccumulators * kTileN;
+  static constexpr uint32_t kStagingBytes = kTileN == 128 ? kSumWarps * 32 * 128 : 0;   // 128 bytes of 32 rows a warp
+  using Queue = ScaleQueue<kRowScales ? kColumns : 0, kRowScales && kTileN == 128 ? 6 : 8>;
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + kSumWarps * Queue::kBytes + 256 + 1024;
+};
+
+// kRowScales: each row of B has scales of its own; otherwise 128 share one.
+template <typename T, int kTileN, bool kSwap, bool kRowScales>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   using namespace gemm;
-  using S = Shape<kTileN>;
+  using S = Shape<kTileN, kRowScales>;
   constexpr int kStages = S::kStages;
   constexpr int kAcc = kAccumulators;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + size_t(kStages) * S::kStageBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + S::kStagingBytes);   // codes and scales of a stage are there
-  uint64_t* empty_bar = full_bar + kStages;     // its MMAs are done, its scales read
+  uint8_t* queues = staging + S::kStagingBytes;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(queues + kSumWarps * S::Queue::kBytes);   // codes of a stage are there
+  uint64_t* empty_bar = full_bar + kStages;     // its MMAs are done
   uint64_t* acc_full = empty_bar + kStages;     // [kAcc] a block's sums are complete
   uint64_t* acc_empty = acc_full + kAcc;        // [kAcc] they are read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + kAcc);
@@ -204,8 +392,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full_bar[s], 1 + 32);          // the byte count, and the copies of each lane
-      mbar_init(&empty_bar[s], 1 + kSumWarps);
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < kAcc; ++a) {
       mbar_init(&acc_full[a], 1);
@@ -232,43 +420,24 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   };
 
   if (warp == 0) {
-    // ------------------------------------------------------------ TMA and scale producer
+    // ------------------------------------------------------------ TMA producer
     uint32_t it = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
       int tm, tn;
       tile_at(t, p, tm, tn);
-      const int m0 = tm * kBM, n0 = tn * kTileN;
       for (int kb = 0; kb < k_blocks; ++kb, ++it) {
         const int s = it % kStages;
         if (!warp_wait(&empty_bar[s], ((it / kStages) & 1u) ^ 1u)) { ok = false; break; }
-        uint8_t* a_dst = smem + size_t(s) * S::kStageBytes;
-        uint8_t* b_dst = a_dst + kABytes;
-        float* scale_dst = reinterpret_cast<float*>(b_dst + S::kBBytes);
-        if (lane == 0) {
-          mbar_expect_tx(&full_bar[s], kABytes + S::kBBytes);
-          tma_load_2d(a_dst, &map_a, &full_bar[s], kb * kBK, m0);
-          tma_load_2d(b_dst, &map_b, &full_bar[s], kb * kBK, n0);
+        uint8_t* dst = smem + size_t(s) * S::kStageBytes;
+        if (gemm2::elect_one()) {
+          mbar_expect_tx(&full_bar[s], S::kStageBytes);
+          tma_load_2d(dst, &map_a, &full_bar[s], kb * kBK, tm * kBM);
+          tma_load_2d(dst + kABytes, &map_b, &full_bar[s], kb * kBK, tn * kTileN);
         }
-#pragma unroll
-        for (int i = 0; i < kBM; i += 32) {
-          const int row = m0 + i + lane;
-          const bool there = row < p.m;
-          copy4(scale_dst + i + lane,
-                p.a.base + (there ? int64_t(row >> p.a.shift) * p.a.row_stride + kb * p.a.block_stride : 0), there);
-        }
-#pragma unroll
-        for (int i = 0; i < kTileN; i += 32) {
-          if (kTileN < 32 && lane >= kTileN) break;
-          const int row = n0 + i + lane;
-          const bool there = row < p.n;
-          copy4(scale_dst + kBM + i + lane,
-                p.b.base + (there ? int64_t(row >> p.b.shift) * p.b.row_stride + kb * p.b.block_stride : 0), there);
-        }
-        copies_arrive(&full_bar[s]);
+        __syncwarp();
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     constexpr uint32_t idesc = make_idesc(kBM, kTileN);
@@ -283,7 +452,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         tc_fence_after();
         const uint32_t a_addr = smem_u32(smem + size_t(s) * S::kStageBytes);
         const uint64_t a_desc = make_smem_desc(a_addr, 16, 1024), b_desc = make_smem_desc(a_addr + kABytes, 16, 1024);
-        if (lane == 0) {
+        if (gemm2::elect_one()) {
 #pragma unroll
           for (int j = 0; j < kBK / 32; ++j)    // 32 codes further along each 128-byte row
             umma_f8(tmem_base + acc * kTileN, a_desc + 2 * j, b_desc + 2 * j, idesc, j > 0 ? 1u : 0u);
@@ -297,83 +466,61 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     // ------------------------------------------------------------ sums and output
     // Two warps for each TMEM sub-partition (a warp reads the 32 lanes 32 * (warp % 4) ..): half of the columns each.
     constexpr int kColumns = S::kColumns;
-    constexpr int kPiece = kColumns < 32 ? kColumns : 32;
     const int sub = warp & 3;
     const int first_column = ((warp - 2) >> 2) * kColumns;
     uint8_t* stage_out = staging + (warp - 2) * 32 * 128;
-    const bool vec = (p.ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15u) == 0;
+    typename S::Queue queue(queues + (warp - 2) * S::Queue::kBytes, lane);
     uint32_t it = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < total_tiles && ok; t += gridDim.x) {
-      float sum[kColumns];
+    int tm, tn;
+    if (blockIdx.x < total_tiles) {
+      tile_at(blockIdx.x, p, tm, tn);
+      queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks);
+    }
+    for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
+      uint64_t sum[kColumns / 2];
 #pragma unroll
-      for (int c = 0; c < kColumns; ++c) sum[c] = 0.0f;
+      for (int c = 0; c < kColumns / 2; ++c) sum[c] = 0;
       for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-        const int s = it % kStages;
         const uint32_t acc = it % kAcc;
-        if (!warp_wait(&full_bar[s], (it / kStages) & 1u)) { ok = false; break; }
-        const float* scales = reinterpret_cast<const float*>(smem + size_t(s) * S::kStageBytes + kABytes + S::kBBytes);
-        const float row_scale = scales[sub * 32 + lane];
-        const float4* column_scales = reinterpret_cast<const float4*>(scales + kBM + first_column);
+        const float* slot = queue.take();
         if (!warp_wait(&acc_full[acc], (it / kAcc) & 1u)) { ok = false; break; }
         tc_fence_after();
-#pragma unroll
-        for (int c0 = 0; c0 < kColumns; c0 += kPiece) {
-          uint32_t v[kPiece];
-          tmem_load<kPiece>(tmem_base + acc * kTileN + uint32_t(first_column + c0) + (uint32_t(sub * 32) << 16), v);
-          tmem_wait<kPiece>(v);
-#pragma unroll
-          for (int c = 0; c < kPiece; c += 4) {
-            const float4 f = column_scales[(c0 + c) / 4];
-            sum[c0 + c] = fmaf(__uint_as_float(v[c]), row_scale * f.x, sum[c0 + c]);
-            sum[c0 + c + 1] = fmaf(__uint_as_float(v[c + 1]), row_scale * f.y, sum[c0 + c + 1]);
-            sum[c0 + c + 2] = fmaf(__uint_as_float(v[c + 2]), row_scale * f.z, sum[c0 + c + 2]);
-            sum[c0 + c + 3] = fmaf(__uint_as_float(v[c + 3]), row_scale * f.w, sum[c0 + c + 3]);
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&acc_empty[acc]);
-          mbar_arrive(&empty_bar[s]);
-        }
+        add_block<kColumns, kColumns < 32 ? kColumns : 32, kRowScales>(
+            tmem_base + acc * kTileN + uint32_t(first_column) + (uint32_t(sub * 32) << 16), slot, lane, sum, [&] {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&acc_empty[acc]);
+            });
       }
       if (!ok) break;
-      int tm, tn;
-      tile_at(t, p, tm, tn);
       const int row0 = tm * kBM + sub * 32, col0 = tn * kTileN + first_column;
+      if (t + int(gridDim.x) < total_tiles) {   // the next tile's first scales come while this one's sums go out
+        tile_at(t + int(gridDim.x), p, tm, tn);
+        queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks);
+      }
+      auto value = [&](int c) {
+        const float2 f = apart(sum[c / 2]);
+        return (c & 1) != 0 ? f.y : f.x;
+      };
       if constexpr (kSwap) {
         // rows of A are columns of the output: 32 lanes write neighbours
         const int column = row0 + lane;
+        const float bias = p.bias != nullptr && column < p.m ? bias_at(p, column) : 0.0f;
 #pragma unroll
         for (int c = 0; c < kColumns; ++c) {
           const int row = col0 + c;
           if (row >= p.n || column >= p.m) continue;
-          const int64_t at = int64_t(row) * p.ldo + column;
-          float f = sum[c];
-          if (p.bias != nullptr) f += load_as(p.bias, column, p.bias_dtype);
-          if (p.accumulate) f += load_as(p.out, at, p.out_dtype);
-          store_as(p.out, at, p.out_dtype, f);
+          T* at = static_cast<T*>(p.out) + int64_t(row) * p.ldo + column;
+          float f = value(c) + bias;
+          if (p.accumulate) f += to_float<T>(*at);
+          *at = from_float<T>(f);
         }
       } else {
-        // 32 columns at a time through shared memory: eight lanes write 32 neighbours of a row
-#pragma unroll
-        for (int c0 = 0; c0 < kColumns; c0 += 32) {
-          __syncwarp();
-#pragma unroll
-          for (int u = 0; u < 8; ++u)
-            *reinterpret_cast<float4*>(stage_out + lane * 128 + ((u ^ (lane & 7)) << 4)) =
-                make_float4(sum[c0 + 4 * u], sum[c0 + 4 * u + 1], sum[c0 + 4 * u + 2], sum[c0 + 4 * u + 3]);
-          __syncwarp();
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = i * 4 + (lane >> 3), u = lane & 7;
-            const float4 f = *reinterpret_cast<const float4*>(stage_out + r * 128 + ((u ^ (r & 7)) << 4));
-            put4(p, row0 + r, col0 + c0 + 4 * u, f, vec);
-          }
-        }
+        write_sums<T, kColumns>(p, stage_out, row0, col0, lane, value);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   // ------------------------------------------------------------ teardown
