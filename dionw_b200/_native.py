@@ -9,6 +9,7 @@ current CUDA stream of the tensors' device.
 from __future__ import annotations
 
 import ctypes
+from array import array
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint8, c_uint32, c_void_p
 from pathlib import Path
 from typing import Any, Sequence
@@ -97,9 +98,10 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "dionw_adamw_multi": (
         c_int, (_PP, _PP, _PP, _PP, _PP, _I64P, c_int, c_float, c_float, c_float, c_float, c_float, c_void_p,
                 c_void_p)),
+    # (host arrays by their address: see adamw8_multi)
     "dionw_adamw8_multi": (
-        c_int, (_PP, _PP, c_int, _PP, _PP, _PP, _PP, _PP, _I64P, c_int, c_float, c_double, c_double, c_float, c_float,
-                c_uint32, c_void_p, c_void_p)),
+        c_int, (c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_float,
+                c_double, c_double, c_float, c_float, c_uint32, c_void_p, c_void_p)),
     "dionw_float8_quantize": (
         c_int, (c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                 c_int64, c_void_p, c_int64, c_void_p)),
@@ -380,31 +382,34 @@ def batched_gemm(a: Tensor, b: Tensor, out: Tensor, *, b_is_nk: bool, cin: Tenso
 # ---------------------------------------------------------------------------
 # 8-bit products
 # ---------------------------------------------------------------------------
-def _leading(t: Tensor) -> int:
-    """Leading dimension; of a single row, whose stride means nothing, its length."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def on_device(device: int, entry: Any, *args: Any) -> None:
+    """Call an entry point with that device current, on its current stream (the entry's last argument).
+
+    The calls around 8-bit products are many and short: the guard's and the stream object's 4 us are saved where the
+    device is current already, and the raw handle is asked for.
+    """
+    if torch.cuda.current_device() == device:
+        _check(entry(*args, torch._C._cuda_getCurrentRawStream(device)))
+        return
+    with torch.cuda.device(device):
+        _check(entry(*args, torch._C._cuda_getCurrentRawStream(device)))
 
 
-def float8_quantize(x: Tensor, *, tiles: bool, q: Tensor | None, scales: Tensor | None, qt: Tensor | None,
-                    scales_t: Tensor | None) -> None:
-    """``q`` and ``qt`` are ``[rows, ld]`` and ``[cols, ld]`` codes; scales as the ABI stores them, two-dimensional."""
-    def ld(t: Tensor | None) -> int:
-        return 0 if t is None else _leading(t)
-
-    rows, cols = x.shape
-    _check(library().dionw_float8_quantize(
-        x.data_ptr(), dtype_code(x.dtype), rows, cols, _leading(x), int(tiles), _ptr(q), ld(q), _ptr(scales), ld(scales),
-        _ptr(qt), ld(qt), _ptr(scales_t), ld(scales_t), _stream(x)))
+def float8_quantize(device: int, x: int, dtype: torch.dtype, rows: int, cols: int, ldx: int, tiles: bool, q: int | None,
+                    ldq: int, scales: int | None, lds: int, qt: int | None, ldqt: int, scales_t: int | None,
+                    ldst: int) -> None:
+    """By address, as the ABI takes it; no matrix without elements."""
+    on_device(device, library().dionw_float8_quantize, x, _DTYPE_CODE[dtype], rows, cols, ldx, tiles, q, ldq, scales, lds,
+              qt, ldqt, scales_t, ldst)
 
 
-def float8_product(a: Tensor, a_scales: Tensor, a_tiles: bool, b: Tensor, b_scales: Tensor, b_tiles: bool, out: Tensor,
-                   *, bias: Tensor | None, accumulate: bool) -> None:
-    """``a`` ``[m, k]``, ``b`` ``[n, k]`` codes; scales ``[rows or tile rows, blocks]`` of any strides."""
-    (m, k), n = a.shape, b.shape[0]
-    _check(library().dionw_float8_product(
-        a.data_ptr(), _leading(a), a_scales.data_ptr(), *a_scales.stride(), int(a_tiles), b.data_ptr(), _leading(b),
-        b_scales.data_ptr(), *b_scales.stride(), int(b_tiles), _ptr(bias), 0 if bias is None else dtype_code(bias.dtype),
-        out.data_ptr(), _leading(out), dtype_code(out.dtype), int(accumulate), m, n, k, _stream(out)))
+def float8_product(device: int, a: tuple[int, int, int, int, int, bool], b: tuple[int, int, int, int, int, bool],
+                   bias: Tensor | None, out: Tensor, accumulate: bool, m: int, n: int, k: int) -> None:
+    """``a`` and ``b``: address and leading dimension of the codes, address and the two strides of the scales, and
+    whether those are tiles'."""
+    on_device(device, library().dionw_float8_product, *a, *b, None if bias is None else bias.data_ptr(),
+              0 if bias is None else _DTYPE_CODE[bias.dtype], out.data_ptr(), out.stride(0) if m > 1 else n,
+              _DTYPE_CODE[out.dtype], accumulate, m, n, k)
 
 
 # ---------------------------------------------------------------------------
@@ -505,18 +510,16 @@ def adamw_multi(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         _ptr(hyper_device), _stream(params[0])))
 
 
-def adamw8_multi(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[Tensor],
-                 exp_avg_sq: Sequence[Tensor], exp_avg_scale: Sequence[Tensor], exp_avg_sq_scale: Sequence[Tensor],
-                 steps: Sequence[Tensor], *, lr: float, beta1: float, beta2: float, weight_decay: float, eps: float,
-                 seed: int, hyper_device: Tensor | None = None) -> None:
-    """``adamw_multi`` with 8-bit moments; gradients of one dtype per call, ``seed`` below 2**32."""
-    if not params:
-        return
-    _check(library().dionw_adamw8_multi(
-        _ptr_array(params), _ptr_array(grads), dtype_code(grads[0].dtype), _ptr_array(exp_avg), _ptr_array(exp_avg_sq),
-        _ptr_array(exp_avg_scale), _ptr_array(exp_avg_sq_scale), _ptr_array(steps),
-        _i64_array([p.numel() for p in params]), len(params), lr, beta1, beta2, weight_decay, eps, seed,
-        _ptr(hyper_device), _stream(params[0])))
+def adamw8_multi(addresses: Sequence[Sequence[int]], numels: Sequence[int], grad_dtype: torch.dtype, *, device: int,
+                 lr: float, beta1: float, beta2: float, weight_decay: float, eps: float, seed: int,
+                 hyper_device: Tensor | None = None) -> None:
+    """``adamw_multi`` with 8-bit moments.  ``addresses``: those of the parameters, gradients (of one dtype), the two
+    moments, their scales and the step counters, on device number ``device``; ``seed`` below 2**32."""
+    tables = [array("Q", column) for column in addresses]
+    counts = array("q", numels)
+    p, g, m, v, m_scale, v_scale, steps = (table.buffer_info()[0] for table in tables)
+    on_device(device, library().dionw_adamw8_multi, p, g, _DTYPE_CODE[grad_dtype], m, v, m_scale, v_scale, steps,
+              counts.buffer_info()[0], len(counts), lr, beta1, beta2, weight_decay, eps, seed, _ptr(hyper_device))
 
 
 def ema_multi(shadows: Sequence[Tensor], sources: Sequence[Tensor], *, weight: float, first: bool) -> None:

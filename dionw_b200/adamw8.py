@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import math
 from collections.abc import Sequence
+from operator import attrgetter
 from typing import Any
 
 import torch
@@ -27,6 +28,7 @@ from dionw_b200._keys import (
 BLOCK = 128                        # consecutive elements that share a scale
 MEAN_DTYPE = torch.float8_e4m3fn
 SQUARE_DTYPE = torch.float8_e5m2
+_dtype_of = attrgetter("dtype")
 _GRAD_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -88,28 +90,30 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         raise ValueError(f"adamw8_step: seed must be in [0, 2**32), got {seed}")
     if not params:
         return
-    device, grad_dtype = params[0].device, grads[0].dtype
-    if device.type != "cuda":
-        raise ValueError(f"adamw8_step runs on CUDA devices, got a parameter on {device}")
+    device, grad_dtype = params[0].get_device(), grads[0].dtype
+    if not params[0].is_cuda:
+        raise ValueError(f"adamw8_step runs on CUDA devices, got a parameter on {params[0].device}")
     if grad_dtype not in _GRAD_DTYPES:
         raise TypeError(f"adamw8_step takes float32, float16 or bfloat16 gradients, got {grad_dtype}")
-    for p, g, m, v, ms, vs, step in zip(params, *lists):
-        n = p.numel()
-        if (p.dtype is not torch.float32 or g.dtype is not grad_dtype or m.dtype is not MEAN_DTYPE
-                or v.dtype is not SQUARE_DTYPE or ms.dtype is not torch.float32 or vs.dtype is not torch.float32
-                or step.dtype is not torch.float32):
-            raise TypeError(f"adamw8_step: dtypes {[t.dtype for t in (p, g, m, v, ms, vs, step)]}")
-        blocks = -(-n // BLOCK)
-        if not (g.numel() == m.numel() == v.numel() == n and ms.numel() == vs.numel() == blocks and step.numel() == 1):
-            raise ValueError(f"adamw8_step: {[t.numel() for t in (p, g, m, v, ms, vs, step)]} elements")
-        for t in (p, g, m, v, ms, vs, step):
-            if t.device != device or not t.is_contiguous():
-                raise ValueError("adamw8_step needs contiguous tensors of one device")
-    if len({p.data_ptr() for p in params if p.numel()}) != sum(1 for p in params if p.numel()):
+    # Hundreds of tensors a step: each question goes to a whole list at a time.
+    columns = (params, *lists)
+    for column, dtype in zip(columns, (torch.float32, grad_dtype, MEAN_DTYPE, SQUARE_DTYPE) + (torch.float32,) * 3):
+        if set(map(_dtype_of, column)) != {dtype}:
+            raise TypeError(f"adamw8_step: expected {dtype}, got {set(map(_dtype_of, column))}")
+        if set(map(Tensor.get_device, column)) != {device} or not all(map(Tensor.is_contiguous, column)):
+            raise ValueError("adamw8_step needs contiguous tensors of one device")
+    numels = list(map(Tensor.numel, params))
+    blocks = [(n + BLOCK - 1) // BLOCK for n in numels]
+    for column, expected in zip(lists, (numels, numels, numels, blocks, blocks, [1] * len(numels))):
+        if list(map(Tensor.numel, column)) != expected:
+            raise ValueError(f"adamw8_step: {list(map(Tensor.numel, column))} elements instead of {expected}")
+    addresses = [list(map(Tensor.data_ptr, column)) for column in columns]
+    if len(set(addresses[0])) != len(numels) and len({a for a, n in zip(addresses[0], numels) if n}) != sum(map(bool, numels)):
         raise ValueError("adamw8_step: a parameter is given twice")
-    if len({step.data_ptr() for step in steps}) != len(steps):
+    if len(set(addresses[6])) != len(numels):
         raise ValueError("adamw8_step: a step counter is given twice")
-    with torch.cuda.device(device):
-        _native.adamw8_multi(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, steps, lr=lr,
-                             beta1=beta1, beta2=beta2, weight_decay=weight_decay, eps=eps, seed=seed,
-                             hyper_device=hyper_device)
+    if hyper_device is not None and (hyper_device.get_device() != device or hyper_device.dtype is not torch.float32
+                                     or hyper_device.numel() != 2 or not hyper_device.is_contiguous()):
+        raise ValueError("adamw8_step: hyper_device must be two contiguous float32 on the parameters' device")
+    _native.adamw8_multi(addresses, numels, grad_dtype, device=device, lr=lr, beta1=beta1, beta2=beta2,
+                         weight_decay=weight_decay, eps=eps, seed=seed, hyper_device=hyper_device)

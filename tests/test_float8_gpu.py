@@ -95,7 +95,8 @@ def test_quantize_leaves_neighbours_alone() -> None:
     q = torch.full((72, 160), 7, dtype=torch.uint8, device=DEV)
     qt = torch.full((140, 96), 7, dtype=torch.uint8, device=DEV)
     scales, scales_t = torch.full((3, 80), 7.0, device=DEV), torch.full((2, 140), 7.0, device=DEV)
-    _native.float8_quantize(x, tiles=False, q=q, scales=scales, qt=qt, scales_t=scales_t)
+    _native.float8_quantize(x.get_device(), x.data_ptr(), x.dtype, 70, 133, 133, False, q.data_ptr(), 160,
+                            scales.data_ptr(), 80, qt.data_ptr(), 96, scales_t.data_ptr(), 140)
     assert bool((q[70:] == 7).all()) and bool((q[:, 136:] == 7).all())
     assert bool((qt[133:] == 7).all()) and bool((qt[:, 72:] == 7).all())
     assert bool((scales[2:] == 7).all()) and bool((scales[:, 70:] == 7).all())
