@@ -66,16 +66,28 @@ __device__ __forceinline__ uint32_t mix(uint32_t h) {
   return h ^ (h >> 15);
 }
 
-// The 8-bit code, without its sign, of x >= 0: rounded down after `noise` / 2^16 of a step is added.  Codes of normal
-// numbers are the top bits of the fp32 ones.  Below the smallest normal number they are evenly spaced; adding that
-// number turns them into its mantissa.
-template <int kMantissa, int kBias, int kMost>
+// The 8-bit code of x >= 0, in the top byte and without its sign: rounded down after `noise` / 2^16 of a step is added.
+// Codes of normal numbers are the top bits of the fp32 ones; a shift brings them into the byte, and the difference of the
+// exponents' biases is 0x40000000 there in both formats.  The largest value of a block may come out a little above the format's:
+// the noise leaves room for 15 units in the last place below the next code.
+template <int kMantissa, int kBias>
+__device__ __forceinline__ uint32_t encode_normal(float x, uint32_t noise) {
+  constexpr int kDrop = 23 - kMantissa;
+  static_assert(((uint64_t(127 - kBias) << 23) << (24 - kDrop)) % (1ull << 32) == 0xC0000000u, "difference of the biases");
+  const uint32_t bits = noise * (1u << (kDrop - 16)) + __float_as_uint(x);
+  return bits * (1u << (24 - kDrop)) + 0x40000000u;
+}
+// Of any x: below the smallest normal number codes are evenly spaced, and adding that number turns them into its
+// mantissa.
+template <int kMantissa, int kBias>
 __device__ __forceinline__ uint32_t encode(float x, uint32_t noise) {
-  constexpr int kDrop = 23 - kMantissa, kFirst = (127 - kBias) << kMantissa;
   const float normal = __uint_as_float(uint32_t(128 - kBias) << 23);
   const bool low = x < normal;
-  const uint32_t bits = __float_as_uint(low ? x + normal : x) + (noise << (kDrop - 16));
-  return uint32_t(min(int(bits >> kDrop) - (low ? kFirst + (1 << kMantissa) : kFirst), kMost));
+  return encode_normal<kMantissa, kBias>(low ? x + normal : x, noise) - (low ? 1u << (24 + kMantissa) : 0u);
+}
+// The top bytes of four words.
+__device__ __forceinline__ uint32_t top_bytes(const uint32_t (&w)[4]) {
+  return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
 }
 
 __device__ __forceinline__ float2 halves(uint32_t h) {
@@ -114,47 +126,82 @@ struct Piece {
 };
 
 struct Factors {
-  float keep;         // 1 - lr * weight decay, as the factor that is subtracted: lr * weight decay
+  float decay;        // lr * weight decay
   float rate;         // lr / (1 - beta1^t)
   float inv_root2;    // 1 / sqrt(1 - beta2^t)
   float eps, beta1, omb1, beta2, omb2;
 };
 
-// Updates a piece; `words` are the four elements' noise.
-__device__ __forceinline__ void update(Piece& x, const Factors& f, const uint32_t (&words)[4]) {
-  float m[4], v[4];
-  decode_mean(x.m, m);
-  decode_square(x.v, v);
-  uint32_t m_top = 0, v_top = 0;
+// Updates a warp's pieces.  words(j, w) gives the noise of piece j's four elements.  Lane 2j of the warp is left with the
+// scale of piece j's first moment, lane 2j + 1 with that of the second.
+//
+// What bounds it: at 16 bytes an element and 6.5 TB/s an SM has about 85 instructions a lane and element.  The first version took 100
+// (39.4 M elements 141 us): each lane worked out each scale and its reciprocal, and each code went through the form that
+// holds for the smallest numbers too.  Those are now left to the pieces that have any (1 of 100 where gradients are
+// normal), and the scales to a lane each.
+template <typename Words>
+__device__ __forceinline__ float update(Piece (&x)[kUnroll], const Factors& f, int lane, Words&& words) {
+  float m[kUnroll][4], v[kUnroll][4];
+  float largest = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float g = x.g[i];
-    // every operation rounded by itself: two evaluations of the moments in fp32 are the same bit for bit, and a
-    // difference in the last bit, rounded to the next code, would be one of a tenth in the steps to come
-    m[i] = __fadd_rn(__fmul_rn(f.beta1, __fmul_rn(m[i], x.m_scale)), __fmul_rn(f.omb1, g));
-    v[i] = __fadd_rn(__fmul_rn(f.beta2, __fmul_rn(v[i], x.v_scale)), __fmul_rn(f.omb2, __fmul_rn(g, g)));
-    float root;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v[i]));
-    x.p[i] = fmaf(-f.keep, x.p[i], x.p[i]) - __fdividef(f.rate * m[i], fmaf(root, f.inv_root2, f.eps));
-    // as integers, magnitudes are in order, infinity and NaN above all numbers
-    m_top = max(m_top, __float_as_uint(m[i]) & 0x7FFFFFFFu);
-    v_top = max(v_top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-  }
-  const float m_largest = __uint_as_float(__reduce_max_sync(0xffffffffu, m_top));
-  const float v_largest = __uint_as_float(__reduce_max_sync(0xffffffffu, v_top));
-  const float nan = __uint_as_float(0x7FFFFFFFu);
-  x.m_scale = m_largest < INFINITY ? fmaxf(m_largest * (1.0f / kMeanMax), kSmallestScale) : nan;
-  x.v_scale = v_largest < INFINITY ? fmaxf(v_largest * (1.0f / kSquareMax), kSmallestScale) : nan;
-  const float m_inv = __frcp_rn(x.m_scale), v_inv = __frcp_rn(x.v_scale);
-  x.m = x.v = 0;
+  for (int j = 0; j < kUnroll; ++j) {
+    decode_mean(x[j].m, m[j]);
+    decode_square(x[j].v, v[j]);
+    uint32_t m_top = 0, v_top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t mean = encode<3, 7, 0x7E>(fabsf(m[i]) * m_inv, words[i] & 0xFFFFu) | ((__float_as_uint(m[i]) >> 24) & 0x80u);
-    uint32_t square = encode<2, 15, 0x7B>(v[i] * v_inv, words[i] >> 16);
-    if (v[i] > 0.0f) square = max(square, 1u);
-    x.m |= mean << (8 * i);
-    x.v |= square << (8 * i);
+    for (int i = 0; i < 4; ++i) {
+      const float g = x[j].g[i];
+      // every operation rounded by itself: two evaluations of the moments in fp32 are the same bit for bit, and a
+      // difference in the last bit, rounded to the next code, would be one of a tenth in the steps to come
+      m[j][i] = __fadd_rn(__fmul_rn(f.beta1, __fmul_rn(m[j][i], x[j].m_scale)), __fmul_rn(f.omb1, g));
+      v[j][i] = __fadd_rn(__fmul_rn(f.beta2, __fmul_rn(v[j][i], x[j].v_scale)), __fmul_rn(f.omb2, __fmul_rn(g, g)));
+      float root, inverse;
+      asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v[j][i]));
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root, f.inv_root2, f.eps)));
+      x[j].p[i] = fmaf(-f.rate * m[j][i], inverse, fmaf(-f.decay, x[j].p[i], x[j].p[i]));
+      // as integers, magnitudes are in order, infinity and NaN above all numbers
+      m_top = max(m_top, __float_as_uint(m[j][i]) & 0x7FFFFFFFu);
+      v_top = max(v_top, __float_as_uint(v[j][i]));
+    }
+    const float m_largest = __uint_as_float(__reduce_max_sync(0xffffffffu, m_top));
+    const float v_largest = __uint_as_float(__reduce_max_sync(0xffffffffu, v_top));
+    if ((lane >> 1) == j) largest = (lane & 1) != 0 ? v_largest : m_largest;
   }
+  const float scaled = largest * ((lane & 1) != 0 ? 1.0f / kSquareMax : 1.0f / kMeanMax);
+  const float scale = scaled < INFINITY ? fmaxf(scaled, kSmallestScale) : __uint_as_float(0x7FFFFFFFu);
+  const float inverse = __frcp_rn(scale);
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) {
+    const float m_inv = __shfl_sync(0xffffffffu, inverse, 2 * j), v_inv = __shfl_sync(0xffffffffu, inverse, 2 * j + 1);
+    uint32_t w[4], mean[4], square[4];
+    words(j, w);
+    float a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      a[i] = fabsf(m[j][i]) * m_inv;
+      b[i] = v[j][i] * v_inv;
+    }
+    const bool low = fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < 0x1p-6f || fminf(fminf(b[0], b[1]), fminf(b[2], b[3])) < 0x1p-14f;
+    if (!__any_sync(0xffffffffu, low)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mean[i] = encode_normal<3, 7>(a[i], w[i] & 0xFFFFu);
+        square[i] = encode_normal<2, 15>(b[i], w[i] >> 16);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        mean[i] = encode<3, 7>(a[i], w[i] & 0xFFFFu);
+        square[i] = encode<2, 15>(b[i], w[i] >> 16);
+        if (v[j][i] > 0.0f) square[i] = max(square[i], 1u << 24);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mean[i] = (mean[i] & 0x7FFFFFFFu) | (__float_as_uint(m[j][i]) & 0x80000000u);
+    x[j].m = top_bytes(mean);
+    x[j].v = top_bytes(square);
+  }
+  return scale;
 }
 
 template <typename G>
@@ -182,7 +229,7 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   const float step = *tab.step[lo];
   // 1 - beta^t without the cancellation of its first steps
   Factors f;
-  f.keep = lr * weight_decay;
+  f.decay = lr * weight_decay;
   f.rate = lr / -expm1f(step * hyper.log_beta1);
   f.inv_root2 = rsqrtf(-expm1f(step * hyper.log_beta2));
   f.eps = hyper.eps;
@@ -193,12 +240,10 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   const uint32_t key = step_key(step, hyper.seed);
   const bool vec = ((reinterpret_cast<uintptr_t>(p) | (reinterpret_cast<uintptr_t>(g) * (4 / sizeof(G)))) & 15u) == 0 &&
                    ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3u) == 0;
-  auto words_of = [&](long long e, uint32_t (&words)[4]) {
-    uint32_t h = uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i, h += 0x9E3779B1u) words[i] = mix(h);   // four elements never straddle 2^32
-  };
   Piece x[kUnroll];
+  // lane 2j, 2j + 1: the scales of block first + j
+  float* const scale_at = ((lane & 1) != 0 ? v_scale : m_scale) + first + (lane >> 1);
+  const bool has_scale = lane < 2 * kUnroll && (first + (lane >> 1)) * kBlock < n;
   if (vec && (first + kUnroll) * kBlock <= n) {
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
@@ -210,58 +255,59 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
       x[j].m_scale = m_scale[first + j];
       x[j].v_scale = v_scale[first + j];
     }
+    const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) {
+      const long long e = (first + j) * kBlock + 4 * lane;
+      uint32_t h = uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i, h += 0x9E3779B1u) w[i] = mix(h);   // four elements never straddle 2^32
+    });
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const long long e = (first + j) * kBlock + 4 * lane;
-      uint32_t words[4];
-      words_of(e, words);
-      update(x[j], f, words);
       Span<4>::store(p + e, x[j].p);
       __stcs(reinterpret_cast<unsigned int*>(m + e), x[j].m);
       __stcs(reinterpret_cast<unsigned int*>(v + e), x[j].v);
-      if (lane == 0) {
-        m_scale[first + j] = x[j].m_scale;
-        v_scale[first + j] = x[j].v_scale;
-      }
     }
+    if (has_scale) *scale_at = scale;
     return;
   }
-  // Tensors between 16-byte boundaries, and the last blocks: element by element.
-  for (int j = 0; j < kUnroll && (first + j) * kBlock < n; ++j) {
-    Piece y{};
-    const long long at = (first + j) * kBlock;
-    // lane l holds elements l, l + 32, l + 64, l + 96, so that neighbours read neighbours
+  // Tensors between 16-byte boundaries, and the last blocks: element by element.  Lane l holds elements l, l + 32, l + 64 and
+  // l + 96 of a block, so that neighbours read neighbours; what lies behind the tensor is zero.
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j) {
+    x[j] = Piece{};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const long long e = at + lane + 32 * i;
+      const long long e = (first + j) * kBlock + lane + 32 * i;
       if (e >= n) continue;
-      y.p[i] = p[e];
-      y.g[i] = to_float<G>(g[e]);
-      y.m |= uint32_t(m[e]) << (8 * i);
-      y.v |= uint32_t(v[e]) << (8 * i);
+      x[j].p[i] = p[e];
+      x[j].g[i] = to_float<G>(g[e]);
+      x[j].m |= uint32_t(m[e]) << (8 * i);
+      x[j].v |= uint32_t(v[e]) << (8 * i);
     }
-    y.m_scale = m_scale[first + j];
-    y.v_scale = v_scale[first + j];
-    uint32_t words[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long e = at + lane + 32 * i;
-      words[i] = mix(uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u));
-    }
-    update(y, f, words);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long e = at + lane + 32 * i;
-      if (e >= n) continue;
-      p[e] = y.p[i];
-      m[e] = uint8_t(y.m >> (8 * i));
-      v[e] = uint8_t(y.v >> (8 * i));
-    }
-    if (lane == 0) {
-      m_scale[first + j] = y.m_scale;
-      v_scale[first + j] = y.v_scale;
+    if ((first + j) * kBlock < n) {
+      x[j].m_scale = m_scale[first + j];
+      x[j].v_scale = v_scale[first + j];
     }
   }
+  const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long e = (first + j) * kBlock + lane + 32 * i;
+      w[i] = mix(uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u));
+    }
+  });
+#pragma unroll
+  for (int j = 0; j < kUnroll; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long e = (first + j) * kBlock + lane + 32 * i;
+      if (e >= n) continue;
+      p[e] = x[j].p[i];
+      m[e] = uint8_t(x[j].m >> (8 * i));
+      v[e] = uint8_t(x[j].v >> (8 * i));
+    }
+  if (has_scale) *scale_at = scale;
 }
 
 template <typename G>
@@ -290,7 +336,7 @@ extern "C" int dionw_adamw8_multi(void* const* params, const void* const* grads,
   Hyper hyper;
   hyper.lr = lr;
   hyper.weight_decay = weight_decay;
-  hyper.eps = eps;
+  hyper.eps = std::fmax(eps, kSmallestScale);   // of a normal number the approximate reciprocal is finite
   hyper.beta1 = float(beta1);
   hyper.one_minus_beta1 = float(1.0 - beta1);
   hyper.log_beta1 = float(std::log(beta1));
