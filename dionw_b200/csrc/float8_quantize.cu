@@ -36,6 +36,7 @@ struct QuantizeParams {
   float* scales_t;     // the same of the transposed matrix
   int64_t ldst;
   int rows, cols;
+  int tiles_x, tiles;  // of 128 x 128
   int vec;             // 16-byte loads
 };
 
@@ -138,12 +139,17 @@ quantize_kernel(const QuantizeParams p) {
   __shared__ uint2 turned[kBlock][16];     // the transposed codes of eight rows: unit u of column c at u ^ (c / 8)
   after_previous();
   const int group = threadIdx.x >> 4, lane16 = threadIdx.x & 15, warp = threadIdx.x >> 5;
-  const int tile_row = int(blockIdx.y) * kBlock, tile_col = int(blockIdx.x) * kBlock;
-  const int row0 = tile_row + group * kRows, col0 = tile_col + lane16 * 8;
   Eight<T> x[kRows];
+  auto load = [&](int tile) {
+    const int ty = tile / p.tiles_x, row0 = ty * kBlock + group * kRows, col0 = (tile - ty * p.tiles_x) * kBlock + lane16 * 8;
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) load8<T>(p, row0 + r, col0, x[r]);
-
+    for (int r = 0; r < kRows; ++r) load8<T>(p, row0 + r, col0, x[r]);
+  };
+  load(blockIdx.x);
+  for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
+  const int ty = tile / p.tiles_x, tx = tile - ty * p.tiles_x;
+  const int tile_row = ty * kBlock, tile_col = tx * kBlock;
+  const int row0 = tile_row + group * kRows, col0 = tile_col + lane16 * 8;
   float inverse = 1.0f;                    // tiles: of all values
   if constexpr (kTiles) {
     uint32_t top = 0;
@@ -161,8 +167,8 @@ quantize_kernel(const QuantizeParams p) {
     }
     const float scale = scale_of(top, inverse);
     if (threadIdx.x == 0) {
-      if (p.q != nullptr) p.scales[int64_t(blockIdx.y) * p.lds + blockIdx.x] = scale;
-      if (p.qt != nullptr) p.scales_t[int64_t(blockIdx.x) * p.ldst + blockIdx.y] = scale;
+      if (p.q != nullptr) p.scales[int64_t(ty) * p.lds + tx] = scale;
+      if (p.qt != nullptr) p.scales_t[int64_t(tx) * p.ldst + ty] = scale;
     }
   } else if (p.qt != nullptr) {
     uint32_t top[kWords];
@@ -191,7 +197,7 @@ quantize_kernel(const QuantizeParams p) {
 #pragma unroll
         for (int step = 8; step > 0; step >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
         const float scale = scale_of(top, inverse);
-        if (lane16 == 0 && row < p.rows) p.scales[int64_t(blockIdx.x) * p.lds + row] = scale;
+        if (lane16 == 0 && row < p.rows) p.scales[int64_t(tx) * p.lds + row] = scale;
       }
       float v[8];
 #pragma unroll
@@ -202,7 +208,11 @@ quantize_kernel(const QuantizeParams p) {
             make_uint2(to_codes(v[0], v[1], v[2], v[3]), to_codes(v[4], v[5], v[6], v[7]));
     }
   }
-  if (p.qt == nullptr) return;
+  if (p.qt == nullptr) {
+    if (tile + int(gridDim.x) < p.tiles) load(tile + int(gridDim.x));
+    if (kTiles) __syncthreads();           // the maxima are read
+    continue;
+  }
   if constexpr (!kTiles) {
     __syncthreads();
     if (threadIdx.x < kBlock) {
@@ -212,7 +222,7 @@ quantize_kernel(const QuantizeParams p) {
       for (int i = 1; i < 16; ++i) top = Eight<T>::larger(top, column_part[i][word]);
       float inv;
       const float scale = scale_of(Eight<T>::of_column(top, c), inv);
-      if (tile_col + c < p.cols) p.scales_t[int64_t(blockIdx.y) * p.ldst + tile_col + c] = scale;
+      if (tile_col + c < p.cols) p.scales_t[int64_t(ty) * p.ldst + tile_col + c] = scale;
       column_inverse[c] = inv;
     }
     __syncthreads();
@@ -233,6 +243,7 @@ quantize_kernel(const QuantizeParams p) {
     unit[group & 1] = to_codes(x[0].value(c) * column[c], x[1].value(c) * column[c], x[2].value(c) * column[c],
                                x[3].value(c) * column[c]);
   }
+  if (tile + int(gridDim.x) < p.tiles) load(tile + int(gridDim.x));
   __syncthreads();
   const int out_col = tile_row + lane16 * 8;   // of the transposed matrix
 #pragma unroll
@@ -241,13 +252,13 @@ quantize_kernel(const QuantizeParams p) {
     if (row < p.cols && out_col < p.rows)
       *reinterpret_cast<uint2*>(p.qt + int64_t(row) * p.ldqt + out_col) = turned[c][lane16 ^ (c >> 3)];
   }
+  }
 }
 
 template <bool kTiles>
 int launch(const QuantizeParams& p, int dtype, cudaStream_t stream) {
-  const dim3 grid(unsigned((p.cols + kBlock - 1) / kBlock), unsigned((p.rows + kBlock - 1) / kBlock));
   cudaLaunchConfig_t config = {};
-  config.gridDim = grid;
+  config.gridDim = dim3(unsigned(p.tiles < 2 * sm_count() ? p.tiles : 2 * sm_count()));
   config.blockDim = dim3(kThreads);
   config.stream = stream;
   cudaLaunchAttribute attribute;
@@ -274,7 +285,7 @@ extern "C" int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int
   DIONW_REQUIRE(rows >= 0 && cols >= 0 && rows <= 0x7FFFFF80ll && cols <= 0x7FFFFF80ll, "float8_quantize: bad shape %lld x %lld",
                 (long long)rows, (long long)cols);
   const int64_t row_blocks = (rows + kBlock - 1) / kBlock, col_blocks = (cols + kBlock - 1) / kBlock;
-  DIONW_REQUIRE(row_blocks <= 65535, "float8_quantize: at most %d rows", 65535 * kBlock);
+  DIONW_REQUIRE(row_blocks * col_blocks < (1ll << 30), "float8_quantize: too large a matrix, %lld x %lld", (long long)rows, (long long)cols);
   if (rows == 0 || cols == 0) return DIONW_OK;
   DIONW_REQUIRE(x != nullptr && ldx >= cols, "float8_quantize: leading dimension %lld of %lld columns", (long long)ldx,
                 (long long)cols);
@@ -296,6 +307,8 @@ extern "C" int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int
   p.ldst = ldst;
   p.rows = int(rows);
   p.cols = int(cols);
+  p.tiles_x = int(col_blocks);
+  p.tiles = int(row_blocks * col_blocks);
   const int64_t size = dtype == DIONW_F32 ? 4 : 2;
   p.vec = aligned16(x) && (rows == 1 || (ldx * size) % 16 == 0);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
