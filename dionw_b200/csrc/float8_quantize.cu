@@ -87,10 +87,18 @@ struct Eight {
   }
   static __device__ __forceinline__ uint32_t of_word(uint32_t word) { return as_float(max(word & 0xFFFFu, word >> 16)); }
   static __device__ __forceinline__ uint32_t of_column(uint32_t word, int c) { return as_float(c & 1 ? word >> 16 : word & 0xFFFFu); }
-  __device__ __forceinline__ float value(int i) const {
-    const uint32_t word = w[i >> 1];
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? word & 0xFFFF0000u : word << 16);
-    return __half2float(__ushort_as_half(uint16_t(i & 1 ? word >> 16 : word & 0xFFFFu)));
+  // The word's two values, times a power of two each.
+  __device__ __forceinline__ float2 scaled(int word, float fa, float fb) const {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+      // exact in bf16 too: what becomes too small for a normal number is far below the smallest code
+      const uint32_t factors = __byte_perm(__float_as_uint(fa), __float_as_uint(fb), 0x7632);
+      const __nv_bfloat162 product = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[word]),
+                                             *reinterpret_cast<const __nv_bfloat162*>(&factors));
+      const uint32_t bits = *reinterpret_cast<const uint32_t*>(&product);
+      return make_float2(__uint_as_float(bits << 16), __uint_as_float(bits & 0xFFFF0000u));
+    }
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[word]));
+    return make_float2(v.x * fa, v.y * fb);
   }
 };
 template <>
@@ -111,7 +119,9 @@ struct Eight<float> {
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
   static __device__ __forceinline__ uint32_t of_word(uint32_t word) { return word; }
   static __device__ __forceinline__ uint32_t of_column(uint32_t word, int) { return word; }
-  __device__ __forceinline__ float value(int i) const { return v[i]; }
+  __device__ __forceinline__ float2 scaled(int pair, float fa, float fb) const {
+    return make_float2(v[2 * pair] * fa, v[2 * pair + 1] * fb);
+  }
 };
 
 template <typename T>
@@ -147,111 +157,134 @@ quantize_kernel(const QuantizeParams p) {
   };
   load(blockIdx.x);
   for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
-  const int ty = tile / p.tiles_x, tx = tile - ty * p.tiles_x;
-  const int tile_row = ty * kBlock, tile_col = tx * kBlock;
-  const int row0 = tile_row + group * kRows, col0 = tile_col + lane16 * 8;
-  float inverse = 1.0f;                    // tiles: of all values
-  if constexpr (kTiles) {
-    uint32_t top = 0;
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) top = Eight<T>::larger(top, x[r].magnitude(i));
-    top = __reduce_max_sync(0xffffffffu, Eight<T>::of_word(top));
-    if ((threadIdx.x & 31) == 0) tile_part[warp] = top;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kThreads / 32; i += 4) {
-      const uint4 four = *reinterpret_cast<const uint4*>(&tile_part[i]);
-      top = max(top, max(max(four.x, four.y), max(four.z, four.w)));
-    }
-    const float scale = scale_of(top, inverse);
-    if (threadIdx.x == 0) {
-      if (p.q != nullptr) p.scales[int64_t(ty) * p.lds + tx] = scale;
-      if (p.qt != nullptr) p.scales_t[int64_t(tx) * p.ldst + ty] = scale;
-    }
-  } else if (p.qt != nullptr) {
-    uint32_t top[kWords];
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) {
-      top[i] = x[0].magnitude(i);
-#pragma unroll
-      for (int r = 1; r < kRows; ++r) top[i] = Eight<T>::larger(top[i], x[r].magnitude(i));
-      top[i] = Eight<T>::larger(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
-    }
-    if ((threadIdx.x & 16) == 0) {
-#pragma unroll
-      for (int i = 0; i < kWords; i += 4)
-        *reinterpret_cast<uint4*>(&column_part[warp][lane16 * kWords + i]) = make_uint4(top[i], top[i + 1], top[i + 2], top[i + 3]);
-    }
-  }
-  if (p.q != nullptr) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      const int row = row0 + r;
-      if constexpr (!kTiles) {
-        uint32_t word = x[r].magnitude(0);
-#pragma unroll
-        for (int i = 1; i < kWords; ++i) word = Eight<T>::larger(word, x[r].magnitude(i));
-        uint32_t top = Eight<T>::of_word(word);
-#pragma unroll
-        for (int step = 8; step > 0; step >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, step));
-        const float scale = scale_of(top, inverse);
-        if (lane16 == 0 && row < p.rows) p.scales[int64_t(tx) * p.lds + row] = scale;
-      }
-      float v[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) v[c] = x[r].value(c) * inverse;
-      // rows have room up to a multiple of 16 elements: codes behind the last column are zero
-      if (row < p.rows && col0 < p.cols)
-        *reinterpret_cast<uint2*>(p.q + int64_t(row) * p.ldq + col0) =
-            make_uint2(to_codes(v[0], v[1], v[2], v[3]), to_codes(v[4], v[5], v[6], v[7]));
-    }
-  }
-  if (p.qt == nullptr) {
-    if (tile + int(gridDim.x) < p.tiles) load(tile + int(gridDim.x));
-    if (kTiles) __syncthreads();           // the maxima are read
-    continue;
-  }
-  if constexpr (!kTiles) {
-    __syncthreads();
-    if (threadIdx.x < kBlock) {
-      const int c = threadIdx.x, word = kWords == 8 ? c : c >> 1;
-      uint32_t top = column_part[0][word];
-#pragma unroll
-      for (int i = 1; i < 16; ++i) top = Eight<T>::larger(top, column_part[i][word]);
-      float inv;
-      const float scale = scale_of(Eight<T>::of_column(top, c), inv);
-      if (tile_col + c < p.cols) p.scales_t[int64_t(ty) * p.ldst + tile_col + c] = scale;
-      column_inverse[c] = inv;
-    }
-    __syncthreads();
-  }
-  float column[8];
-#pragma unroll
-  for (int c = 0; c < 8; c += 4) {
+    const int ty = tile / p.tiles_x, tx = tile - ty * p.tiles_x;
+    const int tile_row = ty * kBlock, tile_col = tx * kBlock;
+    const int row0 = tile_row + group * kRows, col0 = tile_col + lane16 * 8;
+    float inverse = 1.0f;                    // tiles: of all values
     if constexpr (kTiles) {
-      column[c] = column[c + 1] = column[c + 2] = column[c + 3] = inverse;
-    } else {
-      const float4 f = *reinterpret_cast<const float4*>(&column_inverse[lane16 * 8 + c]);
-      column[c] = f.x; column[c + 1] = f.y; column[c + 2] = f.z; column[c + 3] = f.w;
+      uint32_t top = 0;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) top = Eight<T>::larger(top, x[r].magnitude(i));
+      top = __reduce_max_sync(0xffffffffu, Eight<T>::of_word(top));
+      if ((threadIdx.x & 31) == 0) tile_part[warp] = top;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; i += 4) {
+        const uint4 four = *reinterpret_cast<const uint4*>(&tile_part[i]);
+        top = max(top, max(max(four.x, four.y), max(four.z, four.w)));
+      }
+      const float scale = scale_of(top, inverse);
+      if (threadIdx.x == 0) {
+        if (p.q != nullptr) p.scales[int64_t(ty) * p.lds + tx] = scale;
+        if (p.qt != nullptr) p.scales_t[int64_t(tx) * p.ldst + ty] = scale;
+      }
+    } else if (p.qt != nullptr) {
+      uint32_t top[kWords];
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        top[i] = x[0].magnitude(i);
+#pragma unroll
+        for (int r = 1; r < kRows; ++r) top[i] = Eight<T>::larger(top[i], x[r].magnitude(i));
+        top[i] = Eight<T>::larger(top[i], __shfl_xor_sync(0xffffffffu, top[i], 16));
+      }
+      if ((threadIdx.x & 16) == 0) {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 4)
+          *reinterpret_cast<uint4*>(&column_part[warp][lane16 * kWords + i]) = make_uint4(top[i], top[i + 1], top[i + 2], top[i + 3]);
+      }
     }
-  }
+    if (p.q != nullptr) {
+      float row_inverse[kRows];
+      if constexpr (!kTiles) {
+        // The rows' maxima over 16 lanes; lane r of them then works out row r's scale.
+        uint32_t top[kRows];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t* unit = reinterpret_cast<uint32_t*>(&turned[lane16 * 8 + c][(group >> 1) ^ lane16]);
-    unit[group & 1] = to_codes(x[0].value(c) * column[c], x[1].value(c) * column[c], x[2].value(c) * column[c],
-                               x[3].value(c) * column[c]);
-  }
-  if (tile + int(gridDim.x) < p.tiles) load(tile + int(gridDim.x));
-  __syncthreads();
-  const int out_col = tile_row + lane16 * 8;   // of the transposed matrix
+        for (int r = 0; r < kRows; ++r) {
+          uint32_t word = x[r].magnitude(0);
 #pragma unroll
-  for (int i = 0; i < kBlock / (kThreads / 16); ++i) {
-    const int c = group + (kThreads / 16) * i, row = tile_col + c;
-    if (row < p.cols && out_col < p.rows)
-      *reinterpret_cast<uint2*>(p.qt + int64_t(row) * p.ldqt + out_col) = turned[c][lane16 ^ (c >> 3)];
-  }
+          for (int i = 1; i < kWords; ++i) word = Eight<T>::larger(word, x[r].magnitude(i));
+          top[r] = word;
+        }
+        if constexpr (kWords == 4) {   // two rows to a word
+#pragma unroll
+          for (int r = 0; r < kRows; r += 2)
+            top[r / 2] = __vmaxu2(__byte_perm(top[r], top[r + 1], 0x5410), __byte_perm(top[r], top[r + 1], 0x7632));
+        }
+        constexpr int kTops = kWords == 4 ? kRows / 2 : kRows;
+#pragma unroll
+        for (int step = 8; step > 0; step >>= 1)
+#pragma unroll
+          for (int i = 0; i < kTops; ++i) top[i] = Eight<T>::larger(top[i], __shfl_xor_sync(0xffffffffu, top[i], step));
+        uint32_t mine;
+        if constexpr (kWords == 4) mine = Eight<T>::of_column(lane16 & 2 ? top[1] : top[0], lane16);
+        else mine = lane16 & 2 ? (lane16 & 1 ? top[3] : top[2]) : (lane16 & 1 ? top[1] : top[0]);
+        float inv;
+        const float scale = scale_of(mine, inv);
+        if (lane16 < kRows && row0 + lane16 < p.rows) p.scales[int64_t(tx) * p.lds + row0 + lane16] = scale;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) row_inverse[r] = __shfl_sync(0xffffffffu, inv, r, 16);
+      }
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float f = kTiles ? inverse : row_inverse[r];
+        float2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = x[r].scaled(i, f, f);
+        // rows have room up to a multiple of 16 elements: codes behind the last column are zero
+        if (row0 + r < p.rows && col0 < p.cols)
+          *reinterpret_cast<uint2*>(p.q + int64_t(row0 + r) * p.ldq + col0) =
+              make_uint2(to_codes(v[0].x, v[0].y, v[1].x, v[1].y), to_codes(v[2].x, v[2].y, v[3].x, v[3].y));
+      }
+    }
+    if (p.qt == nullptr) {
+      if (tile + int(gridDim.x) < p.tiles) load(tile + int(gridDim.x));
+      if (kTiles) __syncthreads();           // the maxima are read
+      continue;
+    }
+    if constexpr (!kTiles) {
+      __syncthreads();
+      if (threadIdx.x < kBlock) {
+        const int c = threadIdx.x, word = kWords == 8 ? c : c >> 1;
+        uint32_t top = column_part[0][word];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = Eight<T>::larger(top, column_part[i][word]);
+        float inv;
+        const float scale = scale_of(Eight<T>::of_column(top, c), inv);
+        if (tile_col + c < p.cols) p.scales_t[int64_t(ty) * p.ldst + tile_col + c] = scale;
+        column_inverse[c] = inv;
+      }
+      __syncthreads();
+    }
+    float column[8];
+#pragma unroll
+    for (int c = 0; c < 8; c += 4) {
+      if constexpr (kTiles) {
+        column[c] = column[c + 1] = column[c + 2] = column[c + 3] = inverse;
+      } else {
+        const float4 f = *reinterpret_cast<const float4*>(&column_inverse[lane16 * 8 + c]);
+        column[c] = f.x; column[c + 1] = f.y; column[c + 2] = f.z; column[c + 3] = f.w;
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 8; c += 2) {
+      float2 v[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) v[r] = x[r].scaled(c / 2, column[c], column[c + 1]);
+      uint32_t* unit = reinterpret_cast<uint32_t*>(&turned[lane16 * 8 + c][(group >> 1) ^ lane16]) + (group & 1);
+      unit[0] = to_codes(v[0].x, v[1].x, v[2].x, v[3].x);
+      unit[kBlock / 4] = to_codes(v[0].y, v[1].y, v[2].y, v[3].y);   // the next column
+    }
+    if (tile + int(gridDim.x) < p.tiles) load(tile + int(gridDim.x));
+    __syncthreads();
+    const int out_col = tile_row + lane16 * 8;   // of the transposed matrix
+#pragma unroll
+    for (int i = 0; i < kBlock / (kThreads / 16); ++i) {
+      const int c = group + (kThreads / 16) * i, row = tile_col + c;
+      if (row < p.cols && out_col < p.rows)
+        *reinterpret_cast<uint2*>(p.qt + int64_t(row) * p.ldqt + out_col) = turned[c][lane16 ^ (c >> 3)];
+    }
   }
 }
 
