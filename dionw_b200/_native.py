@@ -510,16 +510,17 @@ def adamw_multi(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         _ptr(hyper_device), _stream(params[0])))
 
 
-def adamw8_multi(addresses: Sequence[Sequence[int]], numels: Sequence[int], grad_dtype: torch.dtype, *, device: int,
+def adamw8_multi(addresses: Sequence[int], numels: Sequence[int], grad_dtype: torch.dtype, *, device: int,
                  lr: float, beta1: float, beta2: float, weight_decay: float, eps: float, seed: int,
                  hyper_device: Tensor | None = None) -> None:
-    """``adamw_multi`` with 8-bit moments.  ``addresses``: those of the parameters, gradients (of one dtype), the two
-    moments, their scales and the step counters, on device number ``device``; ``seed`` below 2**32."""
-    tables = [array("Q", column) for column in addresses]
-    counts = array("q", numels)
-    p, g, m, v, m_scale, v_scale, steps = (table.buffer_info()[0] for table in tables)
+    """``adamw_multi`` with 8-bit moments.  ``addresses``: those of the parameters, then of the gradients (of one dtype),
+    the two moments, their scales and the step counters, on device number ``device``; ``seed`` below 2**32."""
+    table, counts = array("Q", addresses), array("q", numels)
+    n = len(counts)
+    base = table.buffer_info()[0]
+    p, g, m, v, m_scale, v_scale, steps = range(base, base + 56 * n, 8 * n)
     on_device(device, library().dionw_adamw8_multi, p, g, _DTYPE_CODE[grad_dtype], m, v, m_scale, v_scale, steps,
-              counts.buffer_info()[0], len(counts), lr, beta1, beta2, weight_decay, eps, seed, _ptr(hyper_device))
+              counts.buffer_info()[0], n, lr, beta1, beta2, weight_decay, eps, seed, _ptr(hyper_device))
 
 
 def ema_multi(shadows: Sequence[Tensor], sources: Sequence[Tensor], *, weight: float, first: bool) -> None:

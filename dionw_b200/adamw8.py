@@ -54,7 +54,6 @@ def dequantize_moments(entry: dict[str, Any]) -> tuple[Tensor, Tensor]:
             values(entry[EXP_AVG_SQ_STATE], entry[EXP_AVG_SQ_SCALE_STATE]))
 
 
-@torch.no_grad()
 def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequence[Tensor],
                 exp_avg_sq: Sequence[Tensor], exp_avg_scale: Sequence[Tensor], exp_avg_sq_scale: Sequence[Tensor],
                 steps: Sequence[Tensor], *, lr: float, betas: tuple[float, float] = (0.9, 0.95),
@@ -95,22 +94,24 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         raise ValueError(f"adamw8_step runs on CUDA devices, got a parameter on {params[0].device}")
     if grad_dtype not in _GRAD_DTYPES:
         raise TypeError(f"adamw8_step takes float32, float16 or bfloat16 gradients, got {grad_dtype}")
-    # Hundreds of tensors a step: each question goes to a whole list at a time.
-    columns = (params, *lists)
-    for column, dtype in zip(columns, (torch.float32, grad_dtype, MEAN_DTYPE, SQUARE_DTYPE) + (torch.float32,) * 3):
-        if set(map(_dtype_of, column)) != {dtype}:
-            raise TypeError(f"adamw8_step: expected {dtype}, got {set(map(_dtype_of, column))}")
-        if set(map(Tensor.get_device, column)) != {device} or not all(map(Tensor.is_contiguous, column)):
-            raise ValueError("adamw8_step needs contiguous tensors of one device")
+    # Hundreds of tensors a step: each question goes to all of them at once.
+    n = len(params)
+    tensors = [*params, *grads, *exp_avg, *exp_avg_sq, *exp_avg_scale, *exp_avg_sq_scale, *steps]
+    dtypes = [torch.float32] * n + [grad_dtype] * n + [MEAN_DTYPE] * n + [SQUARE_DTYPE] * n + [torch.float32] * (3 * n)
+    if list(map(_dtype_of, tensors)) != dtypes:
+        raise TypeError(
+            f"adamw8_step needs float32 parameters, scales and step counters, {grad_dtype} gradients, {MEAN_DTYPE} and "
+            f"{SQUARE_DTYPE} moments, got {sorted(set(map(str, map(_dtype_of, tensors))))}")
+    if set(map(Tensor.get_device, tensors)) != {device} or not all(map(Tensor.is_contiguous, tensors)):
+        raise ValueError("adamw8_step needs contiguous tensors of one device")
     numels = list(map(Tensor.numel, params))
-    blocks = [(n + BLOCK - 1) // BLOCK for n in numels]
-    for column, expected in zip(lists, (numels, numels, numels, blocks, blocks, [1] * len(numels))):
-        if list(map(Tensor.numel, column)) != expected:
-            raise ValueError(f"adamw8_step: {list(map(Tensor.numel, column))} elements instead of {expected}")
-    addresses = [list(map(Tensor.data_ptr, column)) for column in columns]
-    if len(set(addresses[0])) != len(numels) and len({a for a, n in zip(addresses[0], numels) if n}) != sum(map(bool, numels)):
+    blocks = [(numel + BLOCK - 1) // BLOCK for numel in numels]
+    if list(map(Tensor.numel, tensors[n:])) != numels * 3 + blocks * 2 + [1] * n:
+        raise ValueError("adamw8_step: gradients, moments or scales do not have the sizes that their parameters need")
+    addresses = list(map(Tensor.data_ptr, tensors))
+    if len(set(addresses[:n])) != n and len({a for a, k in zip(addresses, numels) if k}) != sum(map(bool, numels)):
         raise ValueError("adamw8_step: a parameter is given twice")
-    if len(set(addresses[6])) != len(numels):
+    if len(set(addresses[6 * n:])) != n:
         raise ValueError("adamw8_step: a step counter is given twice")
     if hyper_device is not None and (hyper_device.get_device() != device or hyper_device.dtype is not torch.float32
                                      or hyper_device.numel() != 2 or not hyper_device.is_contiguous()):

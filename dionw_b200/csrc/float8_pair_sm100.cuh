@@ -17,8 +17,8 @@ namespace pair {
 
 constexpr int kPairM = 256, kPairN = 256;
 constexpr int kThreads = 384;            // warp 0: TMA, warp 1: MMA + TMEM owner, warps 4-11: sums and output
-// Registers: 384 threads are launched with 168 each; 128 * 56 + 256 * 224 = 384 * 168.
-constexpr int kHelperRegisters = 56, kSumRegisters = 224;
+// Registers: 384 threads are launched with 168 each; 128 * 40 + 256 * 232 = 384 * 168.
+constexpr int kHelperRegisters = 40, kSumRegisters = 232;
 constexpr int kStages = 5;
 constexpr int kColumns = kPairN / 2;     // of a summing warp
 constexpr uint32_t kStageBytes = 2 * kABytes;          // 128 rows of A, 128 of B
@@ -160,14 +160,14 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     uint8_t* stage_out = staging + (warp - 4) * 32 * 128;
     const uint32_t tmem_mine = tmem_base + uint32_t(half * kColumns) + (uint32_t(sub * 32) << 16);
     const uint32_t leader_empty = peer_address(acc_empty, 0);
-    Queue<kRowScales> queue(queues + (warp - 4) * Queue<kRowScales>::kBytes, lane);
+    Queue<kRowScales> queue(queues + (warp - 4) * Queue<kRowScales>::kBytes);
     const int row_in_tile = int(rank) * kBM + sub * 32, col_in_tile = half * kColumns;
     uint32_t it = 0;
     bool ok = true;
     int tm, tn;
     if (first_tile < total_tiles) {
       tile_at(first_tile, p, tm, tn);
-      queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks);
+      queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks, lane);
     }
     for (int t = first_tile; t < total_tiles; t += pairs) {
       uint64_t sum[kColumns / 2];
@@ -175,20 +175,21 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       for (int c = 0; c < kColumns / 2; ++c) sum[c] = 0;
       for (int kb = 0; kb < k_blocks; ++kb, ++it) {
         const uint32_t acc = it & 1u;
-        const float* slot = queue.take();
         if (!warp_wait(&acc_full[acc], (it >> 1) & 1u)) { ok = false; break; }
         tc_fence_after();
-        add_block<kColumns, 16, kRowScales>(tmem_mine + acc * uint32_t(kPairN), slot, lane, sum, [&] {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
-        });
+        add_block<kColumns, kRowScales ? 8 : 16, kRowScales>(
+            tmem_mine + acc * uint32_t(kPairN), lane, sum, [&] { return queue.take(p, k_blocks - 1 - kb, lane); },
+            [&] {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
+            });
       }
       if (!ok) break;
       const int row0 = tm * kPairM + row_in_tile, col0 = tn * kPairN + col_in_tile;
       if (t + pairs < total_tiles) {   // the next tile's first scales come while this one's sums go out
         tile_at(t + pairs, p, tm, tn);
-        queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks);
+        queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks, lane);
       }
       write_sums<T, kColumns>(p, stage_out, row0, col0, lane, [&](int c) {
         const float2 f = apart(sum[c / 2]);

@@ -106,12 +106,16 @@ __device__ __forceinline__ void tmem_load<32>(uint32_t taddr, uint32_t* v) {
 }
 // The registers pass through the wait, so that no use of them can be moved in front of it.
 template <int kCount>
-__device__ __forceinline__ void tmem_wait(uint32_t* v) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void tmem_pass(uint32_t* v) {
 #pragma unroll
   for (int i = 0; i < kCount; i += 8)
     asm volatile("" : "+r"(v[i]), "+r"(v[i + 1]), "+r"(v[i + 2]), "+r"(v[i + 3]), "+r"(v[i + 4]), "+r"(v[i + 5]),
                       "+r"(v[i + 6]), "+r"(v[i + 7]));
+}
+template <int kCount>
+__device__ __forceinline__ void tmem_wait(uint32_t* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  tmem_pass<kCount>(v);
 }
 
 template <typename T>
@@ -227,71 +231,61 @@ __device__ __forceinline__ void write_sums(const Params& p, uint8_t* stage, int 
 // 8192 x 14336 x 4096 on SM pairs took 590 us with it, 466 without any scales.)
 template <int kColumnScales, int kDepth>
 struct ScaleQueue {
+  static_assert((kDepth & (kDepth - 1)) == 0, "a power of two");
   static constexpr int kFloats = 32 + (kColumnScales == 0 ? 4 : kColumnScales);
   static constexpr uint32_t kBytes = kDepth * kFloats * 4;
-  static constexpr int kCopies = (kColumnScales + 31) / 32;
 
   float* slots;
   const float* row_at;         // of the next block to fetch
   const float* column_at;
-  int64_t row_step, column_step, column_apart;
-  int left;                    // blocks to fetch
   int columns_there;           // of this warp, from its first one
   bool row_there;
-  int lane;
-  uint32_t next_in, next_out;
+  uint32_t taken;              // blocks, of all tiles
 
-  __device__ __forceinline__ ScaleQueue(void* at, int lane_)
-      : slots(static_cast<float*>(at)), lane(lane_), next_in(0), next_out(0) {}
+  __device__ __forceinline__ explicit ScaleQueue(void* at) : slots(static_cast<float*>(at)), taken(0) {}
 
-  __device__ __forceinline__ void fetch() {
-    if (left > 0) {
-      float* slot = slots + next_in * kFloats;
+  // Block taken + ahead of the queue, where the tile has it.
+  __device__ __forceinline__ void fetch(const Params& p, uint32_t ahead, bool more, int lane) {
+    if (more) {
+      float* slot = slots + ((taken + ahead) & (kDepth - 1)) * kFloats;
       copy4(slot + lane, row_at, row_there);
-      row_at += row_there ? row_step : 0;
       if constexpr (kColumnScales == 0) {
         if (lane == 0) copy4(slot + 32, column_at, columns_there > 0);
       } else {
 #pragma unroll
-        for (int i = 0; i < kCopies; ++i) {
+        for (int i = 0; i < (kColumnScales + 31) / 32; ++i) {
           const int c = 32 * i + lane;
           const bool there = c < columns_there;
-          if (kColumnScales % 32 == 0 || c < kColumnScales) copy4(slot + 32 + c, there ? column_at + i * column_apart : row_at, there);
+          if (kColumnScales % 32 == 0 || c < kColumnScales)
+            copy4(slot + 32 + c, there ? column_at + i * 32 * p.b.row_stride : p.b.base, there);
         }
       }
-      column_at += column_step;
-      --left;
+      if (row_there) row_at += p.a.block_stride;
+      if (columns_there > 0) column_at += p.b.block_stride;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
-    next_in = next_in + 1 == kDepth ? 0 : next_in + 1;
   }
 
   // The first blocks of a tile whose rows and columns start at row0 and col0 for this warp.
-  __device__ __forceinline__ void start(const Params& p, int row0, int col0, int blocks) {
+  __device__ __forceinline__ void start(const Params& p, int row0, int col0, int blocks, int lane) {
     const int row = row0 + lane;
     row_there = row < p.m;
     row_at = p.a.base + (row_there ? int64_t(row >> p.a.shift) * p.a.row_stride : 0);
-    row_step = p.a.block_stride;
     columns_there = p.n - col0;
     const int column = kColumnScales == 0 ? col0 : col0 + lane;
     column_at = p.b.base + (columns_there > 0 ? int64_t(column >> p.b.shift) * p.b.row_stride : 0);
-    column_apart = 32 * p.b.row_stride;
-    column_step = columns_there > 0 ? p.b.block_stride : 0;
-    left = blocks;
-    next_out = next_in;
     __syncwarp();              // nobody reads the last tile's any more
 #pragma unroll
-    for (int i = 0; i < kDepth - 1; ++i) fetch();
+    for (int i = 0; i < kDepth - 1; ++i) fetch(p, i, i < blocks, lane);
   }
 
-  // The slot of the next block, in the order of fetching; the one before it is fetched into.
-  __device__ __forceinline__ const float* take() {
+  // The scales of the next block, in the order of fetching; `after` blocks of the tile follow it.  The slot of the block
+  // before is fetched into.
+  __device__ __forceinline__ const float* take(const Params& p, int after, int lane) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 2) : "memory");
     __syncwarp();              // every lane's copies are there, and the slot before has been read
-    fetch();
-    const float* slot = slots + next_out * kFloats;
-    next_out = next_out + 1 == kDepth ? 0 : next_out + 1;
-    return slot;
+    fetch(p, kDepth - 1, after >= kDepth - 1, lane);
+    return slots + (taken++ & (kDepth - 1)) * kFloats;
   }
 };
 
@@ -315,33 +309,49 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
   return v;
 }
 
-// Adds a block's sums, times their factors, to this lane's kColumns sums (in pairs): from the accumulator at `taddr`, kChunk
-// columns on their way while the ones before are added.  `slot` holds the block's scales.  Calls `release` once the
+// Adds kCount accumulator columns, times their factors, to sums (in pairs).
+template <int kCount, bool kRowScales>
+__device__ __forceinline__ void add_columns(const uint32_t* v, uint64_t factors, const float* column_scales, uint64_t* sum) {
+#pragma unroll
+  for (int c = 0; c < kCount; c += 4) {
+    if constexpr (kRowScales) {
+      const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(column_scales + c);
+      fma2(sum[c / 2], two(v[c], v[c + 1]), mul2(factors, f.x));
+      fma2(sum[c / 2 + 1], two(v[c + 2], v[c + 3]), mul2(factors, f.y));
+    } else {
+      fma2(sum[c / 2], two(v[c], v[c + 1]), factors);
+      fma2(sum[c / 2 + 1], two(v[c + 2], v[c + 3]), factors);
+    }
+  }
+}
+
+// Adds a block's sums, times their factors, to this lane's kColumns sums: from the accumulator at `taddr`, two loads of kChunk
+// columns under way at a time.  `take` gives the block's scales while the first are; `release` is called once the
 // accumulator is in registers.
-template <int kColumns, int kChunk, bool kRowScales, typename Release>
-__device__ __forceinline__ void add_block(uint32_t taddr, const float* slot, int lane, uint64_t (&sum)[kColumns / 2],
+template <int kColumns, int kChunk, bool kRowScales, typename Take, typename Release>
+__device__ __forceinline__ void add_block(uint32_t taddr, int lane, uint64_t (&sum)[kColumns / 2], Take&& take,
                                           Release&& release) {
+  constexpr bool kTwo = kColumns > kChunk;
+  constexpr int kStep = kTwo ? 2 * kChunk : kChunk;
+  static_assert(kColumns % kStep == 0, "whole pairs of loads");
+  uint32_t v0[kChunk], v1[kTwo ? kChunk : 1];
+  tmem_load<kChunk>(taddr, v0);
+  if constexpr (kTwo) tmem_load<kChunk>(taddr + kChunk, v1);
+  const float* slot = take();
   const float factor = kRowScales ? slot[lane] : slot[lane] * slot[32];
   const uint64_t factors = two(__float_as_uint(factor), __float_as_uint(factor));
-  const ulonglong2* column_scales = reinterpret_cast<const ulonglong2*>(slot + 32);
-  uint32_t v[2][kChunk];
-  tmem_load<kChunk>(taddr, v[0]);
+  const float* column_scales = slot + 32;
 #pragma unroll
-  for (int c0 = 0; c0 < kColumns; c0 += kChunk) {
-    uint32_t (&now)[kChunk] = v[(c0 / kChunk) & 1];
-    tmem_wait<kChunk>(now);
-    if (c0 + kChunk < kColumns) tmem_load<kChunk>(taddr + c0 + kChunk, v[(c0 / kChunk + 1) & 1]);
-    else release();
-#pragma unroll
-    for (int c = 0; c < kChunk; c += 4) {
-      if constexpr (kRowScales) {
-        const ulonglong2 f = column_scales[(c0 + c) / 4];
-        fma2(sum[(c0 + c) / 2], two(now[c], now[c + 1]), mul2(factors, f.x));
-        fma2(sum[(c0 + c) / 2 + 1], two(now[c + 2], now[c + 3]), mul2(factors, f.y));
-      } else {
-        fma2(sum[(c0 + c) / 2], two(now[c], now[c + 1]), factors);
-        fma2(sum[(c0 + c) / 2 + 1], two(now[c + 2], now[c + 3]), factors);
-      }
+  for (int c0 = 0; c0 < kColumns; c0 += kStep) {
+    tmem_wait<kChunk>(v0);
+    if constexpr (kTwo) tmem_pass<kChunk>(v1);
+    const bool last = c0 + kStep == kColumns;
+    if (last) release();
+    add_columns<kChunk, kRowScales>(v0, factors, column_scales + c0, sum + c0 / 2);
+    if (!last) tmem_load<kChunk>(taddr + c0 + kStep, v0);
+    if constexpr (kTwo) {
+      add_columns<kChunk, kRowScales>(v1, factors, column_scales + c0 + kChunk, sum + (c0 + kChunk) / 2);
+      if (!last) tmem_load<kChunk>(taddr + c0 + kStep + kChunk, v1);
     }
   }
 }
@@ -363,7 +373,7 @@ struct Shape {
   static constexpr int kStages = kTileN == 128 ? 5 : 8;
   static constexpr uint32_t kTmemCols = kAccumulators * kTileN < 32 ? 32 : kAccumulators * kTileN;
   static constexpr uint32_t kStagingBytes = kTileN == 128 ? kSumWarps * 32 * 128 : 0;   // 128 bytes of 32 rows a warp
-  using Queue = ScaleQueue<kRowScales ? kColumns : 0, kRowScales && kTileN == 128 ? 6 : 8>;
+  using Queue = ScaleQueue<kRowScales ? kColumns : 0, kRowScales && kTileN == 128 ? 4 : 8>;
   static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + kSumWarps * Queue::kBytes + 256 + 1024;
 };
 
@@ -469,13 +479,13 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const int sub = warp & 3;
     const int first_column = ((warp - 2) >> 2) * kColumns;
     uint8_t* stage_out = staging + (warp - 2) * 32 * 128;
-    typename S::Queue queue(queues + (warp - 2) * S::Queue::kBytes, lane);
+    typename S::Queue queue(queues + (warp - 2) * S::Queue::kBytes);
     uint32_t it = 0;
     bool ok = true;
     int tm, tn;
     if (blockIdx.x < total_tiles) {
       tile_at(blockIdx.x, p, tm, tn);
-      queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks);
+      queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks, lane);
     }
     for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
       uint64_t sum[kColumns / 2];
@@ -483,11 +493,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       for (int c = 0; c < kColumns / 2; ++c) sum[c] = 0;
       for (int kb = 0; kb < k_blocks; ++kb, ++it) {
         const uint32_t acc = it % kAcc;
-        const float* slot = queue.take();
         if (!warp_wait(&acc_full[acc], (it / kAcc) & 1u)) { ok = false; break; }
         tc_fence_after();
-        add_block<kColumns, kColumns < 32 ? kColumns : 32, kRowScales>(
-            tmem_base + acc * kTileN + uint32_t(first_column) + (uint32_t(sub * 32) << 16), slot, lane, sum, [&] {
+        add_block<kColumns, kColumns >= 64 ? 32 : kColumns >= 16 ? kColumns / 2 : kColumns, kRowScales>(
+            tmem_base + acc * kTileN + uint32_t(first_column) + (uint32_t(sub * 32) << 16), lane, sum,
+            [&] { return queue.take(p, k_blocks - 1 - kb, lane); },
+            [&] {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) mbar_arrive(&acc_empty[acc]);
@@ -497,7 +508,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const int row0 = tm * kBM + sub * 32, col0 = tn * kTileN + first_column;
       if (t + int(gridDim.x) < total_tiles) {   // the next tile's first scales come while this one's sums go out
         tile_at(t + int(gridDim.x), p, tm, tn);
-        queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks);
+        queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks, lane);
       }
       auto value = [&](int c) {
         const float2 f = apart(sum[c / 2]);

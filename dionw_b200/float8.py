@@ -80,6 +80,13 @@ class Float8Matrix:
         return self.values.float() * scales.repeat_interleave(BLOCK, 1)[:, :cols]
 
 
+def _made(values: Tensor, scales: Tensor) -> Float8Matrix:
+    """A ``Float8Matrix`` of what was just allocated to be one."""
+    matrix = object.__new__(Float8Matrix)
+    matrix.__dict__.update(values=values, scales=scales)
+    return matrix
+
+
 def _require_source(x: Tensor) -> None:
     if x.ndim != 2:
         raise ValueError(f"expected a matrix, got shape {tuple(x.shape)}")
@@ -102,18 +109,19 @@ def _with_rows(x: Tensor) -> tuple[Tensor, int]:
 
 def _quantize(x: Tensor, tiles: bool, transposed: bool) -> Any:
     _require_source(x)
-    x, ldx = _with_rows(x.detach())
+    x, ldx = _with_rows(x)
     rows, cols = x.shape
+    device = x.device
     made: list[tuple[Tensor, Tensor]] = []
     found: list[Float8Matrix] = []
     for high, wide in ((rows, cols), (cols, rows)) if transposed else ((rows, cols),):
         ld = _padded(wide)
-        codes = torch.empty(high, ld, dtype=CODES, device=x.device)
+        codes = torch.empty(high, ld, dtype=CODES, device=device)
         # scales of single rows: those of a block column together, as the product and the quantizer go through them
         scales = torch.empty((_blocks(high), _blocks(wide)) if tiles else (_blocks(wide), high), dtype=torch.float32,
-                             device=x.device)
+                             device=device)
         made.append((codes, scales))
-        found.append(Float8Matrix(codes if ld == wide else codes[:, :wide], scales if tiles else scales.T))
+        found.append(_made(codes if ld == wide else codes[:, :wide], scales if tiles else scales.t()))
     if rows and cols:
         codes, scales = made[0]
         first = codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1]
@@ -144,7 +152,6 @@ def quantize_tiles(x: Tensor, *, transposed: bool = False) -> Any:
     return _quantize(x, True, transposed)
 
 
-@torch.no_grad()
 def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = None, out: Tensor | None = None,
                    accumulate: bool = False, out_dtype: torch.dtype | None = None) -> Tensor:
     """``a @ b.T`` (``a`` ``[m, k]``, ``b`` ``[n, k]``), plus ``bias`` ``[n]``, summed in fp32 and rounded once.
