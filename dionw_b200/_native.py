@@ -104,10 +104,11 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
                 c_double, c_double, c_float, c_float, c_uint32, c_void_p, c_void_p)),
     "dionw_float8_quantize": (
         c_int, (c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                c_int64, c_void_p, c_int64, c_void_p)),
+                c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p)),
     "dionw_float8_product": (
         c_int, (c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64,
-                c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_void_p)),
+                c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                c_void_p)),
     "dionw_ema_multi": (c_int, (_PP, _PP, _I64P, c_int, c_int, c_float, c_int, c_void_p)),
     "dionw_ema_stage_pack": (c_int, (_PP, _I64P, _I64P, c_int, c_int, c_void_p, c_void_p)),
     "dionw_cpu_ema_job_start": (c_void_p, (_PP, _PP, _I64P, POINTER(c_uint8), c_int, c_float, c_void_p, c_int)),
@@ -397,19 +398,20 @@ def on_device(device: int, entry: Any, *args: Any) -> None:
 
 def float8_quantize(device: int, x: int, dtype: torch.dtype, rows: int, cols: int, ldx: int, tiles: bool, q: int | None,
                     ldq: int, scales: int | None, lds: int, qt: int | None, ldqt: int, scales_t: int | None,
-                    ldst: int) -> None:
+                    ldst: int, exponents: int | None = None, exponents_t: int | None = None) -> None:
     """By address, as the ABI takes it; no matrix without elements."""
     on_device(device, library().dionw_float8_quantize, x, _DTYPE_CODE[dtype], rows, cols, ldx, tiles, q, ldq, scales, lds,
-              qt, ldqt, scales_t, ldst)
+              qt, ldqt, scales_t, ldst, exponents, exponents_t)
 
 
 def float8_product(device: int, a: tuple[int, int, int, int, int, bool], b: tuple[int, int, int, int, int, bool],
-                   bias: Tensor | None, out: Tensor, accumulate: bool, m: int, n: int, k: int) -> None:
+                   bias: Tensor | None, out: Tensor, accumulate: bool, m: int, n: int, k: int,
+                   exponents: tuple[int | None, int | None] = (None, None)) -> None:
     """``a`` and ``b``: address and leading dimension of the codes, address and the two strides of the scales, and
-    whether those are tiles'."""
+    whether those are tiles'; ``exponents``: the scales as the quantizer wrote them a second time."""
     on_device(device, library().dionw_float8_product, *a, *b, None if bias is None else bias.data_ptr(),
               0 if bias is None else _DTYPE_CODE[bias.dtype], out.data_ptr(), out.stride(0) if m > 1 else n,
-              _DTYPE_CODE[out.dtype], accumulate, m, n, k)
+              _DTYPE_CODE[out.dtype], accumulate, m, n, k, *exponents)
 
 
 # ---------------------------------------------------------------------------

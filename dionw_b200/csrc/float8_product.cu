@@ -2,6 +2,7 @@
 #include <atomic>
 
 #include "float8_pair_sm100.cuh"
+#include "float8_scaled_sm100.cuh"
 #include "float8_sm100.cuh"
 #include "products.cuh"
 
@@ -10,21 +11,28 @@ namespace {
 
 constexpr int kMaxDevices = 64;
 
+// Sets a kernel's shared memory once for each device.
+template <typename Kernel>
+int allow_shared(Kernel kernel, size_t smem, std::atomic<bool> (&configured)[kMaxDevices]) {
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
+  if (configured[device].load(std::memory_order_acquire)) return DIONW_OK;
+  DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem)));
+  configured[device].store(true, std::memory_order_release);
+  return DIONW_OK;
+}
+
 template <typename T, int kTileN, bool kSwap, bool kRowScales>
 int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
   using S = float8::Shape<kTileN, kRowScales>;
   static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
   auto kernel = float8::product_kernel<T, kTileN, kSwap, kRowScales>;
-  static std::atomic<bool> configured[kMaxDevices];   // the attribute is per device
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
-  if (!configured[device].load(std::memory_order_acquire)) {
-    DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmemBytes)));
-    configured[device].store(true, std::memory_order_release);
-  }
+  static std::atomic<bool> configured[kMaxDevices];
+  int st = allow_shared(kernel, S::kSmemBytes, configured);
+  if (st != DIONW_OK) return st;
   CUtensorMap map_a{}, map_b{};
   if (p.k > 0) {
-    int st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
+    st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
     if (st != DIONW_OK) return st;
     st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, kTileN);
     if (st != DIONW_OK) return st;
@@ -53,34 +61,14 @@ int launch(const void* a, int64_t lda, const void* b, int64_t ldb, const float8:
                         : launch_single<T, kTileN, kSwap, true>(a, lda, b, ldb, p, stream);
 }
 
-// 256 x 256 tiles on SM pairs.
-template <typename T, bool kRowScales>
-int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
-  namespace pair = float8::pair;
-  static_assert(pair::kSmemBytes<kRowScales> <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = pair::product_kernel<T, kRowScales>;
-  static std::atomic<bool> configured[kMaxDevices];
-  int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= kMaxDevices) device = 0;
-  if (!configured[device].load(std::memory_order_acquire)) {
-    DIONW_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(pair::kSmemBytes<kRowScales>)));
-    configured[device].store(true, std::memory_order_release);
-  }
-  CUtensorMap map_a{}, map_b{};
-  if (p.k > 0) {
-    int st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
-    if (st != DIONW_OK) return st;
-    st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, pair::kPairN / 2);
-    if (st != DIONW_OK) return st;
-  }
-  p.tiles_m = (p.m + pair::kPairM - 1) / pair::kPairM;
-  p.tiles_n = (p.n + pair::kPairN - 1) / pair::kPairN;
+// As clusters of two CTAs, one to each SM pair that has a tile.
+template <typename Kernel, typename... Args>
+int launch_clusters_of_two(Kernel kernel, size_t smem, int threads, float8::Params& p, cudaStream_t stream, const Args&... maps) {
   const long long total = (long long)p.tiles_m * p.tiles_n, pairs_max = sm_count() / 2;
-  DIONW_REQUIRE(total <= 0x7FFFFFFFll, "float8_product: too many tiles");
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(unsigned(2 * (total < pairs_max ? total : pairs_max)));
-  config.blockDim = dim3(pair::kThreads);
-  config.dynamicSmemBytes = pair::kSmemBytes<kRowScales>;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
   attributes[0].id = cudaLaunchAttributeClusterDimension;
@@ -92,8 +80,59 @@ int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8:
   config.attrs = attributes;
   config.numAttrs = use_dependent_launch() ? 2 : 1;
   count_launch();
-  return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&config, kernel, maps..., p), "product_kernel launch");
 }
+
+int count_pair_tiles(float8::Params& p) {
+  p.tiles_m = (p.m + float8::pair::kPairM - 1) / float8::pair::kPairM;
+  p.tiles_n = (p.n + float8::pair::kPairN - 1) / float8::pair::kPairN;
+  DIONW_REQUIRE((long long)p.tiles_m * p.tiles_n <= 0x7FFFFFFFll, "float8_product: too many tiles");
+  return DIONW_OK;
+}
+
+// 256 x 256 tiles on SM pairs.
+template <typename T, bool kRowScales>
+int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  namespace pair = float8::pair;
+  static_assert(pair::kSmemBytes<kRowScales> <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = pair::product_kernel<T, kRowScales>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int st = allow_shared(kernel, pair::kSmemBytes<kRowScales>, configured);
+  if (st != DIONW_OK) return st;
+  CUtensorMap map_a{}, map_b{};
+  if (p.k > 0) {
+    st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
+    if (st != DIONW_OK) return st;
+    st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, pair::kPairN / 2);
+    if (st != DIONW_OK) return st;
+  }
+  st = count_pair_tiles(p);
+  if (st != DIONW_OK) return st;
+  return launch_clusters_of_two(kernel, pair::kSmemBytes<kRowScales>, pair::kThreads, p, stream, map_a, map_b);
+}
+
+// The same with exponents that the tensor cores apply.
+template <typename T>
+int launch_scaled(const void* a, int64_t lda, const void* a_exponents, const void* b, int64_t ldb, const void* b_exponents,
+                  float8::Params p, cudaStream_t stream) {
+  namespace scaled = float8::scaled;
+  static_assert(scaled::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = scaled::product_kernel<T>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int st = allow_shared(kernel, scaled::kSmemBytes, configured);
+  if (st != DIONW_OK) return st;
+  scaled::Maps maps;
+  const int64_t blocks = (p.k + 127) / 128;
+  st = make_byte_map(&maps.a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
+  if (st == DIONW_OK) st = make_byte_map(&maps.b, b, p.k, p.n, ldb, float8::kBK, scaled::kPairN / 2);
+  if (st == DIONW_OK) st = make_word_map(&maps.a_scales, a_exponents, blocks * ((p.m + 127) / 128), 1);
+  if (st == DIONW_OK) st = make_word_map(&maps.b_scales, b_exponents, blocks * ((p.n + 127) / 128), 2);
+  if (st == DIONW_OK) st = count_pair_tiles(p);
+  if (st != DIONW_OK) return st;
+  return launch_clusters_of_two(kernel, scaled::kSmemBytes, scaled::kThreads, p, stream, maps);
+}
+
+long long pair_tiles(long long m, long long n) { return ((m + 255) / 256) * ((n + 255) / 256); }
 
 // The kernel for a product of this shape.
 template <typename T>
@@ -107,8 +146,7 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p
     if (m <= 32) return launch<T, 32, true>(b, ldb, a, lda, p, stream);
     return launch<T, 64, true>(b, ldb, a, lda, p, stream);
   }
-  const long long pair_tiles = ((p.m + 255ll) / 256) * ((p.n + 255ll) / 256);
-  if (pair_tiles >= sm_count() / 2)
+  if (pair_tiles(p.m, p.n) >= sm_count() / 2)
     return p.b.shift != 0 ? launch_pairs<T, false>(a, lda, b, ldb, p, stream) : launch_pairs<T, true>(a, lda, b, ldb, p, stream);
   return launch<T, 128, false>(a, lda, b, ldb, p, stream);
 }
@@ -122,7 +160,8 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
                                     int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
                                     const float* b_scales, int64_t b_row_stride, int64_t b_block_stride, int b_tiles,
                                     const void* bias, int bias_dtype, void* out, int64_t ldo, int out_dtype,
-                                    int accumulate, int64_t m, int64_t n, int64_t k, void* stream_ptr) {
+                                    int accumulate, int64_t m, int64_t n, int64_t k, const uint32_t* a_exponents,
+                                    const uint32_t* b_exponents, void* stream_ptr) {
   DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= 0x7FFFFF00ll && n <= 0x7FFFFF00ll && k <= 0x7FFFFF00ll,
                 "float8_product: bad shape %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
   DIONW_REQUIRE(out_dtype >= DIONW_F32 && out_dtype <= DIONW_BF16, "float8_product: bad output dtype");
@@ -150,6 +189,12 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
   p.status = device_status_word();
   p.wait_ns = gemm::kWaitLimitNs;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (a_exponents != nullptr && b_exponents != nullptr && k > 0 && pair_tiles(m, n) >= sm_count() / 2) {
+    DIONW_REQUIRE(aligned16(a_exponents) && aligned16(b_exponents), "float8_product: exponents must be 16-byte aligned");
+    if (out_dtype == DIONW_F32) return launch_scaled<float>(a, lda, a_exponents, b, ldb, b_exponents, p, stream);
+    if (out_dtype == DIONW_F16) return launch_scaled<__half>(a, lda, a_exponents, b, ldb, b_exponents, p, stream);
+    return launch_scaled<__nv_bfloat16>(a, lda, a_exponents, b, ldb, b_exponents, p, stream);
+  }
   if (out_dtype == DIONW_F32) return run<float>(a, lda, b, ldb, p, stream);
   if (out_dtype == DIONW_F16) return run<__half>(a, lda, b, ldb, p, stream);
   return run<__nv_bfloat16>(a, lda, b, ldb, p, stream);

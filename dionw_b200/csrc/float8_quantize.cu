@@ -35,8 +35,10 @@ struct QuantizeParams {
   int64_t lds;
   float* scales_t;     // the same of the transposed matrix
   int64_t ldst;
+  uint32_t* exponents;   // nullable: of the scales of 128 rows together, as float8_scaled_sm100.cuh wants them
+  uint32_t* exponents_t;
   int rows, cols;
-  int tiles_x, tiles;  // of 128 x 128
+  int tiles_x, tiles_y, tiles;  // of 128 x 128
   int vec;             // 16-byte loads
 };
 
@@ -56,6 +58,10 @@ __device__ __forceinline__ float scale_of(uint32_t largest, float& inverse) {
   inverse = __uint_as_float(uint32_t(127 - k) << 23);
   return __uint_as_float(uint32_t(127 + k) << 23);
 }
+
+// Word of row r's exponent among those of 128 rows, and the exponent with fp32's bias (NaN: 255).
+__device__ __forceinline__ int exponent_at(int r) { return 4 * (r & 31) + (r >> 5); }
+__device__ __forceinline__ uint32_t exponent_of(float scale) { return __float_as_uint(scale) >> 23; }
 
 __device__ __forceinline__ uint32_t to_codes(float a, float b, float c, float d) {
   uint16_t lo, hi;
@@ -180,6 +186,10 @@ quantize_kernel(const QuantizeParams p) {
         if (p.q != nullptr) p.scales[int64_t(ty) * p.lds + tx] = scale;
         if (p.qt != nullptr) p.scales_t[int64_t(tx) * p.ldst + ty] = scale;
       }
+      if (threadIdx.x < kBlock) {
+        if (p.exponents != nullptr) p.exponents[(int64_t(tx) * p.tiles_y + ty) * kBlock + threadIdx.x] = exponent_of(scale);
+        if (p.exponents_t != nullptr) p.exponents_t[(int64_t(ty) * p.tiles_x + tx) * kBlock + threadIdx.x] = exponent_of(scale);
+      }
     } else if (p.qt != nullptr) {
       uint32_t top[kWords];
 #pragma unroll
@@ -222,7 +232,11 @@ quantize_kernel(const QuantizeParams p) {
         else mine = lane16 & 2 ? (lane16 & 1 ? top[3] : top[2]) : (lane16 & 1 ? top[1] : top[0]);
         float inv;
         const float scale = scale_of(mine, inv);
-        if (lane16 < kRows && row0 + lane16 < p.rows) p.scales[int64_t(tx) * p.lds + row0 + lane16] = scale;
+        if (lane16 < kRows) {
+          if (row0 + lane16 < p.rows) p.scales[int64_t(tx) * p.lds + row0 + lane16] = scale;
+          if (p.exponents != nullptr)
+            p.exponents[(int64_t(tx) * p.tiles_y + ty) * kBlock + exponent_at(group * kRows + lane16)] = exponent_of(scale);
+        }
 #pragma unroll
         for (int r = 0; r < kRows; ++r) row_inverse[r] = __shfl_sync(0xffffffffu, inv, r, 16);
       }
@@ -253,6 +267,7 @@ quantize_kernel(const QuantizeParams p) {
         float inv;
         const float scale = scale_of(Eight<T>::of_column(top, c), inv);
         if (tile_col + c < p.cols) p.scales_t[int64_t(ty) * p.ldst + tile_col + c] = scale;
+        if (p.exponents_t != nullptr) p.exponents_t[(int64_t(ty) * p.tiles_x + tx) * kBlock + exponent_at(c)] = exponent_of(scale);
         column_inverse[c] = inv;
       }
       __syncthreads();
@@ -313,7 +328,8 @@ using namespace dionw;
 
 extern "C" int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx, int tiles,
                                      void* q, int64_t ldq, float* scales, int64_t lds, void* qt, int64_t ldqt,
-                                     float* scales_t, int64_t ldst, void* stream_ptr) {
+                                     float* scales_t, int64_t ldst, uint32_t* exponents, uint32_t* exponents_t,
+                                     void* stream_ptr) {
   DIONW_REQUIRE(dtype >= DIONW_F32 && dtype <= DIONW_BF16, "float8_quantize: bad dtype");
   DIONW_REQUIRE(rows >= 0 && cols >= 0 && rows <= 0x7FFFFF80ll && cols <= 0x7FFFFF80ll, "float8_quantize: bad shape %lld x %lld",
                 (long long)rows, (long long)cols);
@@ -338,9 +354,12 @@ extern "C" int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int
   p.lds = lds;
   p.scales_t = scales_t;
   p.ldst = ldst;
+  p.exponents = q != nullptr ? exponents : nullptr;
+  p.exponents_t = qt != nullptr ? exponents_t : nullptr;
   p.rows = int(rows);
   p.cols = int(cols);
   p.tiles_x = int(col_blocks);
+  p.tiles_y = int(row_blocks);
   p.tiles = int(row_blocks * col_blocks);
   const int64_t size = dtype == DIONW_F32 ? 4 : 2;
   p.vec = aligned16(x) && (rows == 1 || (ldx * size) % 16 == 0);

@@ -103,6 +103,27 @@ int make_byte_map(CUtensorMap* map, const void* base, int64_t inner, int64_t row
   return DIONW_OK;
 }
 
+// 2-D map over rows of 128 32-bit words that lie one after the other: boxes of `box_rows` whole rows, not swizzled.
+int make_word_map(CUtensorMap* map, const void* base, int64_t rows, uint32_t box_rows) {
+  EncodeFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from this driver");
+    return DIONW_ERR_CUDA;
+  }
+  cuuint64_t dims[2] = {128, cuuint64_t(rows)};
+  cuuint64_t strides[1] = {512};
+  cuuint32_t box[2] = {128, box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult res = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(base), dims, strides, box, elem,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (res != CUDA_SUCCESS) {
+    set_error("cuTensorMapEncodeTiled failed with code %d (%lld rows of 128 words)", int(res), (long long)rows);
+    return DIONW_ERR_CUDA;
+  }
+  return DIONW_OK;
+}
+
 namespace {
 
 constexpr int kMaxDevices = 64;

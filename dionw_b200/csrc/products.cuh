@@ -68,5 +68,7 @@ int run_on_chip(const Product* list, const int* chain_length, const ChainSlot* s
 // Tensor map over a row-major matrix of bytes (rows `ld` apart, 16-byte aligned), 128-byte swizzled boxes.
 int make_byte_map(CUtensorMap* map, const void* base, int64_t inner, int64_t rows, int64_t ld, uint32_t box_inner,
                   uint32_t box_rows);
+// The same over rows of 128 32-bit words, boxes of whole rows as they lie.
+int make_word_map(CUtensorMap* map, const void* base, int64_t rows, uint32_t box_rows);
 
 }  // namespace dionw

@@ -266,23 +266,30 @@ int dionw_batched_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, i
  * 16-byte boundaries and have leading dimensions that are multiples of 16 (codes between the
  * matrix and the next multiple of 8 may be overwritten, with zeros).  The scale of (row r,
  * block c) is scales[c * lds + r], of (tile row r, tile column c) scales[r * lds + c]; scales_t
- * (ldst) is the same for the transposed matrix. */
+ * (ldst) is the same for the transposed matrix.  exponents and exponents_t (nullable) receive
+ * the scales a second time, in the form in which dionw_float8_product hands them to the tensor
+ * cores: one 32-bit word for each row and block, the scale's exponent with fp32's bias in its
+ * low byte, ceil(cols / 128) * ceil(rows / 128) * 128 words: block after block, 128 rows after
+ * 128 rows, of which word 4 l + c is that of row 32 c + l. */
 int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
                           int tiles, void* q, int64_t ldq, float* scales, int64_t lds,
-                          void* qt, int64_t ldqt, float* scales_t, int64_t ldst, void* stream);
+                          void* qt, int64_t ldqt, float* scales_t, int64_t ldst,
+                          uint32_t* exponents, uint32_t* exponents_t, void* stream);
 
 /* out[i, j] = sum over blocks b of 128 k's of sa[i, b] sb[j, b] sum over k in b of a[i, k] b[j, k],
  * + bias[j] (nullable), + out[i, j] (accumulate != 0); sums in fp32, rounded once to out_dtype.
  * a [m, lda] and b [n, ldb] are e4m3 codes, rows on 16-byte boundaries; the scale of row i in
  * block b is a_scales[i * a_row_stride + b * a_block_stride], with i / 128 in the place of i
  * where a_tiles != 0 (b likewise).  out must not overlap an operand.  Results do not depend on
- * anything but the operands: sums are taken in a fixed order. */
+ * anything but the operands: sums are taken in a fixed order.  a_exponents and b_exponents
+ * (both or neither, 16-byte aligned): the scales as dionw_float8_quantize wrote them a second
+ * time; large products then leave them to the tensor cores and sum in one piece. */
 int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int64_t a_row_stride,
                          int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
                          const float* b_scales, int64_t b_row_stride, int64_t b_block_stride,
                          int b_tiles, const void* bias, int bias_dtype, void* out, int64_t ldo,
                          int out_dtype, int accumulate, int64_t m, int64_t n, int64_t k,
-                         void* stream);
+                         const uint32_t* a_exponents, const uint32_t* b_exponents, void* stream);
 
 /* ---- NorMuon and the weight update -------------------------------------- */
 

@@ -117,7 +117,8 @@ def test_quantize_entry_refuses() -> None:
 
     def call(x=at, dtype=0, rows=4, cols=100, ldx=100, q=at, ldq=112, scales=at, lds=4, qt=None, ldqt=0, scales_t=None,
              ldst=0):
-        return lib.dionw_float8_quantize(x, dtype, rows, cols, ldx, 0, q, ldq, scales, lds, qt, ldqt, scales_t, ldst, None)
+        return lib.dionw_float8_quantize(x, dtype, rows, cols, ldx, 0, q, ldq, scales, lds, qt, ldqt, scales_t, ldst, None, None,
+                                         None)
 
     assert call(rows=0) == 0 and call(cols=0) == 0
     for bad, match in ((dict(dtype=3), "dtype"), (dict(rows=-1), "shape"), (dict(ldx=99), "leading dimension"),
@@ -171,7 +172,7 @@ def test_float8_product_entry_refuses() -> None:
 
     def call(a=at, lda=112, sa=at, b=at, ldb=112, sb=at, bias=None, bias_dtype=0, out=at, ldo=6, out_dtype=0, m=4, n=6, k=100):
         return lib.dionw_float8_product(a, lda, sa, 1, 4, 0, b, ldb, sb, 1, 6, 0, bias, bias_dtype, out, ldo, out_dtype, 0,
-                                        m, n, k, None)
+                                        m, n, k, None, None, None)
 
     assert call(m=0) == 0 and call(n=0) == 0
     for bad, match in ((dict(m=-1), "shape"), (dict(k=1 << 33), "shape"), (dict(out_dtype=3), "output"),

@@ -253,6 +253,36 @@ def test_linear(tokens, inputs, outputs, dtype, with_bias) -> None:
         assert bool(((grads[2].cpu().double() - want).abs() <= (tokens + 2) * 2.0**-24 * dy.double().abs().sum(0) + 1e-30).all())
 
 
+@pytest.mark.parametrize("tokens,inputs,outputs", [(2501, 1900, 2405), (4097, 2304, 1281)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_of_many_tiles(tokens, inputs, outputs, dtype) -> None:
+    """Enough tiles for the tensor cores to take the scales themselves."""
+    x, dy = _matrix(tokens, inputs, 1, dtype).to(DEV).requires_grad_(), _matrix(tokens, outputs, 2, dtype).to(DEV)
+    w = (_matrix(outputs, inputs, 3) * 0.1).to(DEV).requires_grad_()
+    y = dionw.float8_linear(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    rows, columns = (q.dequantize().double() for q in dionw.quantize_rows(x, transposed=True))
+    drows, dcolumns = (q.dequantize().double() for q in dionw.quantize_rows(dy, transposed=True))
+    tiles, turned = (q.dequantize().double() for q in dionw.quantize_tiles(w, transposed=True))
+    for got, a, b in ((y.detach(), rows, tiles), (dx, drows, turned), (dw, dcolumns, columns)):
+        # one sum over the whole length on the tensor cores: a rounding of 2^-23 for each 32 products
+        want, size = a @ b.T, a.abs() @ b.abs().T
+        bound = (32 + a.shape[1] / 32) * 2.0**-23 * size + HALF_STEP[got.dtype] * 1.01 * want.abs() + 2.0**-25
+        assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() / bound).max())
+
+
+def test_linear_of_many_tiles_keeps_infinities_in_their_rows() -> None:
+    x = _matrix(2501, 1900, 1).to(DEV)
+    w = (_matrix(2405, 1900, 3) * 0.1).to(DEV)
+    clean = dionw.float8_linear(x, w)
+    x[7, 3], x[2500, 1899], w[1000, 5] = math.inf, math.nan, math.nan
+    y = dionw.float8_linear(x, w)
+    bad = torch.zeros_like(y, dtype=torch.bool)
+    bad[7], bad[2500], bad[:, 896:1024] = True, True, True
+    assert torch.equal(y.isnan(), bad)
+    assert torch.equal(y[~bad], clean[~bad])
+
+
 def test_linear_gradients_are_those_of_differences() -> None:
     """The gradients against differences of the 64-bit layer in random directions.  Each quantized operand is off by at
     most 2^-4 of a value; errors of independent elements add up in squares, so that an inner product of 64 x 256
