@@ -1,4 +1,6 @@
-"""The AdamW route: one fused multi-tensor launch per group (src/dionw/_adamw.py:18-61)."""
+"""The AdamW route: one fused multi-tensor launch per group (src/dionw/_adamw.py:18-61).
+
+A group with ``adamw_state_bits = 8`` keeps its moments as 8-bit codes with block scales (``adamw8.py``)."""
 
 from __future__ import annotations
 
@@ -9,11 +11,18 @@ import torch
 from torch import Tensor
 
 from dionw_b200 import _native
-from dionw_b200._keys import ADAMW_STEP_STATE, EXP_AVG_SQ_STATE, EXP_AVG_STATE, ParamState
+from dionw_b200._keys import (
+    ADAMW_STATE_BITS_KEY, ADAMW_STEP_STATE, EXP_AVG_SCALE_STATE, EXP_AVG_SQ_SCALE_STATE, EXP_AVG_SQ_STATE, EXP_AVG_STATE,
+    ParamState,
+)
+from dionw_b200.adamw8 import adamw8_state
 
 
-def init_adamw_state(param: Tensor, state: dict[str, Any]) -> None:
+def init_adamw_state(param: Tensor, state: dict[str, Any], bits: int = 32) -> None:
     """Fresh moments and an fp32 step counter on the parameter's device."""
+    if bits == 8:
+        state.update(adamw8_state(param))
+        return
     state[EXP_AVG_STATE] = torch.zeros_like(param)
     state[EXP_AVG_SQ_STATE] = torch.zeros_like(param)
     state[ADAMW_STEP_STATE] = torch.zeros((), dtype=torch.float32, device=param.device)
@@ -34,12 +43,14 @@ def adamw_step(group: dict[str, Any], state: ParamState,
             adamw_step({**group, "params": [p for p in params if p.device == device]}, state, hyper)
         return
     device = params[0].device
+    bits = group.get(ADAMW_STATE_BITS_KEY, 32)
     fixups: list[tuple[Tensor, Tensor]] = []
     p_list, g_list, m_list, v_list, s_list = [], [], [], [], []
+    scales: tuple[list[Tensor], list[Tensor]] = ([], [])
     for param in params:
         entry = state[param]
         if EXP_AVG_STATE not in entry:
-            init_adamw_state(param, entry)
+            init_adamw_state(param, entry, bits)
         grad = param.grad
         if grad is None:
             raise RuntimeError("an AdamW update holds a parameter without a gradient")
@@ -55,12 +66,19 @@ def adamw_step(group: dict[str, Any], state: ParamState,
         m_list.append(entry[EXP_AVG_STATE])
         v_list.append(entry[EXP_AVG_SQ_STATE])
         s_list.append(entry[ADAMW_STEP_STATE])
+        if bits == 8:
+            scales[0].append(entry[EXP_AVG_SCALE_STATE])
+            scales[1].append(entry[EXP_AVG_SQ_SCALE_STATE])
     beta1, beta2 = group["betas"]
-    with torch.cuda.device(device):
-        _native.adamw_multi(
-            p_list, g_list, m_list, v_list, s_list, lr=float(group["lr"]), beta1=float(beta1), beta2=float(beta2),
-            weight_decay=float(group["weight_decay"]), eps=float(group["eps"]),
-            hyper_device=None if hyper is None else hyper(device),
-        )
+    settings = dict(lr=float(group["lr"]), beta1=float(beta1), beta2=float(beta2),
+                    weight_decay=float(group["weight_decay"]), eps=float(group["eps"]),
+                    hyper_device=None if hyper is None else hyper(device))
+    if bits == 8:
+        tensors = [*p_list, *g_list, *m_list, *v_list, *scales[0], *scales[1], *s_list]
+        _native.adamw8_multi(list(map(Tensor.data_ptr, tensors)), list(map(Tensor.numel, p_list)), torch.float32,
+                             device=p_list[0].get_device(), seed=0, **settings)
+    else:
+        with torch.cuda.device(device):
+            _native.adamw_multi(p_list, g_list, m_list, v_list, s_list, **settings)
     for param, packed in fixups:
         param.copy_(packed)

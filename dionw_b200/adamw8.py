@@ -118,3 +118,13 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         raise ValueError("adamw8_step: hyper_device must be two contiguous float32 on the parameters' device")
     _native.adamw8_multi(addresses, numels, grad_dtype, device=device, lr=lr, beta1=beta1, beta2=beta2,
                          weight_decay=weight_decay, eps=eps, seed=seed, hyper_device=hyper_device)
+
+
+def require_adamw8_state(param: Tensor, entry: dict[str, Any]) -> None:
+    """Raise ValueError if a state entry is not what ``adamw8_state`` makes for ``param``."""
+    for key, expected in adamw8_state(param.detach().to("meta")).items():
+        found = entry.get(key)
+        if not isinstance(found, Tensor) or found.shape != expected.shape or found.dtype is not expected.dtype:
+            raise ValueError(
+                f"AdamW state of a parameter of shape {tuple(param.shape)} has no 8-bit {key!r} of shape "
+                f"{tuple(expected.shape)}: it was saved with other adamw_state_bits")

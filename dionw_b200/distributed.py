@@ -41,7 +41,7 @@ from dionw_b200 import _matrix_step, _native, _workspace
 from dionw_b200._adamw import init_adamw_state
 from dionw_b200._buckets import Bucket, block_shape, build_buckets
 from dionw_b200._keys import (
-    ADAMW_STEP_STATE, EMA_PENDING, EMA_SCRATCH_KEYS, EMA_SHADOW, EMA_STEP_COUNT_KEY, EXP_AVG_SQ_STATE,
+    ADAMW_STATE_BITS_KEY, ADAMW_STEP_STATE, EMA_PENDING, EMA_SCRATCH_KEYS, EMA_SHADOW, EMA_STEP_COUNT_KEY, EXP_AVG_SQ_STATE,
     EXP_AVG_STATE, FRACTION_KEY, MOMENTUM_STATE, NUM_HEADS_KEY, ROUTE_KEY, VARIANCE_STATE,
 )
 from dionw_b200.ema import EMAConfig, IntegratedEMAOptimizer, ProfileRegion, no_profile
@@ -196,7 +196,7 @@ class _ShardedCore(_DionCore):
         """Whether an AdamW tensor is updated by element range rather than whole on every rank."""
         return is_cut(param.numel(), self._world, param.is_contiguous())
 
-    def _new_adamw_state(self, param: Tensor) -> None:
+    def _new_adamw_state(self, param: Tensor, bits: int = 32) -> None:
         entry = self.state[param]
         if not self._is_cut(param):
             init_adamw_state(param, entry)
@@ -207,6 +207,8 @@ class _ShardedCore(_DionCore):
         entry[ADAMW_STEP_STATE] = torch.zeros((), dtype=torch.float32, device=param.device)
 
     def add_param_group(self, param_group: dict[str, Any]) -> None:
+        if param_group.get(ADAMW_STATE_BITS_KEY, 32) != 32:
+            raise NotImplementedError(f"ShardedDion holds AdamW moments in float32: {ADAMW_STATE_BITS_KEY} must be 32")
         super().add_param_group(param_group)
         self._shared = None
 

@@ -27,9 +27,10 @@ from dionw_b200 import _matrix_step
 from dionw_b200._adamw import adamw_step, init_adamw_state
 from dionw_b200._buckets import Bucket, block_shape, build_buckets
 from dionw_b200._keys import (
-    ADAMW_STEP_STATE, EXP_AVG_SQ_STATE, EXP_AVG_STATE, FRACTION_KEY, MOMENTUM_FORM_KEY, MOMENTUM_KEY, MUON_BETA2_KEY, NEWTON_SCHULZ_KEY,
-    NUM_HEADS_KEY, ROUTE_KEY, ROW_NORMALIZATION_KEY, STRUCTURAL_KEYS,
+    ADAMW_STATE_BITS_KEY, ADAMW_STEP_STATE, EXP_AVG_SCALE_STATE, EXP_AVG_SQ_SCALE_STATE, EXP_AVG_SQ_STATE, EXP_AVG_STATE,
+    FRACTION_KEY, MOMENTUM_FORM_KEY, MOMENTUM_KEY, MUON_BETA2_KEY, NEWTON_SCHULZ_KEY, NUM_HEADS_KEY, ROUTE_KEY, ROW_NORMALIZATION_KEY, STRUCTURAL_KEYS,
 )
+from dionw_b200.adamw8 import MEAN_DTYPE, SQUARE_DTYPE, require_adamw8_state
 from dionw_b200._matrix_step import (
     MAX_RUN_ELEMENTS, apply_result, groups_of_runs, open_run, run_core, run_elements, run_front, step_run, step_runs,
     step_size,
@@ -75,8 +76,13 @@ def _require_group(group: dict[str, Any]) -> None:
     if float(group["lr"]) < 0.0 or float(group["weight_decay"]) < 0.0:
         raise ValueError("a group's lr and weight_decay must be >= 0")
     kind = RouteKind(group[ROUTE_KEY])
+    bits = group.get(ADAMW_STATE_BITS_KEY, 32)
+    if bits not in (8, 32):
+        raise ValueError(f"{ADAMW_STATE_BITS_KEY} must be 8 or 32, got {bits!r}")
     if kind is RouteKind.ADAMW:
         return
+    if ADAMW_STATE_BITS_KEY in group:
+        raise ValueError(f"a matrix group has no {ADAMW_STATE_BITS_KEY}: its momentum is held in float32")
     if kind is not RouteKind.MATRIX:
         raise RuntimeError(f"Unhandled RouteKind: {kind}")
     fraction = float(group[FRACTION_KEY])
@@ -118,6 +124,11 @@ def _require_same_structure(saved: list[dict[str, Any]], current: list[dict[str,
                 raise ValueError(
                     f"Dion state group {index} {key!r}: checkpoint={old[key]!r}, optimizer={new[key]!r}. "
                     "Build the groups as the checkpoint was built to resume it.")
+        bits = old.get(ADAMW_STATE_BITS_KEY, 32), new.get(ADAMW_STATE_BITS_KEY, 32)
+        if bits[0] != bits[1]:
+            raise ValueError(
+                f"Dion state group {index} {ADAMW_STATE_BITS_KEY!r}: checkpoint={bits[0]!r}, optimizer={bits[1]!r}. "
+                "Moments are resumed in the form they were saved in.")
 
 
 def step_scalar_values(groups: list[dict[str, Any]], owners: list[Any]) -> tuple[list[float], int]:
@@ -143,7 +154,10 @@ class _DionCore(Optimizer):
 
     def __init__(self, params: Iterable[dict[str, Any]], *, lr: float, momentum: float, muon_beta2: float,
                  betas: tuple[float, float], weight_decay: float, eps: float,
-                 matrix_update: MatrixUpdate) -> None:
+                 matrix_update: MatrixUpdate, adamw_state_bits: int = 32) -> None:
+        if adamw_state_bits not in (8, 32):
+            raise ValueError(f"{ADAMW_STATE_BITS_KEY} must be 8 or 32, got {adamw_state_bits!r}")
+        self._adamw_state_bits = adamw_state_bits
         if lr < 0.0 or weight_decay < 0.0 or eps <= 0.0:
             raise ValueError("lr and weight_decay must be >= 0 and eps > 0")
         for name, value in ((MOMENTUM_KEY, momentum), (MUON_BETA2_KEY, muon_beta2),
@@ -186,6 +200,8 @@ class _DionCore(Optimizer):
         if isinstance(members, set):
             raise TypeError("Dion param group params must be ordered, not a set")
         group = {**param_group, "params": [members] if isinstance(members, Tensor) else list(members)}
+        if self._adamw_state_bits == 8 and group.get(ROUTE_KEY) == RouteKind.ADAMW.value:
+            group.setdefault(ADAMW_STATE_BITS_KEY, 8)
         for param in group["params"]:
             _require_param(param)
         _require_group({**self.defaults, **group})
@@ -197,11 +213,11 @@ class _DionCore(Optimizer):
         # the buckets at the first step.
         if RouteKind(group[ROUTE_KEY]) is RouteKind.ADAMW:
             for param in group["params"]:
-                self._new_adamw_state(param)
+                self._new_adamw_state(param, group.get(ADAMW_STATE_BITS_KEY, 32))
 
-    def _new_adamw_state(self, param: Tensor) -> None:
+    def _new_adamw_state(self, param: Tensor, bits: int = 32) -> None:
         """Fresh AdamW moments and step counter for ``param`` (a sharded optimizer keeps less)."""
-        init_adamw_state(param, self.state[param])
+        init_adamw_state(param, self.state[param], bits)
 
     def initialize_state(self, param: Tensor) -> None:
         """Create a parameter's fresh state before its first step, without updating it.
@@ -221,7 +237,7 @@ class _DionCore(Optimizer):
             self._ensure_buckets()
         elif kind is RouteKind.ADAMW:
             if EXP_AVG_STATE not in self.state[param]:
-                self._new_adamw_state(param)
+                self._new_adamw_state(param, owner.get(ADAMW_STATE_BITS_KEY, 32))
         else:
             raise RuntimeError(f"Unhandled RouteKind: {kind}")
 
@@ -235,8 +251,24 @@ class _DionCore(Optimizer):
         saved = _fill_legacy_keys(state_dict["param_groups"])
         _require_same_structure(saved, self.param_groups)
         super().load_state_dict({**state_dict, "param_groups": saved})
+        self._restore_adamw8_state()
         self._buckets = None
         self._graph = self._graph_warm = None
+
+    def _restore_adamw8_state(self) -> None:
+        """torch's loader casts floating state to the parameter's dtype: 8-bit moments come back as the fp32 values of
+        their codes, which turn into the same codes again."""
+        for group in self.param_groups:
+            if group.get(ADAMW_STATE_BITS_KEY, 32) != 8:
+                continue
+            for param in group["params"]:
+                entry = self.state.get(param)
+                if not entry or EXP_AVG_STATE not in entry:
+                    continue
+                for key, dtype in ((EXP_AVG_STATE, MEAN_DTYPE), (EXP_AVG_SQ_STATE, SQUARE_DTYPE)):
+                    if EXP_AVG_SCALE_STATE in entry:
+                        entry[key] = entry[key].to(dtype).contiguous()
+                require_adamw8_state(param, entry)
 
     @torch.no_grad()
     def step(self, closure: Callable[[], float] | None = None) -> float | None:
@@ -366,7 +398,8 @@ class _DionCore(Optimizer):
                 parts.append((p.data_ptr(), p.grad.data_ptr()))
                 if adamw:   # a loaded checkpoint replaces these tensors
                     entry = self.state[p]
-                    parts.append(tuple(entry[key].data_ptr() for key in (EXP_AVG_STATE, EXP_AVG_SQ_STATE, ADAMW_STEP_STATE)
+                    parts.append(tuple(entry[key].data_ptr() for key in (EXP_AVG_STATE, EXP_AVG_SQ_STATE, EXP_AVG_SCALE_STATE,
+                                                                            EXP_AVG_SQ_SCALE_STATE, ADAMW_STEP_STATE)
                                        if key in entry))
         for bucket, run in runs:
             parts.append((bucket.momentum.data_ptr(), bucket.variance.data_ptr(), tuple(run)))
@@ -505,6 +538,9 @@ class Dion(IntegratedEMAOptimizer, _DionCore):
         matrix_update: ``DION3_UPDATE`` (default) or ``MUON_UPDATE``.
         ema: EMA schedule and placement, or None.
         profile_region: Named profiling region entered around EMA work.
+        adamw_state_bits: 32, or 8 to hold the moments of AdamW-routed parameters as 8-bit codes with a scale for
+            each 128 elements (``adamw8_step``): 2.1 bytes an element instead of 8.  A group may have its own
+            ``"adamw_state_bits"``.
 
     Raises:
         TypeError: For groups without a route or non-float32 parameters.
@@ -515,7 +551,9 @@ class Dion(IntegratedEMAOptimizer, _DionCore):
     def __init__(self, params: Iterable[dict[str, Any]], *, lr: float, momentum: float = 0.95,
                  muon_beta2: float = 0.95, betas: tuple[float, float] = (0.9, 0.95),
                  weight_decay: float = 0.0, eps: float = 1e-8, matrix_update: MatrixUpdate = DION3_UPDATE,
-                 ema: EMAConfig | None = None, profile_region: ProfileRegion = no_profile) -> None:
+                 ema: EMAConfig | None = None, profile_region: ProfileRegion = no_profile,
+                 adamw_state_bits: int = 32) -> None:
         super().__init__(params, lr=lr, momentum=momentum, muon_beta2=muon_beta2, betas=betas,
-                         weight_decay=weight_decay, eps=eps, matrix_update=matrix_update)
+                         weight_decay=weight_decay, eps=eps, matrix_update=matrix_update,
+                         adamw_state_bits=adamw_state_bits)
         self._init_integrated_ema(ema, profile_region)

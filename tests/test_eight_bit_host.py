@@ -197,3 +197,28 @@ def test_float8_linear_refuses() -> None:
     groups, report = dionw.param_groups(torch.nn.Sequential(torch.nn.Linear(64, 64), dionw.Float8Linear(64, 64)))
     assert [g["dion_route"] for g in groups] == ["adamw", "matrix"] and len(groups[1]["params"]) == 2
     assert isinstance(layer, torch.nn.Linear)
+
+
+# ---------------------------------------------------------------------------
+# Dion's option
+# ---------------------------------------------------------------------------
+def test_dion_state_bits_are_checked() -> None:
+    from dionw_b200._keys import ADAMW_STATE_BITS_KEY
+    from dionw_b200.optimizer import _require_group, _require_same_structure
+
+    assert ADAMW_STATE_BITS_KEY == "adamw_state_bits"
+    with pytest.raises(ValueError, match="adamw_state_bits must be 8 or 32"):
+        dionw.Dion([], lr=1e-3, adamw_state_bits=16)
+    common = {"params": [], "newton_schulz": "gram", "row_normalization": "normuon", "momentum_form": "heavy_ball",
+              "lr": 1e-3, "weight_decay": 0.0, "fraction": 1.0, "num_heads": None}
+    for bits in (8, 32):
+        _require_group({**common, "dion_route": "adamw", "adamw_state_bits": bits})
+    with pytest.raises(ValueError, match="must be 8 or 32"):
+        _require_group({**common, "dion_route": "adamw", "adamw_state_bits": 4})
+    with pytest.raises(ValueError, match="matrix group"):
+        _require_group({**common, "dion_route": "matrix", "adamw_state_bits": 8})
+    plain = {**common, "dion_route": "adamw"}
+    _require_same_structure([plain], [{**plain, "adamw_state_bits": 32}])
+    for old, new in ((8, 32), (32, 8)):
+        with pytest.raises(ValueError, match="checkpoint=%d, optimizer=%d" % (old, new)):
+            _require_same_structure([{**plain, "adamw_state_bits": old}], [{**plain, "adamw_state_bits": new}])
