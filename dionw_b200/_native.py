@@ -109,6 +109,14 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
         c_int, (c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                 c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
                 c_void_p)),
+    "dionw_column_sums": (c_int, (c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p)),
+    "dionw_float8_packed_bytes": (c_size_t, (c_int64, c_int64, c_int)),
+    "dionw_float8_linear_forward": (
+        c_int, (c_void_p, c_int, c_int64, c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64,
+                c_void_p, c_void_p, c_void_p, c_void_p)),
+    "dionw_float8_linear_backward": (
+        c_int, (c_void_p, c_int, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                c_void_p, c_void_p, c_void_p)),
     "dionw_ema_multi": (c_int, (_PP, _PP, _I64P, c_int, c_int, c_float, c_int, c_void_p)),
     "dionw_ema_stage_pack": (c_int, (_PP, _I64P, _I64P, c_int, c_int, c_void_p, c_void_p)),
     "dionw_cpu_ema_job_start": (c_void_p, (_PP, _PP, _I64P, POINTER(c_uint8), c_int, c_float, c_void_p, c_int)),
@@ -412,6 +420,27 @@ def float8_product(device: int, a: tuple[int, int, int, int, int, bool], b: tupl
     on_device(device, library().dionw_float8_product, *a, *b, None if bias is None else bias.data_ptr(),
               0 if bias is None else _DTYPE_CODE[bias.dtype], out.data_ptr(), out.stride(0) if m > 1 else n,
               _DTYPE_CODE[out.dtype], accumulate, m, n, k, *exponents)
+
+
+def float8_packed_bytes(rows: int, cols: int, tiles: bool) -> int:
+    """Bytes of a packed matrix: codes, scales and exponents."""
+    return int(library().dionw_float8_packed_bytes(rows, cols, tiles))
+
+
+def float8_linear_forward(x: Tensor, ldx: int, weight: Tensor, ldw: int, bias: Tensor | None, y: Tensor, inputs: int,
+                          work: Tensor, x_kept: Tensor | None, weight_kept: Tensor | None) -> None:
+    tokens, outputs = y.shape
+    on_device(y.get_device(), library().dionw_float8_linear_forward, x.data_ptr(), _DTYPE_CODE[x.dtype], ldx,
+              weight.data_ptr(), _DTYPE_CODE[weight.dtype], ldw, _ptr(bias), 0 if bias is None else _DTYPE_CODE[bias.dtype],
+              y.data_ptr(), tokens, inputs, outputs, work.data_ptr(), _ptr(x_kept), _ptr(weight_kept))
+
+
+def float8_linear_backward(dy: Tensor, ldy: int, dx: Tensor | None, dw: Tensor | None, db: Tensor | None, tokens: int,
+                           inputs: int, outputs: int, work: Tensor | None, x_kept: Tensor | None,
+                           weight_kept: Tensor | None) -> None:
+    on_device(dy.get_device(), library().dionw_float8_linear_backward, dy.data_ptr(), _DTYPE_CODE[dy.dtype], ldy, _ptr(dx),
+              0 if dx is None else _DTYPE_CODE[dx.dtype], _ptr(dw), 0 if dw is None else _DTYPE_CODE[dw.dtype], _ptr(db),
+              tokens, inputs, outputs, _ptr(work), _ptr(x_kept), _ptr(weight_kept))
 
 
 # ---------------------------------------------------------------------------

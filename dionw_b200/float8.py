@@ -11,6 +11,7 @@ There is no counterpart in the reference.
 
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 from typing import Any
 
@@ -202,82 +203,34 @@ def _operand(x: Float8Matrix) -> tuple[int, int, int, int, int, bool]:
             scales.shape[0] != rows)
 
 
-class _Buffer:
-    """A matrix, its scales and their exponents in one piece of memory, by address: what ``_Linear`` makes for itself and
-    passes on.
-
-    It takes a tensor, a view and a check less for each operand than a ``Float8Matrix``, 10 us of host time.
-    """
-
-    def __init__(self, rows: int, cols: int, tiles: bool) -> None:
-        self.ld = _padded(cols)
-        # scales of single rows: block after block, of tiles: tile row after tile row
-        self.lds = _blocks(cols) if tiles else rows
-        self.scales_at = (rows * self.ld + 255) // 256 * 256
-        high, wide = _blocks(rows), _blocks(cols)
-        self.exponents_at = self.scales_at + (4 * self.lds * (high if tiles else wide) + 255) // 256 * 256
-        self.nbytes = self.exponents_at + 4 * BLOCK * high * wide
-        self.tiles = tiles
-
-    def target(self, base: int) -> tuple[int, int, int, int]:
-        """As the quantizer writes it."""
-        return base, self.ld, base + self.scales_at, self.lds
-
-    def operand(self, base: int) -> tuple[int, int, int, int, int, bool]:
-        """As the product reads it."""
-        return (base, self.ld, base + self.scales_at, *((self.lds, 1) if self.tiles else (1, self.lds)), self.tiles)
-
-
-_NOWHERE = (None, 0, None, 0)
-
-
-def _bytes(n: int, device: torch.device) -> Tensor:
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def _quantize_into(device: int, x: Tensor, tiles: bool, first: tuple[_Buffer, int] | None,
-                   second: tuple[_Buffer, int] | None) -> None:
-    """``x`` and its transpose into buffers at those addresses."""
-    x, ldx = _with_rows(x)
-    rows, cols = x.shape
-    if rows and cols:
-        _native.float8_quantize(
-            device, x.data_ptr(), x.dtype, rows, cols, ldx, tiles,
-            *(_NOWHERE if first is None else first[0].target(first[1])),
-            *(_NOWHERE if second is None else second[0].target(second[1])),
-            None if first is None else first[1] + first[0].exponents_at,
-            None if second is None else second[1] + second[0].exponents_at)
-
-
-def _multiply(device: int, a: tuple[_Buffer, int], b: tuple[_Buffer, int], bias: Tensor | None, out: Tensor, m: int, n: int,
-              k: int) -> None:
-    if m and n:
-        _native.float8_product(device, a[0].operand(a[1]), b[0].operand(b[1]), bias, out, False, m, n, k,
-                               (a[1] + a[0].exponents_at, b[1] + b[0].exponents_at))
+@functools.lru_cache(maxsize=256)
+def _packed_bytes(rows: int, cols: int, tiles: bool) -> int:
+    return _native.float8_packed_bytes(rows, cols, tiles)
 
 
 class _Linear(torch.autograd.Function):
-    """``x @ weight.T`` on 8-bit products; every operand is quantized along the side that is summed over."""
+    """``x @ weight.T`` on 8-bit products; every operand is quantized along the side that is summed over.
+
+    A pass is one call into the library: a layer's host time is most of what small ones take.
+    """
 
     @staticmethod
     def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
         need_x, need_w, _ = ctx.needs_input_grad
-        (tokens, inputs), outputs = x.shape, weight.shape[0]
-        device, number = x.device, x.get_device()
-        # What the backward pass needs, the transposed matrices, a byte an element; and what this one does.
-        x_rows, w_tiles = _Buffer(tokens, inputs, False), _Buffer(outputs, inputs, True)
-        w_at = (x_rows.nbytes + 255) // 256 * 256
-        work = _bytes(w_at + w_tiles.nbytes, device)
-        base = work.data_ptr()
-        x_columns, w_turned = _Buffer(inputs, tokens, False), _Buffer(inputs, outputs, True)
-        x_kept = _bytes(x_columns.nbytes, device) if need_w else None
-        w_kept = _bytes(w_turned.nbytes, device) if need_x else None
-        _quantize_into(number, x, False, (x_rows, base), None if x_kept is None else (x_columns, x_kept.data_ptr()))
-        _quantize_into(number, weight, True, (w_tiles, base + w_at),
-                       None if w_kept is None else (w_turned, w_kept.data_ptr()))
+        (tokens, inputs), outputs, device = x.shape, weight.shape[0], x.device
+        x_rows, ldx = _with_rows(x)
+        w_rows, ldw = _with_rows(weight)
+
+        def room(nbytes: int) -> Tensor:
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+        # What the backward pass needs, a byte an element: the packed transposes of both.
+        x_kept = room(_packed_bytes(inputs, tokens, False)) if need_w else None
+        w_kept = room(_packed_bytes(inputs, outputs, True)) if need_x else None
+        work = room(_packed_bytes(tokens, inputs, False) + _packed_bytes(outputs, inputs, True))
         y = torch.empty(tokens, outputs, dtype=x.dtype, device=device)
-        _multiply(number, (x_rows, base), (w_tiles, base + w_at), None if bias is None else bias.contiguous(), y, tokens,
-                  outputs, inputs)
+        _native.float8_linear_forward(x_rows, ldx, w_rows, ldw, None if bias is None else bias.contiguous(), y, inputs, work,
+                                      x_kept, w_kept)
         ctx.save_for_backward(x_kept, w_kept)
         ctx.made_of = (tokens, inputs, outputs, x.dtype, weight.dtype, None if bias is None else bias.dtype)
         return y
@@ -288,26 +241,15 @@ class _Linear(torch.autograd.Function):
         need_x, need_w, need_b = ctx.needs_input_grad
         tokens, inputs, outputs, x_dtype, w_dtype, b_dtype = ctx.made_of
         x_kept, w_kept = ctx.saved_tensors
-        device, number = grad.device, grad.get_device()
-        dx = dw = db = None
-        if need_x or need_w:
-            rows, columns = _Buffer(tokens, outputs, False), _Buffer(outputs, tokens, False)
-            columns_at = (rows.nbytes + 255) // 256 * 256 if need_x else 0
-            work = _bytes(columns_at + (columns.nbytes if need_w else 0), device)
-            base = work.data_ptr()
-            _quantize_into(number, grad, False, (rows, base) if need_x else None,
-                           (columns, base + columns_at) if need_w else None)
-            if need_x:
-                dx = torch.empty(tokens, inputs, dtype=x_dtype, device=device)
-                _multiply(number, (rows, base), (_Buffer(inputs, outputs, True), w_kept.data_ptr()), None, dx, tokens, inputs,
-                          outputs)
-            if need_w:
-                dw = torch.empty(outputs, inputs, dtype=w_dtype, device=device)
-                _multiply(number, (columns, base + columns_at), (_Buffer(inputs, tokens, False), x_kept.data_ptr()), None, dw,
-                          outputs, inputs, tokens)
-        if need_b:
-            db = grad.sum(0, dtype=torch.float32).to(b_dtype)
-        return dx, dw, db
+        device = grad.device
+        dx = torch.empty(tokens, inputs, dtype=x_dtype, device=device) if need_x else None
+        dw = torch.empty(outputs, inputs, dtype=w_dtype, device=device) if need_w else None
+        db = torch.empty(outputs, dtype=torch.float32, device=device) if need_b else None
+        work = torch.empty((_packed_bytes(tokens, outputs, False) if need_x else 0)
+                           + (_packed_bytes(outputs, tokens, False) if need_w else 0), dtype=torch.uint8, device=device)
+        dy, ldy = _with_rows(grad)
+        _native.float8_linear_backward(dy, ldy, dx, dw, db, tokens, inputs, outputs, work, x_kept, w_kept)
+        return dx, dw, db if db is None or b_dtype is torch.float32 else db.to(b_dtype)
 
 
 def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:

@@ -291,6 +291,34 @@ int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int6
                          int out_dtype, int accumulate, int64_t m, int64_t n, int64_t k,
                          const uint32_t* a_exponents, const uint32_t* b_exponents, void* stream);
 
+/* out[c] = sum over r of x[r, c] in fp32, in a fixed order: the gradient of a bias. */
+int dionw_column_sums(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,
+                      float* out, void* stream);
+
+/* A linear layer's passes on these operators.  A packed matrix is what
+ * dionw_float8_quantize makes -- codes, scales, exponents -- in one 256-byte aligned buffer of
+ * dionw_float8_packed_bytes() bytes, whose inside is the library's own. */
+size_t dionw_float8_packed_bytes(int64_t rows, int64_t cols, int tiles);
+
+/* y = x weight^T + bias (nullable): x [tokens, ldx], weight [outputs, ldw] (inputs columns each),
+ * y [tokens, outputs] of x's dtype.  work holds a packed [tokens, inputs] matrix and, behind it, a
+ * packed one of tiles [outputs, inputs].  x_kept (nullable) receives the packed transpose
+ * [inputs, tokens] of x, which the weight's gradient needs, weight_kept (nullable) that of the
+ * weight [inputs, outputs] in tiles, for x's gradient. */
+int dionw_float8_linear_forward(const void* x, int x_dtype, int64_t ldx, const void* weight,
+                                int weight_dtype, int64_t ldw, const void* bias, int bias_dtype,
+                                void* y, int64_t tokens, int64_t inputs, int64_t outputs,
+                                void* work, void* x_kept, void* weight_kept, void* stream);
+
+/* From y's gradient dy [tokens, ldy]: dx [tokens, inputs] = dy weight, dw [outputs, inputs] =
+ * dy^T x and db [outputs] = dy's column sums, each where it is not null.  work holds a packed
+ * [tokens, outputs] matrix where dx is wanted and, behind it, a packed [outputs, tokens] one
+ * where dw is. */
+int dionw_float8_linear_backward(const void* dy, int dy_dtype, int64_t ldy, void* dx, int dx_dtype,
+                                 void* dw, int dw_dtype, float* db, int64_t tokens, int64_t inputs,
+                                 int64_t outputs, void* work, const void* x_kept,
+                                 const void* weight_kept, void* stream);
+
 /* ---- NorMuon and the weight update -------------------------------------- */
 
 /* s[b*k + r] = sum_c o[b, r, c]^2 for a bf16 batch [blocks, k, ldo] (used where

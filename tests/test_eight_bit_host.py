@@ -222,3 +222,22 @@ def test_dion_state_bits_are_checked() -> None:
     for old, new in ((8, 32), (32, 8)):
         with pytest.raises(ValueError, match="checkpoint=%d, optimizer=%d" % (old, new)):
             _require_same_structure([{**plain, "adamw_state_bits": old}], [{**plain, "adamw_state_bits": new}])
+
+
+def test_linear_entries_refuse() -> None:
+    lib = _native.library()
+    at = 1 << 20
+    assert lib.dionw_float8_packed_bytes(-1, 4, 0) == 0 and lib.dionw_float8_packed_bytes(0, 0, 0) == 256
+    # codes 130 x 304, scales 3 x 130, exponents 3 x 2 x 128, each from a multiple of 256 bytes on
+    assert lib.dionw_float8_packed_bytes(130, 300, 0) == 39680 + 1792 + 3072
+    assert lib.dionw_float8_packed_bytes(130, 300, 1) == 39680 + 256 + 3072
+    assert lib.dionw_float8_linear_forward(at, 0, 8, at, 0, 8, None, 0, at, -1, 8, 8, at, None, None, None) == -1
+    assert "bad shape" in _native.last_error()
+    assert lib.dionw_float8_linear_backward(at, 0, 8, at, 0, None, 0, None, 4, 8, 8, at, None, None, None) == -1
+    assert "keeps" in _native.last_error()
+    assert lib.dionw_float8_linear_backward(at, 0, 8, None, 0, at, 0, None, 4, 8, 8, at, None, at, None) == -1
+    assert lib.dionw_column_sums(None, 0, 0, 0, 0, None, None) == 0
+    for call in ((at, 3, 4, 8, 8, at, None), (at, 0, -1, 8, 8, at, None), (None, 0, 4, 8, 8, at, None),
+                 (at, 0, 4, 8, 7, at, None), (at, 0, 4, 8, 8, None, None)):
+        assert lib.dionw_column_sums(*call) == -1
+        assert "column_sums" in _native.last_error()

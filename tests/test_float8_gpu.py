@@ -305,6 +305,21 @@ def test_linear_gradients_are_those_of_differences() -> None:
         assert difference == pytest.approx(float(grad.double().norm()), rel=0.05)
 
 
+@pytest.mark.parametrize("rows,cols,shift", [(1, 1, 0), (0, 5, 0), (7, 33, 0), (1000, 130, 1), (33, 2000, 0), (4097, 64, 0)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_column_sums(rows, cols, shift, dtype) -> None:
+    """A column's 64 partial sums are each of rows / 64 values: rows / 64 + 64 roundings of 2^-24."""
+    from dionw_b200 import _native
+
+    room = _matrix(rows, cols + shift + 3, 1, dtype).to(DEV)
+    x = room[:, shift:cols + shift]
+    out = torch.full((cols + 1,), 7.0, device=DEV)
+    _native.on_device(0, _native.library().dionw_column_sums, x.data_ptr(), _native.dtype_code(dtype), rows, cols,
+                      room.stride(0), out.data_ptr())
+    want, size = x.double().sum(0), x.double().abs().sum(0)
+    assert bool(((out[:cols].double() - want).abs() <= (rows / 64 + 66) * 2.0**-24 * size).all()) and float(out[cols]) == 7.0
+
+
 def test_linear_of_any_leading_shape_and_partial_gradients() -> None:
     x = _matrix(24, 64, 8, torch.bfloat16).view(2, 3, 4, 64).to(DEV)
     layer = dionw.Float8Linear(64, 48, device=DEV)
