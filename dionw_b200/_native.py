@@ -108,7 +108,8 @@ SIGNATURES: dict[str, tuple[object, tuple[object, ...]]] = {
     "dionw_float8_product": (
         c_int, (c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_void_p, c_int64, c_int64,
                 c_int, c_void_p, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p,
-                c_void_p)),
+                c_void_p, c_size_t, c_void_p)),
+    "dionw_float8_product_workspace_bytes": (c_size_t, (c_int64, c_int64, c_int64)),
     "dionw_column_sums": (c_int, (c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p)),
     "dionw_float8_packed_bytes": (c_size_t, (c_int64, c_int64, c_int)),
     "dionw_float8_linear_forward": (
@@ -412,14 +413,21 @@ def float8_quantize(device: int, x: int, dtype: torch.dtype, rows: int, cols: in
               qt, ldqt, scales_t, ldst, exponents, exponents_t)
 
 
+def float8_product_workspace_bytes(device: int, m: int, n: int, k: int) -> int:
+    """Scratch with which a product of this shape looks at its scales on that device; 0: it does not."""
+    with torch.cuda.device(device):
+        return int(library().dionw_float8_product_workspace_bytes(m, n, k))
+
+
 def float8_product(device: int, a: tuple[int, int, int, int, int, bool], b: tuple[int, int, int, int, int, bool],
                    bias: Tensor | None, out: Tensor, accumulate: bool, m: int, n: int, k: int,
-                   exponents: tuple[int | None, int | None] = (None, None)) -> None:
+                   workspace: Tensor | None) -> None:
     """``a`` and ``b``: address and leading dimension of the codes, address and the two strides of the scales, and
-    whether those are tiles'; ``exponents``: the scales as the quantizer wrote them a second time."""
+    whether those are tiles'."""
     on_device(device, library().dionw_float8_product, *a, *b, None if bias is None else bias.data_ptr(),
               0 if bias is None else _DTYPE_CODE[bias.dtype], out.data_ptr(), out.stride(0) if m > 1 else n,
-              _DTYPE_CODE[out.dtype], accumulate, m, n, k, *exponents)
+              _DTYPE_CODE[out.dtype], accumulate, m, n, k, None, None,
+              *((None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())))
 
 
 def float8_packed_bytes(rows: int, cols: int, tiles: bool) -> int:

@@ -41,7 +41,7 @@ int multiply(const Packed& x, const void* a, const Packed& y, const void* b, con
              int out_dtype, void* stream) {
   return dionw_float8_product(x.codes(a), x.ld, x.scales(a), x.tiles ? x.lds : 1, x.tiles ? 1 : x.lds, x.tiles, y.codes(b), y.ld,
                               y.scales(b), y.tiles ? y.lds : 1, y.tiles ? 1 : y.lds, y.tiles, bias, bias_dtype, out, y.rows,
-                              out_dtype, 0, x.rows, y.rows, x.cols, x.exponents(a), y.exponents(b), stream);
+                              out_dtype, 0, x.rows, y.rows, x.cols, x.exponents(a), y.exponents(b), nullptr, 0, stream);
 }
 
 // ---------------------------------------------------------------------------

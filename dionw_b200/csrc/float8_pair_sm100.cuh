@@ -67,7 +67,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int first_tile = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int total_tiles = p.tiles_m * p.tiles_n;
+  int total_tiles = p.tiles_m * p.tiles_n;
   const int k_blocks = (p.k + kBK - 1) / kBK;
 
   if (threadIdx.x == 0) {
@@ -95,6 +95,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
   griddep_launch();
+  // Scales that are all powers of two have been left to the tensor cores: nothing is left to do.
+  if (p.odd_scales != nullptr && !any_odd_scale(p)) total_tiles = 0;
 
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, p.wait_ns)) != 0;

@@ -83,9 +83,9 @@ int launch_clusters_of_two(Kernel kernel, size_t smem, int threads, float8::Para
   return check_cuda(cudaLaunchKernelEx(&config, kernel, maps..., p), "product_kernel launch");
 }
 
-int count_pair_tiles(float8::Params& p) {
+int count_pair_tiles(float8::Params& p, int tile_n) {
   p.tiles_m = (p.m + float8::pair::kPairM - 1) / float8::pair::kPairM;
-  p.tiles_n = (p.n + float8::pair::kPairN - 1) / float8::pair::kPairN;
+  p.tiles_n = (p.n + tile_n - 1) / tile_n;
   DIONW_REQUIRE((long long)p.tiles_m * p.tiles_n <= 0x7FFFFFFFll, "float8_product: too many tiles");
   return DIONW_OK;
 }
@@ -106,33 +106,92 @@ int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8:
     st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, pair::kPairN / 2);
     if (st != DIONW_OK) return st;
   }
-  st = count_pair_tiles(p);
+  st = count_pair_tiles(p, pair::kPairN);
   if (st != DIONW_OK) return st;
   return launch_clusters_of_two(kernel, pair::kSmemBytes<kRowScales>, pair::kThreads, p, stream, map_a, map_b);
 }
 
 // The same with exponents that the tensor cores apply.
-template <typename T>
+template <typename T, int kTileN>
 int launch_scaled(const void* a, int64_t lda, const void* a_exponents, const void* b, int64_t ldb, const void* b_exponents,
                   float8::Params p, cudaStream_t stream) {
   namespace scaled = float8::scaled;
-  static_assert(scaled::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = scaled::product_kernel<T>;
+  static_assert(scaled::Shape<kTileN>::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = scaled::product_kernel<T, kTileN>;
   static std::atomic<bool> configured[kMaxDevices];
-  int st = allow_shared(kernel, scaled::kSmemBytes, configured);
+  int st = allow_shared(kernel, scaled::Shape<kTileN>::kSmemBytes, configured);
   if (st != DIONW_OK) return st;
   scaled::Maps maps;
   const int64_t blocks = (p.k + 127) / 128;
   st = make_byte_map(&maps.a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
-  if (st == DIONW_OK) st = make_byte_map(&maps.b, b, p.k, p.n, ldb, float8::kBK, scaled::kPairN / 2);
+  if (st == DIONW_OK) st = make_byte_map(&maps.b, b, p.k, p.n, ldb, float8::kBK, kTileN / 2);
   if (st == DIONW_OK) st = make_word_map(&maps.a_scales, a_exponents, blocks * ((p.m + 127) / 128), 1);
-  if (st == DIONW_OK) st = make_word_map(&maps.b_scales, b_exponents, blocks * ((p.n + 127) / 128), 2);
-  if (st == DIONW_OK) st = count_pair_tiles(p);
+  if (st == DIONW_OK) st = make_word_map(&maps.b_scales, b_exponents, blocks * ((p.n + 127) / 128), kTileN / 128);
+  if (st == DIONW_OK) st = count_pair_tiles(p, kTileN);
   if (st != DIONW_OK) return st;
-  return launch_clusters_of_two(kernel, scaled::kSmemBytes, scaled::kThreads, p, stream, maps);
+  return launch_clusters_of_two(kernel, scaled::Shape<kTileN>::kSmemBytes, scaled::kThreads, p, stream, maps);
+}
+
+// ---------------------------------------------------------------------------
+// exponents of scales of any strides
+// ---------------------------------------------------------------------------
+constexpr int kExponentThreads = 256, kExponentCtas = 128;
+
+struct ExponentJob {
+  float8::Scales scales;
+  uint32_t* out;
+  int rows, atoms;
+  long long words;         // blocks * atoms * 128
+};
+
+// The exponents of both operands' scales, and one word a CTA that says whether one of its scales is neither a power of two nor
+// NaN.  Row 32 c + l of 128 is word 4 l + c; rows behind the matrix get 1.
+__global__ void __launch_bounds__(kExponentThreads)
+exponents_kernel(const ExponentJob a, const ExponentJob b, int* odd) {
+  after_previous();
+  bool mine = false;
+  for (long long i = (long long)blockIdx.x * kExponentThreads + threadIdx.x; i < a.words + b.words;
+       i += (long long)gridDim.x * kExponentThreads) {
+    const bool second = i >= a.words;
+    const ExponentJob& job = second ? b : a;
+    const long long word = second ? i - a.words : i;
+    const long long atom = word >> 7, block = atom / job.atoms;
+    const int within = int(word & 127);
+    const long long row = (atom - block * job.atoms) * 128 + 32 * (within & 3) + (within >> 2);
+    uint32_t bits = 0x3F800000u;
+    if (row < job.rows)
+      bits = __float_as_uint(job.scales.base[(row >> job.scales.shift) * job.scales.row_stride + block * job.scales.block_stride]);
+    const uint32_t exponent = (bits >> 23) & 0xFFu;
+    const bool nan = (bits & 0x7FFFFFFFu) > 0x7F800000u;
+    mine = mine || (!nan && ((bits & 0x807FFFFFu) != 0 || exponent == 0 || exponent == 255));
+    job.out[word] = exponent;
+  }
+  const int any = __syncthreads_or(mine);
+  if (threadIdx.x == 0) odd[blockIdx.x] = any;
 }
 
 long long pair_tiles(long long m, long long n) { return ((m + 255) / 256) * ((n + 255) / 256); }
+
+// Products with a tile for every SM pair are left to the tensor cores where their scales are powers of two.
+bool takes_exponents(long long m, long long n, long long k) { return k > 0 && pair_tiles(m, n) >= sm_count() / 2; }
+
+// Scratch of a product whose scales are looked at: a word a CTA, and both operands' exponents.
+struct ExponentRoom {
+  size_t a_at, b_at, bytes;
+  ExponentRoom(long long m, long long n, long long k) {
+    const long long blocks = (k + 127) / 128;
+    a_at = 4 * kExponentCtas;
+    b_at = a_at + 512 * size_t(blocks * ((m + 127) / 128));
+    bytes = b_at + 512 * size_t(blocks * ((n + 127) / 128));
+  }
+};
+
+template <typename T>
+int run_scaled(const void* a, int64_t lda, const void* ea, const void* b, int64_t ldb, const void* eb, const float8::Params& p,
+               cudaStream_t stream) {
+  if (pair_tiles(p.m, p.n) >= sm_count() / 2) return launch_scaled<T, 256>(a, lda, ea, b, ldb, eb, p, stream);
+  return launch_scaled<T, 128>(a, lda, ea, b, ldb, eb, p, stream);
+}
 
 // The kernel for a product of this shape.
 template <typename T>
@@ -156,12 +215,18 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p
 
 using namespace dionw;
 
+extern "C" size_t dionw_float8_product_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+  if (m <= 0 || n <= 0 || !takes_exponents(m, n, k)) return 0;
+  return ExponentRoom(m, n, k).bytes;
+}
+
 extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int64_t a_row_stride,
                                     int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
                                     const float* b_scales, int64_t b_row_stride, int64_t b_block_stride, int b_tiles,
                                     const void* bias, int bias_dtype, void* out, int64_t ldo, int out_dtype,
                                     int accumulate, int64_t m, int64_t n, int64_t k, const uint32_t* a_exponents,
-                                    const uint32_t* b_exponents, void* stream_ptr) {
+                                    const uint32_t* b_exponents, void* workspace, size_t workspace_bytes,
+                                    void* stream_ptr) {
   DIONW_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= 0x7FFFFF00ll && n <= 0x7FFFFF00ll && k <= 0x7FFFFF00ll,
                 "float8_product: bad shape %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
   DIONW_REQUIRE(out_dtype >= DIONW_F32 && out_dtype <= DIONW_BF16, "float8_product: bad output dtype");
@@ -189,11 +254,39 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
   p.status = device_status_word();
   p.wait_ns = gemm::kWaitLimitNs;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (a_exponents != nullptr && b_exponents != nullptr && k > 0 && pair_tiles(m, n) >= sm_count() / 2) {
+  auto scaled = [&](const uint32_t* ea, const uint32_t* eb) {
+    if (out_dtype == DIONW_F32) return run_scaled<float>(a, lda, ea, b, ldb, eb, p, stream);
+    if (out_dtype == DIONW_F16) return run_scaled<__half>(a, lda, ea, b, ldb, eb, p, stream);
+    return run_scaled<__nv_bfloat16>(a, lda, ea, b, ldb, eb, p, stream);
+  };
+  if (a_exponents != nullptr && b_exponents != nullptr && k > 0 && m > 64) {
     DIONW_REQUIRE(aligned16(a_exponents) && aligned16(b_exponents), "float8_product: exponents must be 16-byte aligned");
-    if (out_dtype == DIONW_F32) return launch_scaled<float>(a, lda, a_exponents, b, ldb, b_exponents, p, stream);
-    if (out_dtype == DIONW_F16) return launch_scaled<__half>(a, lda, a_exponents, b, ldb, b_exponents, p, stream);
-    return launch_scaled<__nv_bfloat16>(a, lda, a_exponents, b, ldb, b_exponents, p, stream);
+    return scaled(a_exponents, b_exponents);
+  }
+  if (takes_exponents(m, n, k)) {
+    const ExponentRoom room(m, n, k);
+    if (workspace != nullptr) {
+      DIONW_REQUIRE(aligned16(workspace), "float8_product: the workspace must be 16-byte aligned");
+      if (workspace_bytes < room.bytes) {
+        set_error("float8_product: workspace of %zu bytes, %zu needed", workspace_bytes, room.bytes);
+        return DIONW_ERR_WORKSPACE;
+      }
+      // Three launches: what the scales are, the product if they are powers of two, the product if they are not.  The one that has
+      // nothing to do costs 2 to 3 us of some hundred.
+      char* base = static_cast<char*>(workspace);
+      const long long blocks = (k + 127) / 128;
+      ExponentJob ja{p.a, reinterpret_cast<uint32_t*>(base + room.a_at), int(m), int((m + 127) / 128), 0};
+      ExponentJob jb{p.b, reinterpret_cast<uint32_t*>(base + room.b_at), int(n), int((n + 127) / 128), 0};
+      ja.words = blocks * ja.atoms * 128;
+      jb.words = blocks * jb.atoms * 128;
+      const long long ctas = (ja.words + jb.words + kExponentThreads - 1) / kExponentThreads;
+      p.odd_scales = static_cast<const int*>(workspace);
+      p.odd_parts = int(ctas < kExponentCtas ? ctas : kExponentCtas);
+      launch_dependent(exponents_kernel, unsigned(p.odd_parts), kExponentThreads, stream, ja, jb, static_cast<int*>(workspace));
+      int st = launch_status("exponents_kernel");
+      if (st == DIONW_OK) st = scaled(ja.out, jb.out);
+      if (st != DIONW_OK) return st;
+    }
   }
   if (out_dtype == DIONW_F32) return run<float>(a, lda, b, ldb, p, stream);
   if (out_dtype == DIONW_F16) return run<__half>(a, lda, b, ldb, p, stream);

@@ -9,7 +9,7 @@
 // one scale for 32 codes of a row; the four MMAs of a block use the same ones.
 //
 // A tile's 256 columns are half of TMEM and there is one of them: the eight warps take it into registers at once, and
-// convert and store while the next tile is computed.
+// convert and store while the next tile is computed.  Tiles of 256 x 128 are for products that have too few of the wide ones.
 #pragma once
 
 #include "float8_pair_sm100.cuh"
@@ -18,19 +18,26 @@ namespace dionw {
 namespace float8 {
 namespace scaled {
 
-using pair::kColumns;
 using pair::kPairM;
-using pair::kPairN;
 constexpr int kThreads = pair::kThreads;
-constexpr int kStages = 5;
 constexpr uint32_t kAtomBytes = 512;                       // the exponents of 128 rows
-constexpr uint32_t kCodeBytes = 2 * kABytes;               // 128 rows of A, 128 of B
-constexpr uint32_t kLoadBytes = kCodeBytes + 3 * kAtomBytes;
-constexpr uint32_t kStageBytes = (kLoadBytes + 1023) / 1024 * 1024;
 constexpr uint32_t kStagingBytes = kSumWarps * 32 * 128;
-constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + 256 + 1024;
-constexpr uint32_t kScaleColumns = 16;                     // of TMEM, for a block's exponents: 4 of A, 8 of B
+constexpr uint32_t kScaleColumns = 16;                     // of TMEM, for a block's exponents: 4 of A, 4 for each 128 of B
 constexpr uint32_t kScaleBuffers = 8;
+constexpr uint32_t kScalesAt = 256;                        // the columns behind the sums
+
+// kTileN: 256 or 128.
+template <int kTileN>
+struct Shape {
+  static constexpr int kColumns = kTileN / 2;                               // of a warp
+  static constexpr int kStages = kTileN == 256 ? 5 : 6;
+  static constexpr uint32_t kCodeBytes = kABytes + kTileN / 2 * kBK;        // 128 rows of A, half of B's
+  static constexpr uint32_t kAtoms = 1 + kTileN / 128;
+  static constexpr uint32_t kLoadBytes = kCodeBytes + kAtoms * kAtomBytes;
+  static constexpr uint32_t kStageBytes = (kLoadBytes + 1023) / 1024 * 1024;
+  static constexpr uint32_t kSums = 256 / kTileN;                           // accumulators
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + 256 + 1024;
+};
 
 struct Maps {
   CUtensorMap a, b, a_scales, b_scales;
@@ -62,24 +69,26 @@ constexpr uint32_t make_idesc(int m, int n) {
   return (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 4) << 24);
 }
 
-template <typename T>
+template <typename T, int kTileN>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const Params p) {
   using namespace gemm;
+  using S = Shape<kTileN>;
+  constexpr int kStages = S::kStages, kColumns = S::kColumns;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* staging = smem + size_t(kStages) * kStageBytes;
+  uint8_t* staging = smem + size_t(kStages) * S::kStageBytes;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + kStagingBytes);  // leader's: both CTAs' stage landed
   uint64_t* empty_bar = full_bar + kStages;            // both: the pair's MMAs on this stage completed
-  uint64_t* acc_full = empty_bar + kStages;            // both: the tile's sums are complete
-  uint64_t* acc_empty = acc_full + 1;                  // leader's: both CTAs have them in registers
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 1);
+  uint64_t* acc_full = empty_bar + kStages;            // [kSums] both: a tile's sums are complete
+  uint64_t* acc_empty = acc_full + S::kSums;           // [kSums] leader's: both CTAs have them in registers
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + S::kSums);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const int first_tile = blockIdx.x >> 1, pairs = gridDim.x >> 1;
-  const int total_tiles = p.tiles_m * p.tiles_n;
+  int total_tiles = p.tiles_m * p.tiles_n;
   const int k_blocks = (p.k + kBK - 1) / kBK;          // at least one
 
   if (threadIdx.x == 0) {
@@ -87,8 +96,10 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    mbar_init(acc_full, 1);
-    mbar_init(acc_empty, 2 * kSumWarps);
+    for (uint32_t a = 0; a < S::kSums; ++a) {
+      mbar_init(&acc_full[a], 1);
+      mbar_init(&acc_empty[a], 2 * kSumWarps);
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -105,6 +116,8 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
   griddep_launch();
+  // With a scale of any other value the kernel after this one does the work.
+  if (p.odd_scales != nullptr && any_odd_scale(p)) total_tiles = 0;
 
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, p.wait_ns)) != 0;
@@ -121,19 +134,19 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
     for (int t = first_tile; t < total_tiles && ok; t += pairs) {
       int tm, tn;
       tile_at(t, p, tm, tn);
-      const int m0 = tm * kPairM + int(rank) * kBM, n0 = tn * kPairN + int(rank) * (kPairN / 2);
+      const int m0 = tm * kPairM + int(rank) * kBM, n0 = tn * kTileN + int(rank) * (kTileN / 2);
       for (int kb = 0; kb < k_blocks; ++kb) {
         if (!warp_wait(&empty_bar[s], released)) { ok = false; break; }
         if (gemm2::elect_one()) {
-          const uint32_t dst = ring + uint32_t(s) * kStageBytes;
+          const uint32_t dst = ring + uint32_t(s) * S::kStageBytes;
           const uint32_t landed = leader_full + uint32_t(s) * uint32_t(sizeof(uint64_t));
           // The peer's bytes may land before the leader announces them: the phase cannot complete before its arrive.
-          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * kLoadBytes);
+          if (rank == 0) mbar_expect_tx(&full_bar[s], 2 * S::kLoadBytes);
           pair::tma_load_pair(dst, &maps.a, landed, kb * kBK, m0);
           pair::tma_load_pair(dst + kABytes, &maps.b, landed, kb * kBK, n0);
           // (the second half of a last tile may be past its block's exponents: those rows are not stored)
-          pair::tma_load_pair(dst + kCodeBytes, &maps.a_scales, landed, 0, kb * a_atoms + m0 / 128);
-          pair::tma_load_pair(dst + kCodeBytes + kAtomBytes, &maps.b_scales, landed, 0, kb * b_atoms + tn * 2);
+          pair::tma_load_pair(dst + S::kCodeBytes, &maps.a_scales, landed, 0, kb * a_atoms + m0 / 128);
+          pair::tma_load_pair(dst + S::kCodeBytes + kAtomBytes, &maps.b_scales, landed, 0, kb * b_atoms + tn * (kTileN / 128));
         }
         __syncwarp();
         if (++s == kStages) s = 0, released ^= 1u;
@@ -142,30 +155,31 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
   } else if (warp == 1) {
     if (rank == 0) {   // the second CTA's MMA warp has nothing to issue
       // ---------------------------------------------------------- MMA issuer (leader)
-      constexpr uint32_t idesc = make_idesc(kPairM, kPairN);
+      constexpr uint32_t idesc = make_idesc(kPairM, kTileN);
       int s = 0;
       uint32_t loaded = 0, local = 0, buffer = 0;
       bool ok = true;
       const uint32_t ring = smem_u32(smem);
       for (int t = first_tile; t < total_tiles && ok; t += pairs, ++local) {
-        if (!warp_wait(acc_empty, (local & 1u) ^ 1u)) break;
+        const uint32_t acc = local % S::kSums;
+        if (!warp_wait(&acc_empty[acc], ((local / S::kSums) & 1u) ^ 1u)) break;
         tc_fence_after();
         for (int kb = 0; kb < k_blocks; ++kb) {
           if (!warp_wait(&full_bar[s], loaded)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a_addr = ring + uint32_t(s) * kStageBytes;
+          const uint32_t a_addr = ring + uint32_t(s) * S::kStageBytes;
           const uint64_t a_desc = make_smem_desc(a_addr, 16, 1024), b_desc = make_smem_desc(a_addr + kABytes, 16, 1024);
-          const uint64_t scales = scale_desc(a_addr + kCodeBytes);
-          const uint32_t sa = tmem_base + uint32_t(kPairN) + buffer * kScaleColumns, sb = sa + 4;
+          const uint64_t scales = scale_desc(a_addr + S::kCodeBytes);
+          const uint32_t sa = tmem_base + kScalesAt + buffer * kScaleColumns, sb = sa + 4;
           if (gemm2::elect_one()) {
             copy_scales(sa, scales);
             copy_scales(sb, scales + (kAtomBytes >> 4));
-            copy_scales(sb + 4, scales + (2 * kAtomBytes >> 4));
+            if (kTileN == 256) copy_scales(sb + 4, scales + (2 * kAtomBytes >> 4));
 #pragma unroll
             for (int j = 0; j < kBK / 32; ++j)
-              umma2_scaled(tmem_base, a_desc + 2 * j, b_desc + 2 * j, idesc, sa, sb, kb > 0 || j > 0 ? 1u : 0u);
+              umma2_scaled(tmem_base + acc * kTileN, a_desc + 2 * j, b_desc + 2 * j, idesc, sa, sb, kb > 0 || j > 0 ? 1u : 0u);
             gemm2::umma2_commit_both(&empty_bar[s]);
-            if (kb + 1 == k_blocks) gemm2::umma2_commit_both(acc_full);
+            if (kb + 1 == k_blocks) gemm2::umma2_commit_both(&acc_full[acc]);
           }
           __syncwarp();
           buffer = (buffer + 1) % kScaleBuffers;
@@ -182,18 +196,19 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
     const uint32_t leader_empty = peer_address(acc_empty, 0);
     uint32_t local = 0;
     for (int t = first_tile; t < total_tiles; t += pairs, ++local) {
-      if (!warp_wait(acc_full, local & 1u)) break;
+      const uint32_t acc = local % S::kSums;
+      if (!warp_wait(&acc_full[acc], (local / S::kSums) & 1u)) break;
       tc_fence_after();
       uint32_t sum[kColumns];
 #pragma unroll
-      for (int c = 0; c < kColumns; c += 32) tmem_load<32>(tmem_mine + c, sum + c);
+      for (int c = 0; c < kColumns; c += 32) tmem_load<32>(tmem_mine + acc * kTileN + c, sum + c);
       tmem_wait<kColumns>(sum);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) gemm2::remote_arrive(leader_empty);
+      if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
       int tm, tn;
       tile_at(t, p, tm, tn);
-      write_sums<T, kColumns>(p, stage_out, tm * kPairM + int(rank) * kBM + sub * 32, tn * kPairN + half * kColumns, lane,
+      write_sums<T, kColumns>(p, stage_out, tm * kPairM + int(rank) * kBM + sub * 32, tn * kTileN + half * kColumns, lane,
                               [&](int c) { return __uint_as_float(sum[c]); });
     }
   }

@@ -192,8 +192,16 @@ def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = No
             raise ValueError(f"float8_product: bias must have {n} elements on {device}, got {tuple(bias.shape)} on {bias.device}")
         bias = bias.contiguous()
     if m and n:
-        _native.float8_product(out.get_device(), _operand(a), _operand(b), bias, out, accumulate, m, n, k)
+        number = out.get_device()
+        scratch = _product_scratch(number, m, n, k)
+        _native.float8_product(number, _operand(a), _operand(b), bias, out, accumulate, m, n, k,
+                               torch.empty(scratch, dtype=torch.uint8, device=device) if scratch else None)
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _product_scratch(device: int, m: int, n: int, k: int) -> int:
+    return _native.float8_product_workspace_bytes(device, m, n, k)
 
 
 def _operand(x: Float8Matrix) -> tuple[int, int, int, int, int, bool]:

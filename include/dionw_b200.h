@@ -283,13 +283,18 @@ int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, 
  * where a_tiles != 0 (b likewise).  out must not overlap an operand.  Results do not depend on
  * anything but the operands: sums are taken in a fixed order.  a_exponents and b_exponents
  * (both or neither, 16-byte aligned): the scales as dionw_float8_quantize wrote them a second
- * time; large products then leave them to the tensor cores and sum in one piece. */
+ * time; large products then leave them to the tensor cores and sum in one piece.  Without
+ * them, and with a workspace (nullable, 16-byte aligned, of the bytes that the function below
+ * says, 0 for small products), a large product first looks whether all scales are powers of two
+ * (or NaN) and does the same if so. */
 int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int64_t a_row_stride,
                          int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
                          const float* b_scales, int64_t b_row_stride, int64_t b_block_stride,
                          int b_tiles, const void* bias, int bias_dtype, void* out, int64_t ldo,
                          int out_dtype, int accumulate, int64_t m, int64_t n, int64_t k,
-                         const uint32_t* a_exponents, const uint32_t* b_exponents, void* stream);
+                         const uint32_t* a_exponents, const uint32_t* b_exponents,
+                         void* workspace, size_t workspace_bytes, void* stream);
+size_t dionw_float8_product_workspace_bytes(int64_t m, int64_t n, int64_t k);
 
 /* out[c] = sum over r of x[r, c] in fp32, in a fixed order: the gradient of a bias. */
 int dionw_column_sums(const void* x, int dtype, int64_t rows, int64_t cols, int64_t ldx,

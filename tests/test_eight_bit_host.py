@@ -172,7 +172,7 @@ def test_float8_product_entry_refuses() -> None:
 
     def call(a=at, lda=112, sa=at, b=at, ldb=112, sb=at, bias=None, bias_dtype=0, out=at, ldo=6, out_dtype=0, m=4, n=6, k=100):
         return lib.dionw_float8_product(a, lda, sa, 1, 4, 0, b, ldb, sb, 1, 6, 0, bias, bias_dtype, out, ldo, out_dtype, 0,
-                                        m, n, k, None, None, None)
+                                        m, n, k, None, None, None, 0, None)
 
     assert call(m=0) == 0 and call(n=0) == 0
     for bad, match in ((dict(m=-1), "shape"), (dict(k=1 << 33), "shape"), (dict(out_dtype=3), "output"),
@@ -181,6 +181,18 @@ def test_float8_product_entry_refuses() -> None:
                        (dict(lda=100), "16-byte"), (dict(ldb=104), "16-byte"), (dict(ldb=96), "16-byte")):
         assert call(**bad) == -1, bad
         assert match in _native.last_error(), (bad, _native.last_error())
+
+
+def test_float8_product_scratch() -> None:
+    lib = _native.library()
+    assert lib.dionw_float8_product_workspace_bytes(64, 4096, 4096) == 0
+    assert lib.dionw_float8_product_workspace_bytes(0, 1 << 20, 8) == 0
+    assert lib.dionw_float8_product_workspace_bytes(1 << 14, 1 << 14, 0) == 0
+    # 128 words, and 512 bytes for each 128 rows and block of both operands
+    assert lib.dionw_float8_product_workspace_bytes(8192, 14336, 4096) == 512 + 512 * 32 * (64 + 112)
+    status = lib.dionw_float8_product(1 << 20, 4096, 1 << 20, 1, 8192, 0, 1 << 20, 4096, 1 << 20, 1, 14336, 0, None, 0, 1 << 20,
+                                      14336, 0, 0, 8192, 14336, 4096, None, None, 1 << 20, 100, None)
+    assert status == -3 and "workspace" in _native.last_error()
 
 
 def test_float8_linear_refuses() -> None:

@@ -152,6 +152,34 @@ def test_product_of_many_tiles(m, n, k, b_tiles) -> None:
     _close(dionw.float8_product(a, b, out=held.to(DEV), accumulate=True), a64, b64, held.double())
 
 
+@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 300)])
+@pytest.mark.parametrize("b_tiles", [False, True])
+@pytest.mark.parametrize("layout", ["rows", "blocks"])
+def test_product_of_many_tiles_and_powers_of_two(m, n, k, b_tiles, layout) -> None:
+    """Scales that the tensor cores take; one other one, first or last of either operand, sends the product the other way."""
+    from dionw_b200 import _native
+
+    gen = torch.Generator().manual_seed(9)
+    (a, _), (b, _) = _operand(m, k, False, 1, layout), _operand(n, k, b_tiles, 2, layout)
+    for x in (a, b):
+        x.scales.copy_(torch.exp2(torch.randint(-20, 20, x.scales.shape, generator=gen).float()))
+
+    def values(x: Float8Matrix) -> Tensor:
+        return oracle.spread(x.values.cpu().float(), x.scales.cpu())
+
+    assert _native.float8_product_workspace_bytes(0, m, n, k) > 0
+    for dtype in DTYPES[:2]:
+        _close(dionw.float8_product(a, b, out_dtype=dtype), values(a), values(b))
+    for x, at in ((a, (0, 0)), (a, (-1, -1)), (b, (0, 0)), (b, (-1, -1))):
+        for other in (1.5, 0.0, -2.0, 2.0**-130):
+            kept = x.scales[at].clone()
+            x.scales[at] = other
+            _close(dionw.float8_product(a, b), values(a), values(b))
+            x.scales[at] = kept
+    a.scales[3, 1] = math.nan
+    assert dionw.float8_product(a, b).isnan().any(1).nonzero().flatten().tolist() == [3]
+
+
 @pytest.mark.parametrize("m", [40, 200])
 def test_product_with_weights_on_the_left(m) -> None:
     a, a64 = _operand(m, 700, True, 3)
