@@ -135,36 +135,44 @@ int launch_scaled(const void* a, int64_t lda, const void* a_exponents, const voi
 // ---------------------------------------------------------------------------
 // exponents of scales of any strides
 // ---------------------------------------------------------------------------
-constexpr int kExponentThreads = 256, kExponentCtas = 128;
+constexpr int kExponentThreads = 256, kExponentCtas = 296;
 
 struct ExponentJob {
   float8::Scales scales;
   uint32_t* out;
-  int rows, atoms;
-  long long words;         // blocks * atoms * 128
+  int rows, atoms;         // 128 rows of a block are an atom
+  long long all;           // blocks * atoms
 };
 
 // The exponents of both operands' scales, and one word a CTA that says whether one of its scales is neither a power of two nor
-// NaN.  Row 32 c + l of 128 is word 4 l + c; rows behind the matrix get 1.
+// NaN.  A warp takes an atom: lane l reads the scales of rows l, 32 + l, 64 + l and 96 + l and writes them as words 4 l .. 4 l + 3;
+// rows behind the matrix get 1.
 __global__ void __launch_bounds__(kExponentThreads)
 exponents_kernel(const ExponentJob a, const ExponentJob b, int* odd) {
   after_previous();
+  const int lane = threadIdx.x & 31;
   bool mine = false;
-  for (long long i = (long long)blockIdx.x * kExponentThreads + threadIdx.x; i < a.words + b.words;
-       i += (long long)gridDim.x * kExponentThreads) {
-    const bool second = i >= a.words;
+  for (long long i = ((long long)blockIdx.x * kExponentThreads + threadIdx.x) >> 5; i < a.all + b.all;
+       i += ((long long)gridDim.x * kExponentThreads) >> 5) {
+    const bool second = i >= a.all;
     const ExponentJob& job = second ? b : a;
-    const long long word = second ? i - a.words : i;
-    const long long atom = word >> 7, block = atom / job.atoms;
-    const int within = int(word & 127);
-    const long long row = (atom - block * job.atoms) * 128 + 32 * (within & 3) + (within >> 2);
-    uint32_t bits = 0x3F800000u;
-    if (row < job.rows)
-      bits = __float_as_uint(job.scales.base[(row >> job.scales.shift) * job.scales.row_stride + block * job.scales.block_stride]);
-    const uint32_t exponent = (bits >> 23) & 0xFFu;
-    const bool nan = (bits & 0x7FFFFFFFu) > 0x7F800000u;
-    mine = mine || (!nan && ((bits & 0x807FFFFFu) != 0 || exponent == 0 || exponent == 255));
-    job.out[word] = exponent;
+    const long long atom = second ? i - a.all : i, block = atom / job.atoms;
+    const long long row0 = (atom - block * job.atoms) * 128 + lane;
+    const float* base = job.scales.base + block * job.scales.block_stride;
+    uint32_t bits[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const long long row = row0 + 32 * c;
+      bits[c] = row < job.rows ? __float_as_uint(base[(row >> job.scales.shift) * job.scales.row_stride]) : 0x3F800000u;
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const bool nan = (bits[c] & 0x7FFFFFFFu) > 0x7F800000u;
+      const uint32_t exponent = (bits[c] >> 23) & 0xFFu;
+      mine = mine || (!nan && ((bits[c] & 0x807FFFFFu) != 0 || exponent == 0 || exponent == 255));
+      bits[c] = exponent;
+    }
+    reinterpret_cast<uint4*>(job.out)[atom * 32 + lane] = make_uint4(bits[0], bits[1], bits[2], bits[3]);
   }
   const int any = __syncthreads_or(mine);
   if (threadIdx.x == 0) odd[blockIdx.x] = any;
@@ -172,15 +180,22 @@ exponents_kernel(const ExponentJob a, const ExponentJob b, int* odd) {
 
 long long pair_tiles(long long m, long long n) { return ((m + 255) / 256) * ((n + 255) / 256); }
 
-// Products with a tile for every SM pair are left to the tensor cores where their scales are powers of two.
-bool takes_exponents(long long m, long long n, long long k) { return k > 0 && pair_tiles(m, n) >= sm_count() / 2; }
+// Whether a product looks at its scales, to leave them to the tensor cores where they are powers of two: where its SMs would
+// otherwise go through 18 blocks of 128 x 128 tiles or more, one after the other.  The two launches more cost 5 us.
+// Measured, own sums against looking first (us): 6 blocks (1000 x 2304 x 768) 7.2 and 10.7, 8 (1024^3) 7.0 and 9.6, 16 (300 x 700 x
+// 2048) 14.3 and 15.2, 18 (1000 x 768 x 2304) 12.5 and 12.5, 23 (1531 x 1100 x 2927) 25.3 and 20.1, 32 (2048^3) 20.3 and 17.8,
+// 64 (256 x 14336 x 4096) 36 and 27, 112 (512 x 4096 x 14336) 54 and 41.
+bool takes_exponents(long long m, long long n, long long k) {
+  const long long tiles = ((m + 127) / 128) * ((n + 127) / 128);
+  return m > 64 && (tiles + sm_count() - 1) / sm_count() * ((k + 127) / 128) >= 18;
+}
 
 // Scratch of a product whose scales are looked at: a word a CTA, and both operands' exponents.
 struct ExponentRoom {
   size_t a_at, b_at, bytes;
   ExponentRoom(long long m, long long n, long long k) {
     const long long blocks = (k + 127) / 128;
-    a_at = 4 * kExponentCtas;
+    a_at = (4 * kExponentCtas + 511) / 512 * 512;
     b_at = a_at + 512 * size_t(blocks * ((m + 127) / 128));
     bytes = b_at + 512 * size_t(blocks * ((n + 127) / 128));
   }
@@ -277,9 +292,9 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
       const long long blocks = (k + 127) / 128;
       ExponentJob ja{p.a, reinterpret_cast<uint32_t*>(base + room.a_at), int(m), int((m + 127) / 128), 0};
       ExponentJob jb{p.b, reinterpret_cast<uint32_t*>(base + room.b_at), int(n), int((n + 127) / 128), 0};
-      ja.words = blocks * ja.atoms * 128;
-      jb.words = blocks * jb.atoms * 128;
-      const long long ctas = (ja.words + jb.words + kExponentThreads - 1) / kExponentThreads;
+      ja.all = blocks * ja.atoms;
+      jb.all = blocks * jb.atoms;
+      const long long ctas = (32 * (ja.all + jb.all) + kExponentThreads - 1) / kExponentThreads;
       p.odd_scales = static_cast<const int*>(workspace);
       p.odd_parts = int(ctas < kExponentCtas ? ctas : kExponentCtas);
       launch_dependent(exponents_kernel, unsigned(p.odd_parts), kExponentThreads, stream, ja, jb, static_cast<int*>(workspace));

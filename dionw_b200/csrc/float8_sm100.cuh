@@ -418,7 +418,7 @@ struct Shape {
   static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + kSumWarps * Queue::kBytes + 256 + 1024;
 };
 
-// Whether some scale is no power of two, as the kernel before found out.  Called by all threads of a CTA of 384 or more.
+// Whether some scale is no power of two, as the kernel before found out.  Called by all threads of a CTA, which are as many as parts at least.
 __device__ __forceinline__ bool any_odd_scale(const Params& p) {
   const bool mine = int(threadIdx.x) < p.odd_parts && __ldcg(p.odd_scales + threadIdx.x) != 0;
   return __syncthreads_or(mine) != 0;
@@ -444,7 +444,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int total_tiles = p.tiles_m * p.tiles_n;
+  int total_tiles = p.tiles_m * p.tiles_n;
   const int k_blocks = (p.k + kBK - 1) / kBK;
 
   if (threadIdx.x == 0) {
@@ -471,6 +471,8 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();
   griddep_launch();
+  // Scales that are all powers of two have been left to the tensor cores: nothing is left to do.
+  if (p.odd_scales != nullptr && !any_odd_scale(p)) total_tiles = 0;
 
   auto warp_wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p.status, p.wait_ns)) != 0;

@@ -188,8 +188,8 @@ def test_float8_product_scratch() -> None:
     assert lib.dionw_float8_product_workspace_bytes(64, 4096, 4096) == 0
     assert lib.dionw_float8_product_workspace_bytes(0, 1 << 20, 8) == 0
     assert lib.dionw_float8_product_workspace_bytes(1 << 14, 1 << 14, 0) == 0
-    # 128 words, and 512 bytes for each 128 rows and block of both operands
-    assert lib.dionw_float8_product_workspace_bytes(8192, 14336, 4096) == 512 + 512 * 32 * (64 + 112)
+    # 296 words, and 512 bytes for each 128 rows and block of both operands
+    assert lib.dionw_float8_product_workspace_bytes(8192, 14336, 4096) == 1536 + 512 * 32 * (64 + 112)
     status = lib.dionw_float8_product(1 << 20, 4096, 1 << 20, 1, 8192, 0, 1 << 20, 4096, 1 << 20, 1, 14336, 0, None, 0, 1 << 20,
                                       14336, 0, 0, 8192, 14336, 4096, None, None, 1 << 20, 100, None)
     assert status == -3 and "workspace" in _native.last_error()

@@ -152,7 +152,7 @@ def test_product_of_many_tiles(m, n, k, b_tiles) -> None:
     _close(dionw.float8_product(a, b, out=held.to(DEV), accumulate=True), a64, b64, held.double())
 
 
-@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 300)])
+@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 1153), (300, 260, 2400)])
 @pytest.mark.parametrize("b_tiles", [False, True])
 @pytest.mark.parametrize("layout", ["rows", "blocks"])
 def test_product_of_many_tiles_and_powers_of_two(m, n, k, b_tiles, layout) -> None:
