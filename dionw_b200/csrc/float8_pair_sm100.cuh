@@ -169,7 +169,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     int tm, tn;
     if (first_tile < total_tiles) {
       tile_at(first_tile, p, tm, tn);
-      queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks, lane);
+      queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, 0, k_blocks, lane);
     }
     for (int t = first_tile; t < total_tiles; t += pairs) {
       uint64_t sum[kColumns / 2];
@@ -191,7 +191,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const int row0 = tm * kPairM + row_in_tile, col0 = tn * kPairN + col_in_tile;
       if (t + pairs < total_tiles) {   // the next tile's first scales come while this one's sums go out
         tile_at(t + pairs, p, tm, tn);
-        queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, k_blocks, lane);
+        queue.start(p, tm * kPairM + row_in_tile, tn * kPairN + col_in_tile, 0, k_blocks, lane);
       }
       write_sums<T, kColumns>(p, stage_out, row0, col0, lane, [&](int c) {
         const float2 f = apart(sum[c / 2]);

@@ -4,6 +4,7 @@
 #include "float8_pair_sm100.cuh"
 #include "float8_scaled_sm100.cuh"
 #include "float8_sm100.cuh"
+#include "float8_tokens_sm100.cuh"
 #include "products.cuh"
 
 namespace dionw {
@@ -22,65 +23,83 @@ int allow_shared(Kernel kernel, size_t smem, std::atomic<bool> (&configured)[kMa
   return DIONW_OK;
 }
 
-template <typename T, int kTileN, bool kSwap, bool kRowScales>
-int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
-  using S = float8::Shape<kTileN, kRowScales>;
-  static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = float8::product_kernel<T, kTileN, kSwap, kRowScales>;
-  static std::atomic<bool> configured[kMaxDevices];
-  int st = allow_shared(kernel, S::kSmemBytes, configured);
-  if (st != DIONW_OK) return st;
-  CUtensorMap map_a{}, map_b{};
-  if (p.k > 0) {
-    st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
-    if (st != DIONW_OK) return st;
-    st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, kTileN);
-    if (st != DIONW_OK) return st;
-  }
-  p.tiles_m = (p.m + float8::kBM - 1) / float8::kBM;
-  p.tiles_n = (p.n + kTileN - 1) / kTileN;
-  const long long total = (long long)p.tiles_m * p.tiles_n;
-  DIONW_REQUIRE(total <= 0x7FFFFFFFll, "float8_product: too many tiles");
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(total < sm_count() ? total : sm_count()));
-  config.blockDim = dim3(float8::kThreads);
-  config.dynamicSmemBytes = S::kSmemBytes;
-  config.stream = stream;
-  cudaLaunchAttribute attribute;
-  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attribute.val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = &attribute;
-  config.numAttrs = use_dependent_launch() ? 1 : 0;
-  count_launch();
-  return check_cuda(cudaLaunchKernelEx(&config, kernel, map_a, map_b, p), "product_kernel launch");
-}
-
-template <typename T, int kTileN, bool kSwap>
-int launch(const void* a, int64_t lda, const void* b, int64_t ldb, const float8::Params& p, cudaStream_t stream) {
-  return p.b.shift != 0 ? launch_single<T, kTileN, kSwap, false>(a, lda, b, ldb, p, stream)
-                        : launch_single<T, kTileN, kSwap, true>(a, lda, b, ldb, p, stream);
-}
-
-// As clusters of two CTAs, one to each SM pair that has a tile.
+// In clusters of `cluster` CTAs.
 template <typename Kernel, typename... Args>
-int launch_clusters_of_two(Kernel kernel, size_t smem, int threads, float8::Params& p, cudaStream_t stream, const Args&... maps) {
-  const long long total = (long long)p.tiles_m * p.tiles_n, pairs_max = sm_count() / 2;
+int launch_in_clusters(Kernel kernel, unsigned ctas, unsigned cluster, size_t smem, int threads, const float8::Params& p,
+                       cudaStream_t stream, const Args&... maps) {
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(unsigned(2 * (total < pairs_max ? total : pairs_max)));
+  config.gridDim = dim3(ctas);
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;
   cudaLaunchAttribute attributes[2];
-  attributes[0].id = cudaLaunchAttributeClusterDimension;
-  attributes[0].val.clusterDim.x = 2;
-  attributes[0].val.clusterDim.y = 1;
-  attributes[0].val.clusterDim.z = 1;
-  attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attributes[1].val.programmaticStreamSerializationAllowed = 1;
-  config.attrs = attributes;
-  config.numAttrs = use_dependent_launch() ? 2 : 1;
+  attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attributes[0].val.programmaticStreamSerializationAllowed = 1;
+  attributes[1].id = cudaLaunchAttributeClusterDimension;
+  attributes[1].val.clusterDim.x = cluster;
+  attributes[1].val.clusterDim.y = 1;
+  attributes[1].val.clusterDim.z = 1;
+  // the attributes that are wanted lie together
+  config.attrs = use_dependent_launch() ? attributes : attributes + 1;
+  config.numAttrs = (use_dependent_launch() ? 1 : 0) + (cluster > 1 ? 1 : 0);
   count_launch();
   return check_cuda(cudaLaunchKernelEx(&config, kernel, maps..., p), "product_kernel launch");
+}
+
+// Tensor maps of the codes, where there are any.
+int code_maps(CUtensorMap& map_a, CUtensorMap& map_b, const void* a, int64_t lda, uint32_t a_rows, const void* b, int64_t ldb,
+              uint32_t b_rows, const float8::Params& p) {
+  if (p.k == 0) return DIONW_OK;
+  const int st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, a_rows);
+  return st != DIONW_OK ? st : make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, b_rows);
+}
+
+// 128 x 128 tiles.
+template <typename T, bool kRowScales>
+int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  using S = float8::Shape<kRowScales>;
+  static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = float8::product_kernel<T, kRowScales>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int st = allow_shared(kernel, S::kSmemBytes, configured);
+  CUtensorMap map_a{}, map_b{};
+  if (st == DIONW_OK) st = code_maps(map_a, map_b, a, lda, float8::kBM, b, ldb, float8::kTileN, p);
+  if (st != DIONW_OK) return st;
+  p.tiles_m = (p.m + float8::kBM - 1) / float8::kBM;
+  p.tiles_n = (p.n + float8::kTileN - 1) / float8::kTileN;
+  const long long total = (long long)p.tiles_m * p.tiles_n;
+  DIONW_REQUIRE(total <= 0x7FFFFFFFll, "float8_product: too many tiles");
+  return launch_in_clusters(kernel, unsigned(total < sm_count() ? total : sm_count()), 1, S::kSmemBytes, float8::kThreads, p,
+                            stream, map_a, map_b);
+}
+
+// Up to kTokens rows of B, tiles of 128 rows of A.
+template <typename T, int kTokens, bool kRowScales>
+int launch_tokens(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+  using S = float8::tokens::Shape<kTokens, kRowScales>;
+  static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
+  auto kernel = float8::tokens::product_kernel<T, kTokens, kRowScales>;
+  static std::atomic<bool> configured[kMaxDevices];
+  int st = allow_shared(kernel, S::kSmemBytes, configured);
+  CUtensorMap map_a{}, map_b{};
+  if (st == DIONW_OK) st = code_maps(map_a, map_b, a, lda, float8::kBM, b, ldb, kTokens, p);
+  if (st != DIONW_OK) return st;
+  p.tiles_m = (p.m + float8::kBM - 1) / float8::kBM;
+  p.tiles_n = 1;
+  // A tile's blocks are shared out while that keeps more SMs busy, and each part has two stages at least.
+  const int blocks = (p.k + 127) / 128;
+  unsigned parts = 1;
+  while (parts < 8 && 2 * parts * p.tiles_m <= sm_count() && blocks >= int(4 * parts * float8::tokens::kGroup)) parts *= 2;
+  const unsigned ctas = parts > 1 || p.tiles_m < sm_count() ? parts * p.tiles_m : sm_count();
+  return launch_in_clusters(kernel, ctas, parts, S::kSmemBytes, float8::kThreads, p, stream, map_a, map_b);
+}
+
+// As clusters of two CTAs, one to each SM pair that has a tile.
+template <typename Kernel, typename... Args>
+int launch_clusters_of_two(Kernel kernel, size_t smem, int threads, const float8::Params& p, cudaStream_t stream,
+                           const Args&... maps) {
+  const long long total = (long long)p.tiles_m * p.tiles_n, pairs_max = sm_count() / 2;
+  return launch_in_clusters(kernel, unsigned(2 * (total < pairs_max ? total : pairs_max)), 2, smem, threads, p, stream, maps...);
 }
 
 int count_pair_tiles(float8::Params& p, int tile_n) {
@@ -100,12 +119,8 @@ int launch_pairs(const void* a, int64_t lda, const void* b, int64_t ldb, float8:
   int st = allow_shared(kernel, pair::kSmemBytes<kRowScales>, configured);
   if (st != DIONW_OK) return st;
   CUtensorMap map_a{}, map_b{};
-  if (p.k > 0) {
-    st = make_byte_map(&map_a, a, p.k, p.m, lda, float8::kBK, float8::kBM);
-    if (st != DIONW_OK) return st;
-    st = make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, pair::kPairN / 2);
-    if (st != DIONW_OK) return st;
-  }
+  st = code_maps(map_a, map_b, a, lda, float8::kBM, b, ldb, pair::kPairN / 2, p);
+  if (st != DIONW_OK) return st;
   st = count_pair_tiles(p, pair::kPairN);
   if (st != DIONW_OK) return st;
   return launch_clusters_of_two(kernel, pair::kSmemBytes<kRowScales>, pair::kThreads, p, stream, map_a, map_b);
@@ -216,13 +231,17 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p
     // A few tokens: the weights are the 128 rows of a tile.
     std::swap(p.a, p.b);
     std::swap(p.m, p.n);
-    if (m <= 16) return launch<T, 16, true>(b, ldb, a, lda, p, stream);
-    if (m <= 32) return launch<T, 32, true>(b, ldb, a, lda, p, stream);
-    return launch<T, 64, true>(b, ldb, a, lda, p, stream);
+    auto launch = [&](auto row_scales) {
+      constexpr bool kRowScales = decltype(row_scales)::value;
+      if (m <= 16) return launch_tokens<T, 16, kRowScales>(b, ldb, a, lda, p, stream);
+      if (m <= 32) return launch_tokens<T, 32, kRowScales>(b, ldb, a, lda, p, stream);
+      return launch_tokens<T, 64, kRowScales>(b, ldb, a, lda, p, stream);
+    };
+    return p.b.shift == 0 ? launch(std::true_type()) : launch(std::false_type());
   }
   if (pair_tiles(p.m, p.n) >= sm_count() / 2)
     return p.b.shift != 0 ? launch_pairs<T, false>(a, lda, b, ldb, p, stream) : launch_pairs<T, true>(a, lda, b, ldb, p, stream);
-  return launch<T, 128, false>(a, lda, b, ldb, p, stream);
+  return p.b.shift != 0 ? launch_single<T, false>(a, lda, b, ldb, p, stream) : launch_single<T, true>(a, lda, b, ldb, p, stream);
 }
 
 }  // namespace

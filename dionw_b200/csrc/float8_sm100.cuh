@@ -7,8 +7,7 @@
 // blocks in the other accumulators.  The codes come by TMA; each summing warp fetches the scales it needs itself, a few blocks
 // ahead, by 4-byte asynchronous copies (any strides) into a queue of its own.
 //
-// A is [m, k], B is [n, k], both with rows of k codes: 128 of A times kTileN of B make a tile.  With kSwap A holds the
-// weights and B a few tokens, and `out` is the transposed tile.
+// A is [m, k], B is [n, k], both with rows of k codes: 128 of each make a tile.  (Few rows on the left: float8_tokens_sm100.cuh.)
 //
 // Every spin-wait is bounded, as in gemm_sm100.cuh.
 #pragma once
@@ -25,6 +24,7 @@ constexpr int kBK = 128;                 // codes, and bytes, of a block
 constexpr int kThreads = 320;            // warp 0: TMA, warp 1: MMA + TMEM owner, warps 2-9: sums and output
 constexpr int kSumWarps = 8;
 constexpr uint32_t kABytes = kBM * kBK;  // 16 KB
+constexpr int kTileN = 128;
 constexpr int kAccumulators = 4;
 
 // Scale of row i of an operand in block b: base[(i >> shift) * row_stride + b * block_stride].
@@ -307,14 +307,14 @@ struct ScaleQueue {
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
 
-  // The first blocks of a tile whose rows and columns start at row0 and col0 for this warp.
-  __device__ __forceinline__ void start(const Params& p, int row0, int col0, int blocks, int lane) {
+  // The first of `blocks` blocks, from first_block on, of a tile whose rows and columns start at row0 and col0 for this warp.
+  __device__ __forceinline__ void start(const Params& p, int row0, int col0, int first_block, int blocks, int lane) {
     const int row = row0 + lane;
     row_there = row < p.m;
-    row_at = p.a.base + (row_there ? int64_t(row >> p.a.shift) * p.a.row_stride : 0);
+    row_at = p.a.base + (row_there ? int64_t(row >> p.a.shift) * p.a.row_stride + first_block * p.a.block_stride : 0);
     columns_there = p.n - col0;
     const int column = kColumnScales == 0 ? col0 : col0 + lane;
-    column_at = p.b.base + (columns_there > 0 ? int64_t(column >> p.b.shift) * p.b.row_stride : 0);
+    column_at = p.b.base + (columns_there > 0 ? int64_t(column >> p.b.shift) * p.b.row_stride + first_block * p.b.block_stride : 0);
     __syncwarp();              // nobody reads the last tile's any more
 #pragma unroll
     for (int i = 0; i < kDepth - 1; ++i) fetch(p, i, i < blocks, lane);
@@ -407,14 +407,14 @@ __device__ __forceinline__ void tile_at(int t, const Params& p, int& tm, int& tn
   tn = r / rows_here;
 }
 
-template <int kTileN, bool kRowScales>
+template <bool kRowScales>
 struct Shape {
   static constexpr int kColumns = kTileN / 2;                      // of a summing warp: half of the tile's
   static constexpr uint32_t kStageBytes = kABytes + kTileN * kBK;
-  static constexpr int kStages = kTileN == 128 ? 5 : 8;
-  static constexpr uint32_t kTmemCols = kAccumulators * kTileN < 32 ? 32 : kAccumulators * kTileN;
-  static constexpr uint32_t kStagingBytes = kTileN == 128 ? kSumWarps * 32 * 128 : 0;   // 128 bytes of 32 rows a warp
-  using Queue = ScaleQueue<kRowScales ? kColumns : 0, kRowScales && kTileN == 128 ? 4 : 8>;
+  static constexpr int kStages = 5;
+  static constexpr uint32_t kTmemCols = kAccumulators * kTileN;
+  static constexpr uint32_t kStagingBytes = kSumWarps * 32 * 128;  // 128 bytes of 32 rows a warp
+  using Queue = ScaleQueue<kRowScales ? kColumns : 0, kRowScales ? 4 : 8>;
   static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kStagingBytes + kSumWarps * Queue::kBytes + 256 + 1024;
 };
 
@@ -425,11 +425,11 @@ __device__ __forceinline__ bool any_odd_scale(const Params& p) {
 }
 
 // kRowScales: each row of B has scales of its own; otherwise 128 share one.
-template <typename T, int kTileN, bool kSwap, bool kRowScales>
+template <typename T, bool kRowScales>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   using namespace gemm;
-  using S = Shape<kTileN, kRowScales>;
+  using S = Shape<kRowScales>;
   constexpr int kStages = S::kStages;
   constexpr int kAcc = kAccumulators;
   extern __shared__ uint8_t smem_raw[];
@@ -534,7 +534,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     int tm, tn;
     if (blockIdx.x < total_tiles) {
       tile_at(blockIdx.x, p, tm, tn);
-      queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks, lane);
+      queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, 0, k_blocks, lane);
     }
     for (int t = blockIdx.x; t < total_tiles; t += gridDim.x) {
       uint64_t sum[kColumns / 2];
@@ -544,7 +544,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         const uint32_t acc = it % kAcc;
         if (!warp_wait(&acc_full[acc], (it / kAcc) & 1u)) { ok = false; break; }
         tc_fence_after();
-        add_block<kColumns, kColumns >= 32 ? 16 : kColumns >= 16 ? kColumns / 2 : kColumns, kRowScales>(
+        add_block<kColumns, 16, kRowScales>(
             tmem_base + acc * kTileN + uint32_t(first_column) + (uint32_t(sub * 32) << 16), lane, sum,
             [&] { return queue.take(p, k_blocks - 1 - kb, lane); },
             [&] {
@@ -557,28 +557,12 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
       const int row0 = tm * kBM + sub * 32, col0 = tn * kTileN + first_column;
       if (t + int(gridDim.x) < total_tiles) {   // the next tile's first scales come while this one's sums go out
         tile_at(t + int(gridDim.x), p, tm, tn);
-        queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, k_blocks, lane);
+        queue.start(p, tm * kBM + sub * 32, tn * kTileN + first_column, 0, k_blocks, lane);
       }
-      auto value = [&](int c) {
+      write_sums<T, kColumns>(p, stage_out, row0, col0, lane, [&](int c) {
         const float2 f = apart(sum[c / 2]);
         return (c & 1) != 0 ? f.y : f.x;
-      };
-      if constexpr (kSwap) {
-        // rows of A are columns of the output: 32 lanes write neighbours
-        const int column = row0 + lane;
-        const float bias = p.bias != nullptr && column < p.m ? bias_at(p, column) : 0.0f;
-#pragma unroll
-        for (int c = 0; c < kColumns; ++c) {
-          const int row = col0 + c;
-          if (row >= p.n || column >= p.m) continue;
-          T* at = static_cast<T*>(p.out) + int64_t(row) * p.ldo + column;
-          float f = value(c) + bias;
-          if (p.accumulate) f += to_float<T>(*at);
-          *at = from_float<T>(f);
-        }
-      } else {
-        write_sums<T, kColumns>(p, stage_out, row0, col0, lane, value);
-      }
+      });
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }

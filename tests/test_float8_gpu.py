@@ -131,7 +131,7 @@ def _close(got: Tensor, a: Tensor, b: Tensor, extra: Tensor | float = 0.0) -> No
 
 
 @pytest.mark.parametrize("m,n,k", [
-    (1, 1, 1), (1, 128, 128), (1, 300, 517), (7, 129, 1000), (16, 256, 384), (17, 1000, 129), (33, 64, 4000),
+    (1, 1, 1), (1, 128, 128), (1, 300, 517), (7, 129, 1000), (16, 256, 384), (17, 1000, 129), (33, 64, 4000), (1, 20000, 300), (5, 130, 14336), (20, 400, 8200), (64, 129, 5000), (2, 1000, 4097),
     (64, 500, 640), (65, 127, 255), (128, 128, 128), (129, 257, 1153), (300, 700, 2048), (256, 256, 8192), (1000, 48, 96)])
 @pytest.mark.parametrize("b_tiles", [False, True])
 def test_product(m, n, k, b_tiles) -> None:
