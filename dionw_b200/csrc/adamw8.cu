@@ -106,9 +106,13 @@ __device__ __forceinline__ void decode_square(uint32_t codes, float (&out)[4]) {
   out[0] = a.x; out[1] = a.y; out[2] = b.x; out[3] = b.y;
 }
 
+// Four neighbours, in one access where all of a tensor's may be.
 template <typename G>
-__device__ __forceinline__ void load_gradient(const G* g, float (&out)[4]) {
-  if constexpr (std::is_same<G, float>::value) {
+__device__ __forceinline__ void load_four(const G* g, bool whole, float (&out)[4]) {
+  if (!whole) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] = to_float<G>(g[i]);
+  } else if constexpr (std::is_same<G, float>::value) {
     Span<4>::load(g, out);
   } else {
     const uint2 raw = __ldcs(reinterpret_cast<const uint2*>(g));
@@ -238,18 +242,19 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   f.beta2 = hyper.beta2;
   f.omb2 = hyper.one_minus_beta2;
   const uint32_t key = step_key(step, hyper.seed);
-  const bool vec = ((reinterpret_cast<uintptr_t>(p) | (reinterpret_cast<uintptr_t>(g) * (4 / sizeof(G)))) & 15u) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3u) == 0;
+  const bool p_whole = (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+  const bool g_whole = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0;
+  const bool codes_whole = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3u) == 0;
   Piece x[kUnroll];
   // lane 2j, 2j + 1: the scales of block first + j
   float* const scale_at = ((lane & 1) != 0 ? v_scale : m_scale) + first + (lane >> 1);
   const bool has_scale = lane < 2 * kUnroll && (first + (lane >> 1)) * kBlock < n;
-  if (vec && (first + kUnroll) * kBlock <= n) {
+  if (codes_whole && (first + kUnroll) * kBlock <= n) {
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const long long e = (first + j) * kBlock + 4 * lane;
-      Span<4>::load(p + e, x[j].p);
-      load_gradient<G>(g + e, x[j].g);
+      load_four<float>(p + e, p_whole, x[j].p);
+      load_four<G>(g + e, g_whole, x[j].g);
       x[j].m = __ldcs(reinterpret_cast<const unsigned int*>(m + e));
       x[j].v = __ldcs(reinterpret_cast<const unsigned int*>(v + e));
       x[j].m_scale = m_scale[first + j];
@@ -264,14 +269,19 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const long long e = (first + j) * kBlock + 4 * lane;
-      Span<4>::store(p + e, x[j].p);
+      if (p_whole) {
+        Span<4>::store(p + e, x[j].p);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[e + i] = x[j].p[i];
+      }
       __stcs(reinterpret_cast<unsigned int*>(m + e), x[j].m);
       __stcs(reinterpret_cast<unsigned int*>(v + e), x[j].v);
     }
     if (has_scale) *scale_at = scale;
     return;
   }
-  // Tensors between 16-byte boundaries, and the last blocks: element by element.  Lane l holds elements l, l + 32, l + 64 and
+  // The last blocks, and codes between 4-byte boundaries: element by element.  Lane l holds elements l, l + 32, l + 64 and
   // l + 96 of a block, so that neighbours read neighbours; what lies behind the tensor is zero.
 #pragma unroll
   for (int j = 0; j < kUnroll; ++j) {
