@@ -22,9 +22,11 @@ namespace {
 
 constexpr int kBlock = 128;          // elements of a scale: four for each lane of a warp
 constexpr int kTable = 96;
-constexpr int kThreads = 256;
 constexpr int kUnroll = 2;           // blocks of a warp
-constexpr int kChunk = kThreads / 32 * kUnroll * kBlock;   // elements per CTA
+// Threads of a CTA.  Many small ones where SMs are full of them; large ones, that take a whole tensor each and count its step
+// themselves, where no tensor is larger than that: a launch less for the vectors of a model, which are a group of their own.
+constexpr int kThreads = 128, kVectorThreads = 512;
+constexpr int elements_of(int threads) { return threads / 32 * kUnroll * kBlock; }
 constexpr float kMeanMax = 448.0f, kSquareMax = 57344.0f;
 constexpr float kSmallestScale = 1.17549435e-38f;          // 2^-126: its reciprocal is finite
 
@@ -208,8 +210,13 @@ __device__ __forceinline__ float update(Piece (&x)[kUnroll], const Factors& f, i
   return scale;
 }
 
-template <typename G>
-__global__ void __launch_bounds__(kThreads, 4)
+// 1 - e^x for x < 0: without the cancellation near zero, and in a few instructions away from it, where the exponential's 2^-21
+// at most is one of a third and less.
+__device__ __forceinline__ float correction(float x) { return x < -1.0f ? 1.0f - __expf(x) : -expm1f(x); }
+
+// kWhole: a CTA takes all of a tensor, and its step has not been counted yet.
+template <typename G, int kCtaThreads, bool kWhole>
+__global__ void __launch_bounds__(kCtaThreads, 1024 / kCtaThreads)
 adamw8_kernel(const Table tab, const Hyper hyper) {
   after_previous();
   const float lr = hyper.device != nullptr ? hyper.device[0] : hyper.lr;
@@ -221,8 +228,13 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   }
   const unsigned first_cta = lo == 0 ? 0u : tab.block_end[lo - 1];
   const int lane = threadIdx.x & 31;
-  const long long first = ((long long)(blockIdx.x - first_cta) * (kThreads / 32) + (threadIdx.x >> 5)) * kUnroll;
+  const long long first = ((long long)(blockIdx.x - first_cta) * (kCtaThreads / 32) + (threadIdx.x >> 5)) * kUnroll;
   const long long n = tab.numel[lo];
+  const float step = kWhole ? *tab.step[lo] + 1.0f : *tab.step[lo];
+  if constexpr (kWhole) {
+    __syncthreads();   // everyone has read it
+    if (threadIdx.x == 0) *tab.step[lo] = step;
+  }
   if (first * kBlock >= n) return;
   float* p = tab.p[lo];
   const G* g = static_cast<const G*>(tab.g[lo]);
@@ -230,12 +242,10 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   uint8_t* v = tab.v[lo];
   float* m_scale = tab.m_scale[lo];
   float* v_scale = tab.v_scale[lo];
-  const float step = *tab.step[lo];
-  // 1 - beta^t without the cancellation of its first steps
   Factors f;
   f.decay = lr * weight_decay;
-  f.rate = lr / -expm1f(step * hyper.log_beta1);
-  f.inv_root2 = rsqrtf(-expm1f(step * hyper.log_beta2));
+  f.rate = __fdividef(lr, correction(step * hyper.log_beta1));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(f.inv_root2) : "f"(correction(step * hyper.log_beta2)));
   f.eps = hyper.eps;
   f.beta1 = hyper.beta1;
   f.omb1 = hyper.one_minus_beta1;
@@ -321,11 +331,15 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
 }
 
 template <typename G>
-int launch(const Table& tab, unsigned ctas, const Hyper& hyper, cudaStream_t stream) {
+int launch(const Table& tab, unsigned ctas, bool whole, const Hyper& hyper, cudaStream_t stream) {
+  if (whole) {
+    launch_dependent(adamw8_kernel<G, kVectorThreads, true>, ctas, kVectorThreads, stream, tab, hyper);
+    return launch_status("adamw8_kernel");
+  }
   launch_dependent(adamw8_bump_steps_kernel, 1, kTable, stream, tab);
   const int st = launch_status("adamw8_bump_steps_kernel");
-  if (st != DIONW_OK) return st;
-  launch_dependent(adamw8_kernel<G>, ctas, kThreads, stream, tab, hyper);
+  if (st != DIONW_OK || ctas == 0) return st;   // empty tensors still count the step
+  launch_dependent(adamw8_kernel<G, kThreads, false>, ctas, kThreads, stream, tab, hyper);
   return launch_status("adamw8_kernel");
 }
 
@@ -358,13 +372,11 @@ extern "C" int dionw_adamw8_multi(void* const* params, const void* const* grads,
   for (int start = 0; start < n_tensors;) {
     Table tab;
     int count = 0;
-    unsigned long long ctas = 0;
+    bool whole = true;
     for (; start + count < n_tensors && count < kTable; ++count) {
       const int i = start + count;
       DIONW_REQUIRE(numels[i] >= 0, "adamw8_multi: tensor %d has %lld elements", i, (long long)numels[i]);
-      const unsigned long long need = (unsigned long long)((numels[i] + kChunk - 1) / kChunk);
-      if (ctas + need > 0x7FFFFFFFull) break;
-      ctas += need;
+      whole = whole && numels[i] <= elements_of(kVectorThreads);
       tab.p[count] = static_cast<float*>(params[i]);
       tab.g[count] = grads[i];
       tab.m[count] = static_cast<uint8_t*>(exp_avg[i]);
@@ -373,23 +385,26 @@ extern "C" int dionw_adamw8_multi(void* const* params, const void* const* grads,
       tab.v_scale[count] = static_cast<float*>(exp_avg_sq_scale[i]);
       tab.step[count] = static_cast<float*>(steps[i]);
       tab.numel[count] = numels[i];
-      tab.block_end[count] = unsigned(ctas);
     }
-    if (count == 0) {
-      set_error("adamw8_multi: a tensor of %lld elements is too large for one launch", (long long)numels[start]);
-      return DIONW_ERR_UNSUPPORTED;
+    unsigned long long ctas = 0;
+    for (int i = 0; i < count; ++i) {
+      const unsigned long long need = whole ? 1 : (unsigned long long)((tab.numel[i] + elements_of(kThreads) - 1) / elements_of(kThreads));
+      if (ctas + need > 0x7FFFFFFFull) {
+        if (i == 0) {
+          set_error("adamw8_multi: a tensor of %lld elements is too large for one launch", (long long)tab.numel[i]);
+          return DIONW_ERR_UNSUPPORTED;
+        }
+        count = i;
+        break;
+      }
+      ctas += need;
+      tab.block_end[i] = unsigned(ctas);
     }
     tab.n = count;
     start += count;
-    if (ctas == 0) {   // empty tensors still count the step
-      launch_dependent(adamw8_bump_steps_kernel, 1, kTable, stream, tab);
-      const int st = launch_status("adamw8_bump_steps_kernel");
-      if (st != DIONW_OK) return st;
-      continue;
-    }
-    const int st = grad_dtype == DIONW_F32   ? launch<float>(tab, unsigned(ctas), hyper, stream)
-                   : grad_dtype == DIONW_F16 ? launch<__half>(tab, unsigned(ctas), hyper, stream)
-                                             : launch<__nv_bfloat16>(tab, unsigned(ctas), hyper, stream);
+    const int st = grad_dtype == DIONW_F32   ? launch<float>(tab, unsigned(ctas), whole, hyper, stream)
+                   : grad_dtype == DIONW_F16 ? launch<__half>(tab, unsigned(ctas), whole, hyper, stream)
+                                             : launch<__nv_bfloat16>(tab, unsigned(ctas), whole, hyper, stream);
     if (st != DIONW_OK) return st;
   }
   return DIONW_OK;
