@@ -81,11 +81,18 @@ class Float8Matrix:
         return self.values.float() * scales.repeat_interleave(BLOCK, 1)[:, :cols]
 
 
-def _made(values: Tensor, scales: Tensor) -> Float8Matrix:
-    """A ``Float8Matrix`` of what was just allocated to be one."""
-    matrix = object.__new__(Float8Matrix)
-    matrix.__dict__.update(values=values, scales=scales)
-    return matrix
+def _room(rows: int, cols: int, tiles: bool, device: torch.device) -> tuple[Float8Matrix, tuple[int, int, int, int]]:
+    """A matrix to quantize into, and how the quantizer is told of it: codes, their leading dimension, scales, theirs."""
+    ld, blocks = (cols + 15) // 16 * 16, (cols + BLOCK - 1) // BLOCK
+    values = torch.empty(rows, ld, dtype=CODES, device=device)
+    if tiles:
+        scales, lds = torch.empty(_blocks(rows), blocks, dtype=torch.float32, device=device), blocks
+    else:   # of single rows: those of a block together, as the product and the quantizer go through them
+        scales, lds = torch.empty_strided((rows, blocks), (1, rows), dtype=torch.float32, device=device), rows
+    target = values.data_ptr(), ld, scales.data_ptr(), lds
+    matrix = object.__new__(Float8Matrix)   # nothing to check
+    matrix.__dict__.update(values=values if ld == cols else values[:, :cols], scales=scales)
+    return matrix, target
 
 
 def _require_source(x: Tensor) -> None:
@@ -108,30 +115,18 @@ def _with_rows(x: Tensor) -> tuple[Tensor, int]:
     return x, ld if rows > 1 else cols
 
 
+_NOWHERE = (None, 0, None, 0)
+
+
 def _quantize(x: Tensor, tiles: bool, transposed: bool) -> Any:
     _require_source(x)
     x, ldx = _with_rows(x)
-    rows, cols = x.shape
-    device = x.device
-    made: list[tuple[Tensor, Tensor]] = []
-    found: list[Float8Matrix] = []
-    for high, wide in ((rows, cols), (cols, rows)) if transposed else ((rows, cols),):
-        ld = _padded(wide)
-        codes = torch.empty(high, ld, dtype=CODES, device=device)
-        # scales of single rows: those of a block column together, as the product and the quantizer go through them
-        scales = torch.empty((_blocks(high), _blocks(wide)) if tiles else (_blocks(wide), high), dtype=torch.float32,
-                             device=device)
-        made.append((codes, scales))
-        found.append(_made(codes if ld == wide else codes[:, :wide], scales if tiles else scales.t()))
+    (rows, cols), device = x.shape, x.device
+    matrix, target = _room(rows, cols, tiles, device)
+    turned, target_t = _room(cols, rows, tiles, device) if transposed else (None, _NOWHERE)
     if rows and cols:
-        codes, scales = made[0]
-        first = codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1]
-        second: tuple[Any, ...] = (None, 0, None, 0)
-        if transposed:
-            codes, scales = made[1]
-            second = codes.data_ptr(), codes.shape[1], scales.data_ptr(), scales.shape[1]
-        _native.float8_quantize(x.get_device(), x.data_ptr(), x.dtype, rows, cols, ldx, tiles, *first, *second)
-    return tuple(found) if transposed else found[0]
+        _native.float8_quantize(x.get_device(), x.data_ptr(), x.dtype, rows, cols, ldx, tiles, *target, *target_t)
+    return (matrix, turned) if transposed else matrix
 
 
 def quantize_rows(x: Tensor, *, transposed: bool = False) -> Any:
