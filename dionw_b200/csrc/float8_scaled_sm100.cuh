@@ -1,12 +1,16 @@
 // The 8-bit product with powers of two for scales, on SM pairs: the tensor cores apply the scales themselves
-// (tcgen05.mma kind::mxf8f6f4, block_scale), so that a tile's sums stay in TMEM over the whole length and the warps that
-// write them out have nothing to do in the main loop.  For what the quantizer makes; scales of any value take
+// (tcgen05.mma kind::mxf8f6f4, block_scale), so that a tile's sums stay in TMEM and the warps that write them
+// out have next to nothing to do in the main loop.  For what the quantizer makes; scales of any value take
 // float8_pair_sm100.cuh, whose warps add 256 x 256 sums for each block of 128.
 //
 // Exponents travel as words of 32 bits with the scale's exponent in the low byte (UE8M0, the same bias as fp32's), 128 rows of a
 // block together, in the order that the tensor cores want them: word 4 l + c is row 32 c + l.  TMA brings 128 of A and 256 of B
 // into each CTA with the codes of a block, tcgen05.cp from there into TMEM, where each 32 lanes get a copy.  The hardware takes
 // one scale for 32 codes of a row; the four MMAs of a block use the same ones.
+//
+// The tensor cores cut off what an addition to their fp32 sums leaves behind the last place, so that sums of one sign fall behind
+// by up to 2^-24 each 32 products: 4e-6 of a sum of 8192, 1e-3 of one of half a million.  After kPiece blocks the sums are therefore
+// taken into registers, where the pieces are added to nearest: 1.5e-6 at most, at any length.
 //
 // A tile's 256 columns are half of TMEM and there is one of them: the eight warps take it into registers at once, and
 // convert and store while the next tile is computed.  Tiles of 256 x 128 are for products that have too few of the wide ones.
@@ -24,6 +28,7 @@ constexpr uint32_t kAtomBytes = 512;                       // the exponents of 1
 constexpr uint32_t kStagingBytes = kSumWarps * 32 * 128;
 constexpr uint32_t kScaleColumns = 16;                     // of TMEM, for a block's exponents: 4 of A, 4 for each 128 of B
 constexpr uint32_t kScaleBuffers = 8;
+constexpr int kPiece = 32;                                 // blocks of 128 that are summed in TMEM
 constexpr uint32_t kScalesAt = 256;                        // the columns behind the sums
 
 // kTileN: 256 or 128.
@@ -160,11 +165,16 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
       uint32_t loaded = 0, local = 0, buffer = 0;
       bool ok = true;
       const uint32_t ring = smem_u32(smem);
-      for (int t = first_tile; t < total_tiles && ok; t += pairs, ++local) {
-        const uint32_t acc = local % S::kSums;
-        if (!warp_wait(&acc_empty[acc], ((local / S::kSums) & 1u) ^ 1u)) break;
-        tc_fence_after();
+      for (int t = first_tile; t < total_tiles && ok; t += pairs) {
+        uint32_t acc = 0;
         for (int kb = 0; kb < k_blocks; ++kb) {
+          const bool first = kb % kPiece == 0, last = (kb + 1) % kPiece == 0 || kb + 1 == k_blocks;   // of a piece
+          if (first) {
+            acc = local % S::kSums;
+            if (!warp_wait(&acc_empty[acc], ((local / S::kSums) & 1u) ^ 1u)) { ok = false; break; }
+            tc_fence_after();
+            ++local;
+          }
           if (!warp_wait(&full_bar[s], loaded)) { ok = false; break; }
           tc_fence_after();
           const uint32_t a_addr = ring + uint32_t(s) * S::kStageBytes;
@@ -177,9 +187,9 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
             if (kTileN == 256) copy_scales(sb + 4, scales + (2 * kAtomBytes >> 4));
 #pragma unroll
             for (int j = 0; j < kBK / 32; ++j)
-              umma2_scaled(tmem_base + acc * kTileN, a_desc + 2 * j, b_desc + 2 * j, idesc, sa, sb, kb > 0 || j > 0 ? 1u : 0u);
+              umma2_scaled(tmem_base + acc * kTileN, a_desc + 2 * j, b_desc + 2 * j, idesc, sa, sb, !first || j > 0 ? 1u : 0u);
             gemm2::umma2_commit_both(&empty_bar[s]);
-            if (kb + 1 == k_blocks) gemm2::umma2_commit_both(&acc_full[acc]);
+            if (last) gemm2::umma2_commit_both(&acc_full[acc]);
           }
           __syncwarp();
           buffer = (buffer + 1) % kScaleBuffers;
@@ -195,17 +205,33 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
     const uint32_t tmem_mine = tmem_base + uint32_t(half * kColumns) + (uint32_t(sub * 32) << 16);
     const uint32_t leader_empty = peer_address(acc_empty, 0);
     uint32_t local = 0;
-    for (int t = first_tile; t < total_tiles; t += pairs, ++local) {
-      const uint32_t acc = local % S::kSums;
-      if (!warp_wait(&acc_full[acc], (local / S::kSums) & 1u)) break;
-      tc_fence_after();
+    bool ok = true;
+    for (int t = first_tile; t < total_tiles; t += pairs) {
       uint32_t sum[kColumns];
+      for (int kb = 0; kb < k_blocks; kb += kPiece, ++local) {
+        const uint32_t acc = local % S::kSums;
+        if (!warp_wait(&acc_full[acc], (local / S::kSums) & 1u)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t from = tmem_mine + acc * kTileN;
+        if (kb == 0) {
 #pragma unroll
-      for (int c = 0; c < kColumns; c += 32) tmem_load<32>(tmem_mine + acc * kTileN + c, sum + c);
-      tmem_wait<kColumns>(sum);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
+          for (int c = 0; c < kColumns; c += 32) tmem_load<32>(from + c, sum + c);
+          tmem_wait<kColumns>(sum);
+        } else {
+#pragma unroll
+          for (int c = 0; c < kColumns; c += 32) {
+            uint32_t v[32];
+            tmem_load<32>(from + c, v);
+            tmem_wait<32>(v);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) sum[c + i] = __float_as_uint(__uint_as_float(sum[c + i]) + __uint_as_float(v[i]));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
+      }
+      if (!ok) break;
       int tm, tn;
       tile_at(t, p, tm, tn);
       write_sums<T, kColumns>(p, stage_out, tm * kPairM + int(rank) * kBM + sub * 32, tn * kTileN + half * kColumns, lane,

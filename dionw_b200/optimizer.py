@@ -250,6 +250,12 @@ class _DionCore(Optimizer):
         """
         saved = _fill_legacy_keys(state_dict["param_groups"])
         _require_same_structure(saved, self.param_groups)
+        for group, current in zip(saved, self.param_groups):
+            if group.get(ADAMW_STATE_BITS_KEY, 32) == 8:
+                for index, param in zip(group["params"], current["params"]):
+                    entry = state_dict["state"].get(index)
+                    if entry:
+                        require_adamw8_state(param, entry)
         super().load_state_dict({**state_dict, "param_groups": saved})
         self._restore_adamw8_state()
         self._buckets = None
@@ -262,13 +268,10 @@ class _DionCore(Optimizer):
             if group.get(ADAMW_STATE_BITS_KEY, 32) != 8:
                 continue
             for param in group["params"]:
-                entry = self.state.get(param)
-                if not entry or EXP_AVG_STATE not in entry:
-                    continue
+                entry = self.state.get(param) or {}
                 for key, dtype in ((EXP_AVG_STATE, MEAN_DTYPE), (EXP_AVG_SQ_STATE, SQUARE_DTYPE)):
-                    if EXP_AVG_SCALE_STATE in entry:
+                    if key in entry:
                         entry[key] = entry[key].to(dtype).contiguous()
-                require_adamw8_state(param, entry)
 
     @torch.no_grad()
     def step(self, closure: Callable[[], float] | None = None) -> float | None:

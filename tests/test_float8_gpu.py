@@ -299,6 +299,19 @@ def test_linear_of_many_tiles(tokens, inputs, outputs, dtype) -> None:
         assert bool(((got.double() - want).abs() <= bound).all()), float(((got.double() - want).abs() / bound).max())
 
 
+@pytest.mark.parametrize("tokens,width", [(4096, 256), (4224, 256), (20000, 130), (9000, 2300)])
+def test_long_sums_of_one_sign(tokens, width) -> None:
+    """The weight's gradient over many tokens, all of it positive: what the tensor cores cut off in a piece of 32 blocks is
+    128 times 2^-24 at most, and the pieces are added with a rounding each."""
+    x, dy = _matrix(tokens, width, 1).abs().to(DEV), _matrix(tokens, width, 2).abs().to(DEV)
+    w = torch.zeros(width, width, device=DEV, requires_grad=True)
+    dw, = torch.autograd.grad(dionw.float8_linear(x, w), w, dy)
+    want = dionw.quantize_rows(dy, transposed=True)[1].dequantize().double() @ \
+        dionw.quantize_rows(x, transposed=True)[1].dequantize().double().T
+    pieces = -(-tokens // 4096)
+    assert float(((dw.double() - want).abs() / want).max()) <= (128 + 4 + pieces) * 2.0**-24
+
+
 def test_linear_of_many_tiles_keeps_infinities_in_their_rows() -> None:
     x = _matrix(2501, 1900, 1).to(DEV)
     w = (_matrix(2405, 1900, 3) * 0.1).to(DEV)
