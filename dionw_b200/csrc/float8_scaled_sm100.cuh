@@ -74,6 +74,29 @@ constexpr uint32_t make_idesc(int m, int n) {
   return (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 4) << 24);
 }
 
+// Adds the accumulator at `taddr` to this lane's sums (in pairs); `release` is called once it is in registers.
+template <int kColumns, typename Release>
+__device__ __forceinline__ void add_pieces(uint32_t taddr, uint64_t (&sum)[kColumns / 2], Release&& release) {
+  uint32_t v[2][16];
+  tmem_load<16>(taddr, v[0]);
+  tmem_load<16>(taddr + 16, v[1]);
+#pragma unroll
+  for (int c0 = 0; c0 < kColumns; c0 += 32) {
+    tmem_wait<16>(v[0]);
+    tmem_pass<16>(v[1]);
+    if (c0 + 32 == kColumns) release();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        uint64_t& s = sum[(c0 + 16 * h + i) / 2];
+        asm("add.rn.f32x2 %0, %0, %1;" : "+l"(s) : "l"(two(v[h][i], v[h][i + 1])));
+      }
+      if (c0 + 32 < kColumns) tmem_load<16>(taddr + c0 + 32 + 16 * h, v[h]);
+    }
+  }
+}
+
 template <typename T, int kTileN>
 __global__ void __launch_bounds__(kThreads, 1)
 product_kernel(const __grid_constant__ Maps maps, const Params p) {
@@ -207,35 +230,28 @@ product_kernel(const __grid_constant__ Maps maps, const Params p) {
     uint32_t local = 0;
     bool ok = true;
     for (int t = first_tile; t < total_tiles; t += pairs) {
-      uint32_t sum[kColumns];
+      uint64_t sum[kColumns / 2];
+#pragma unroll
+      for (int c = 0; c < kColumns / 2; ++c) sum[c] = 0;
       for (int kb = 0; kb < k_blocks; kb += kPiece, ++local) {
         const uint32_t acc = local % S::kSums;
         if (!warp_wait(&acc_full[acc], (local / S::kSums) & 1u)) { ok = false; break; }
         tc_fence_after();
         const uint32_t from = tmem_mine + acc * kTileN;
-        if (kb == 0) {
-#pragma unroll
-          for (int c = 0; c < kColumns; c += 32) tmem_load<32>(from + c, sum + c);
-          tmem_wait<kColumns>(sum);
-        } else {
-#pragma unroll
-          for (int c = 0; c < kColumns; c += 32) {
-            uint32_t v[32];
-            tmem_load<32>(from + c, v);
-            tmem_wait<32>(v);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) sum[c + i] = __float_as_uint(__uint_as_float(sum[c + i]) + __uint_as_float(v[i]));
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
+        add_pieces<kColumns>(from, sum, [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) gemm2::remote_arrive(leader_empty + acc * uint32_t(sizeof(uint64_t)));
+        });
       }
       if (!ok) break;
       int tm, tn;
       tile_at(t, p, tm, tn);
       write_sums<T, kColumns>(p, stage_out, tm * kPairM + int(rank) * kBM + sub * 32, tn * kTileN + half * kColumns, lane,
-                              [&](int c) { return __uint_as_float(sum[c]); });
+                              [&](int c) {
+                                const float2 f = apart(sum[c / 2]);
+                                return (c & 1) != 0 ? f.y : f.x;
+                              });
     }
   }
 
