@@ -68,16 +68,16 @@ __device__ __forceinline__ uint32_t mix(uint32_t h) {
   return h ^ (h >> 15);
 }
 
-// The 8-bit code of x >= 0, in the top byte and without its sign: rounded down after `noise` / 2^16 of a step is added.
+// The 8-bit code of x >= 0, in the top byte and without its sign: rounded down after the noise, in 2^-16 of a step, is added.
 // Codes of normal numbers are the top bits of the fp32 ones; a shift brings them into the byte, and the difference of the
 // exponents' biases is 0x40000000 there in both formats.  The largest value of a block may come out a little above the format's:
 // the noise leaves room for 15 units in the last place below the next code.
+// `noise` holds its 16 bits in the two middle bytes and 0x40 in the top one.
 template <int kMantissa, int kBias>
 __device__ __forceinline__ uint32_t encode_normal(float x, uint32_t noise) {
-  constexpr int kDrop = 23 - kMantissa;
-  static_assert(((uint64_t(127 - kBias) << 23) << (24 - kDrop)) % (1ull << 32) == 0xC0000000u, "difference of the biases");
-  const uint32_t bits = noise * (1u << (kDrop - 16)) + __float_as_uint(x);
-  return bits * (1u << (24 - kDrop)) + 0x40000000u;
+  constexpr int kUp = kMantissa + 1;   // what brings 8 bits, and the sign before them, to the top
+  static_assert(((uint64_t(127 - kBias) << 23) << kUp) % (1ull << 32) == 0xC0000000u, "difference of the biases");
+  return (__float_as_uint(x) << kUp) + noise;
 }
 // Of any x: below the smallest normal number codes are evenly spaced, and adding that number turns them into its
 // mantissa.
@@ -87,6 +87,9 @@ __device__ __forceinline__ uint32_t encode(float x, uint32_t noise) {
   const bool low = x < normal;
   return encode_normal<kMantissa, kBias>(low ? x + normal : x, noise) - (low ? 1u << (24 + kMantissa) : 0u);
 }
+// The low and the high 16 bits of a word as such noise.
+__device__ __forceinline__ uint32_t low_noise(uint32_t word) { return __byte_perm(word, 0x40u, 0x4105u); }
+__device__ __forceinline__ uint32_t high_noise(uint32_t word) { return __byte_perm(word, 0x40u, 0x4325u); }
 // The top bytes of four words.
 __device__ __forceinline__ uint32_t top_bytes(const uint32_t (&w)[4]) {
   return __byte_perm(__byte_perm(w[0], w[1], 0x0073), __byte_perm(w[2], w[3], 0x0073), 0x5410);
@@ -108,25 +111,33 @@ __device__ __forceinline__ void decode_square(uint32_t codes, float (&out)[4]) {
   out[0] = a.x; out[1] = a.y; out[2] = b.x; out[3] = b.y;
 }
 
-// Four neighbours, in one access where all of a tensor's may be.
+// Four gradients in the type they have: turned into floats only when all loads are under way.
 template <typename G>
-__device__ __forceinline__ void load_four(const G* g, bool whole, float (&out)[4]) {
-  if (!whole) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = to_float<G>(g[i]);
-  } else if constexpr (std::is_same<G, float>::value) {
-    Span<4>::load(g, out);
-  } else {
+struct Raw {
+  uint32_t w[2];
+  __device__ __forceinline__ void load(const G* g) {
     const uint2 raw = __ldcs(reinterpret_cast<const uint2*>(g));
-    const G* h = reinterpret_cast<const G*>(&raw);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] = to_float<G>(h[i]);
+    w[0] = raw.x; w[1] = raw.y;
   }
-}
+  __device__ __forceinline__ void set(int i, G v) { w[i >> 1] |= uint32_t(*reinterpret_cast<const uint16_t*>(&v)) << (16 * (i & 1)); }
+  __device__ __forceinline__ float value(int i) const {
+    const uint16_t h = uint16_t(w[i >> 1] >> (16 * (i & 1)));
+    return to_float<G>(*reinterpret_cast<const G*>(&h));
+  }
+};
+template <>
+struct Raw<float> {
+  float f[4];
+  __device__ __forceinline__ void load(const float* g) { Span<4>::load(g, f); }
+  __device__ __forceinline__ void set(int i, float v) { f[i] = v; }
+  __device__ __forceinline__ float value(int i) const { return f[i]; }
+};
 
 // One block of 128 elements: four for each lane.
+template <typename G>
 struct Piece {
-  float p[4], g[4];
+  Raw<float> p;
+  Raw<G> g;
   uint32_t m, v;
   float m_scale, v_scale;
 };
@@ -141,12 +152,13 @@ struct Factors {
 // Updates a warp's pieces.  words(j, w) gives the noise of piece j's four elements.  Lane 2j of the warp is left with the
 // scale of piece j's first moment, lane 2j + 1 with that of the second.
 //
-// What bounds it: at 16 bytes an element and 6.5 TB/s an SM has about 85 instructions a lane and element.  The first version took 100
-// (39.4 M elements 141 us): each lane worked out each scale and its reciprocal, and each code went through the form that
-// holds for the smallest numbers too.  Those are now left to the pieces that have any (1 of 100 where gradients are
-// normal), and the scales to a lane each.
-template <typename Words>
-__device__ __forceinline__ float update(Piece (&x)[kUnroll], const Factors& f, int lane, Words&& words) {
+// What bounds it: at 16 bytes an element and 6.5 TB/s an SM has about 85 instructions a lane and element, so that both the
+// memory and the issue slots are nearly full.  39.4 M elements with fp32 gradients take 105 us, 6.0 TB/s.  The first version took
+// 141 us: each lane worked out each scale and its reciprocal, and each code went through the form that holds for the smallest
+// numbers too.  Those are now left to the pieces that have any (1 of 100 where gradients are normal), and the scales to a
+// lane each.  Noise that a byte permutation puts where the code wants it, instead of a shift and a mask, was 3 us.
+template <typename G, typename Words>
+__device__ __forceinline__ float update(Piece<G> (&x)[kUnroll], const Factors& f, int lane, Words&& words) {
   float m[kUnroll][4], v[kUnroll][4];
   float largest = 0.0f;
 #pragma unroll
@@ -156,7 +168,7 @@ __device__ __forceinline__ float update(Piece (&x)[kUnroll], const Factors& f, i
     uint32_t m_top = 0, v_top = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float g = x[j].g[i];
+      const float g = x[j].g.value(i);
       // every operation rounded by itself: two evaluations of the moments in fp32 are the same bit for bit, and a
       // difference in the last bit, rounded to the next code, would be one of a tenth in the steps to come
       m[j][i] = __fadd_rn(__fmul_rn(f.beta1, __fmul_rn(m[j][i], x[j].m_scale)), __fmul_rn(f.omb1, g));
@@ -164,7 +176,7 @@ __device__ __forceinline__ float update(Piece (&x)[kUnroll], const Factors& f, i
       float root, inverse;
       asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v[j][i]));
       asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inverse) : "f"(fmaf(root, f.inv_root2, f.eps)));
-      x[j].p[i] = fmaf(-f.rate * m[j][i], inverse, fmaf(-f.decay, x[j].p[i], x[j].p[i]));
+      x[j].p.f[i] = fmaf(-f.rate * m[j][i], inverse, fmaf(-f.decay, x[j].p.f[i], x[j].p.f[i]));
       // as integers, magnitudes are in order, infinity and NaN above all numbers
       m_top = max(m_top, __float_as_uint(m[j][i]) & 0x7FFFFFFFu);
       v_top = max(v_top, __float_as_uint(v[j][i]));
@@ -191,14 +203,14 @@ __device__ __forceinline__ float update(Piece (&x)[kUnroll], const Factors& f, i
     if (!__any_sync(0xffffffffu, low)) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        mean[i] = encode_normal<3, 7>(a[i], w[i] & 0xFFFFu);
-        square[i] = encode_normal<2, 15>(b[i], w[i] >> 16);
+        mean[i] = encode_normal<3, 7>(a[i], low_noise(w[i]));
+        square[i] = encode_normal<2, 15>(b[i], high_noise(w[i]));
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        mean[i] = encode<3, 7>(a[i], w[i] & 0xFFFFu);
-        square[i] = encode<2, 15>(b[i], w[i] >> 16);
+        mean[i] = encode<3, 7>(a[i], low_noise(w[i]));
+        square[i] = encode<2, 15>(b[i], high_noise(w[i]));
         if (v[j][i] > 0.0f) square[i] = max(square[i], 1u << 24);
       }
     }
@@ -252,82 +264,95 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   f.beta2 = hyper.beta2;
   f.omb2 = hyper.one_minus_beta2;
   const uint32_t key = step_key(step, hyper.seed);
-  const bool p_whole = (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
-  const bool g_whole = (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0;
-  const bool codes_whole = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3u) == 0;
-  Piece x[kUnroll];
-  // lane 2j, 2j + 1: the scales of block first + j
+  const bool codes_fours = ((reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(v)) & 3u) == 0 && (first + kUnroll) * kBlock <= n;
+  const bool all_fours = codes_fours && (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (reinterpret_cast<uintptr_t>(g) & (4 * sizeof(G) - 1)) == 0;
+  Piece<G> x[kUnroll];
+  // Whole blocks go four neighbours to a lane: in one access to each array, or, where weights or gradients lie between its
+  // boundaries, codes alone so.  The last blocks of a tensor, and codes between 4-byte boundaries, go element by element: lane l
+  // holds elements l, l + 32, l + 64 and l + 96 of a block, and what lies behind the tensor is zero.  The first way has a copy of
+  // update() to itself: with one for all three the 39.4 M elements took 117 us instead of 105.
+  // Noise of four elements, `apart` times the hash's factor from one to the next.
+  auto words = [&](long long e, uint32_t apart, uint32_t (&w)[4]) {   // (a block never straddles 2^32)
+    uint32_t h = uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i, h += apart) w[i] = mix(h);
+  };
+  // lane 2j, 2j + 1 of the warp: the scales of block first + j
   float* const scale_at = ((lane & 1) != 0 ? v_scale : m_scale) + first + (lane >> 1);
-  const bool has_scale = lane < 2 * kUnroll && (first + (lane >> 1)) * kBlock < n;
-  if (codes_whole && (first + kUnroll) * kBlock <= n) {
+  if (all_fours) {
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const long long e = (first + j) * kBlock + 4 * lane;
-      load_four<float>(p + e, p_whole, x[j].p);
-      load_four<G>(g + e, g_whole, x[j].g);
+      x[j].p.load(p + e);
+      x[j].g.load(g + e);
       x[j].m = __ldcs(reinterpret_cast<const unsigned int*>(m + e));
       x[j].v = __ldcs(reinterpret_cast<const unsigned int*>(v + e));
       x[j].m_scale = m_scale[first + j];
       x[j].v_scale = v_scale[first + j];
     }
-    const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) {
-      const long long e = (first + j) * kBlock + 4 * lane;
-      uint32_t h = uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i, h += 0x9E3779B1u) w[i] = mix(h);   // four elements never straddle 2^32
-    });
+    const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) { words((first + j) * kBlock + 4 * lane, 0x9E3779B1u, w); });
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const long long e = (first + j) * kBlock + 4 * lane;
-      if (p_whole) {
-        Span<4>::store(p + e, x[j].p);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[e + i] = x[j].p[i];
-      }
+      Span<4>::store(p + e, x[j].p.f);
       __stcs(reinterpret_cast<unsigned int*>(m + e), x[j].m);
       __stcs(reinterpret_cast<unsigned int*>(v + e), x[j].v);
     }
-    if (has_scale) *scale_at = scale;
+    if (lane < 2 * kUnroll) *scale_at = scale;
     return;
   }
-  // The last blocks, and codes between 4-byte boundaries: element by element.  Lane l holds elements l, l + 32, l + 64 and
-  // l + 96 of a block, so that neighbours read neighbours; what lies behind the tensor is zero.
 #pragma unroll
   for (int j = 0; j < kUnroll; ++j) {
-    x[j] = Piece{};
+    x[j] = Piece<G>{};
+    const long long at = (first + j) * kBlock;
+    if (at >= n) continue;
+    x[j].m_scale = m_scale[first + j];
+    x[j].v_scale = v_scale[first + j];
+    if (codes_fours) {
+      const long long e = at + 4 * lane;
+      x[j].m = __ldcs(reinterpret_cast<const unsigned int*>(m + e));
+      x[j].v = __ldcs(reinterpret_cast<const unsigned int*>(v + e));
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long e = (first + j) * kBlock + lane + 32 * i;
-      if (e >= n) continue;
-      x[j].p[i] = p[e];
-      x[j].g[i] = to_float<G>(g[e]);
-      x[j].m |= uint32_t(m[e]) << (8 * i);
-      x[j].v |= uint32_t(v[e]) << (8 * i);
-    }
-    if ((first + j) * kBlock < n) {
-      x[j].m_scale = m_scale[first + j];
-      x[j].v_scale = v_scale[first + j];
+      for (int i = 0; i < 4; ++i) {
+        x[j].p.set(i, p[e + i]);
+        x[j].g.set(i, g[e + i]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long e = at + lane + 32 * i;
+        if (e >= n) continue;
+        x[j].p.set(i, p[e]);
+        x[j].g.set(i, g[e]);
+        x[j].m |= uint32_t(m[e]) << (8 * i);
+        x[j].v |= uint32_t(v[e]) << (8 * i);
+      }
     }
   }
   const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long e = (first + j) * kBlock + lane + 32 * i;
-      w[i] = mix(uint32_t(e) * 0x9E3779B1u + (key + uint32_t(e >> 32) * 0xC2B2AE35u));
-    }
+    words((first + j) * kBlock + (codes_fours ? 4 * lane : lane), codes_fours ? 0x9E3779B1u : 32u * 0x9E3779B1u, w);
   });
 #pragma unroll
-  for (int j = 0; j < kUnroll; ++j)
+  for (int j = 0; j < kUnroll; ++j) {
+    const long long at = (first + j) * kBlock;
+    if (codes_fours) {
+      const long long e = at + 4 * lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const long long e = (first + j) * kBlock + lane + 32 * i;
-      if (e >= n) continue;
-      p[e] = x[j].p[i];
-      m[e] = uint8_t(x[j].m >> (8 * i));
-      v[e] = uint8_t(x[j].v >> (8 * i));
+      for (int i = 0; i < 4; ++i) p[e + i] = x[j].p.f[i];
+      __stcs(reinterpret_cast<unsigned int*>(m + e), x[j].m);
+      __stcs(reinterpret_cast<unsigned int*>(v + e), x[j].v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long e = at + lane + 32 * i;
+        if (e >= n) continue;
+        p[e] = x[j].p.f[i];
+        m[e] = uint8_t(x[j].m >> (8 * i));
+        v[e] = uint8_t(x[j].v >> (8 * i));
+      }
     }
-  if (has_scale) *scale_at = scale;
+  }
+  if (lane < 2 * kUnroll && (first + (lane >> 1)) * kBlock < n) *scale_at = scale;
 }
 
 template <typename G>
