@@ -51,6 +51,8 @@ def adamw_step(group: dict[str, Any], state: ParamState,
         entry = state[param]
         if EXP_AVG_STATE not in entry:
             init_adamw_state(param, entry, bits)
+        if (EXP_AVG_SCALE_STATE in entry) != (bits == 8):
+            raise ValueError(f"a group's {ADAMW_STATE_BITS_KEY} cannot change once its moments exist")
         grad = param.grad
         if grad is None:
             raise RuntimeError("an AdamW update holds a parameter without a gradient")
@@ -75,6 +77,9 @@ def adamw_step(group: dict[str, Any], state: ParamState,
                     hyper_device=None if hyper is None else hyper(device))
     if bits == 8:
         tensors = [*p_list, *g_list, *m_list, *v_list, *scales[0], *scales[1], *s_list]
+        if device.type != "cuda" or set(map(Tensor.get_device, tensors)) != {p_list[0].get_device()}:
+            raise ValueError(f"an AdamW update needs its parameters, gradients and moments on one CUDA device, not {device} and "
+                             f"{sorted({str(t.device) for t in tensors})}")
         _native.adamw8_multi(list(map(Tensor.data_ptr, tensors)), list(map(Tensor.numel, p_list)), torch.float32,
                              device=p_list[0].get_device(), seed=0, **settings)
     else:

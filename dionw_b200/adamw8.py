@@ -62,7 +62,7 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
     """One decoupled-decay, bias-corrected AdamW step of every parameter, in place.
 
     Args:
-        params: fp32 CUDA tensors of one device, contiguous, each once.
+        params: fp32 CUDA tensors of one device, contiguous, each once.  What is written must not overlap.
         grads: Their gradients, of one dtype (float32, float16 or bfloat16), contiguous.
         exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, steps: The state, as ``adamw8_state`` makes
             it.  Every step counter goes up by one.
@@ -109,10 +109,11 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
     if list(map(Tensor.numel, tensors[n:])) != numels * 3 + blocks * 2 + [1] * n:
         raise ValueError("adamw8_step: gradients, moments or scales do not have the sizes that their parameters need")
     addresses = list(map(Tensor.data_ptr, tensors))
-    if len(set(addresses[:n])) != n and len({a for a, k in zip(addresses, numels) if k}) != sum(map(bool, numels)):
-        raise ValueError("adamw8_step: a parameter is given twice")
-    if len(set(addresses[6 * n:])) != n:
-        raise ValueError("adamw8_step: a step counter is given twice")
+    written = addresses[:n] + addresses[2 * n:]
+    if len(set(written)) != 6 * n:   # tensors without elements may share an address
+        written = [a for a, k in zip(written, numels * 5 + [1] * n) if k]
+        if len(set(written)) != len(written):
+            raise ValueError("adamw8_step: a parameter, a moment, a scale or a step counter is given twice")
     if hyper_device is not None and (hyper_device.get_device() != device or hyper_device.dtype is not torch.float32
                                      or hyper_device.numel() != 2 or not hyper_device.is_contiguous()):
         raise ValueError("adamw8_step: hyper_device must be two contiguous float32 on the parameters' device")

@@ -379,6 +379,8 @@ extern "C" int dionw_adamw8_multi(void* const* params, const void* const* grads,
                                   double beta2, float weight_decay, float eps, uint32_t seed,
                                   const float* hyper_device, void* stream_ptr) {
   DIONW_REQUIRE(n_tensors >= 0, "adamw8_multi: negative tensor count");
+  DIONW_REQUIRE(n_tensors == 0 || (params && grads && exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && steps && numels),
+                "adamw8_multi: null list");
   DIONW_REQUIRE(grad_dtype >= DIONW_F32 && grad_dtype <= DIONW_BF16, "adamw8_multi: bad gradient dtype");
   DIONW_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0, "adamw8_multi: betas must be in [0, 1)");
   cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);

@@ -134,6 +134,8 @@ extern "C" int dionw_float8_linear_forward(const void* x, int x_dtype, int64_t l
                                            void* stream) {
   int st = check_shape("float8_linear_forward", tokens, inputs, outputs);
   if (st != DIONW_OK) return st;
+  DIONW_REQUIRE(work != nullptr && aligned16(work) && aligned16(x_kept) && aligned16(weight_kept),
+                "float8_linear_forward: packed matrices need 16-byte aligned room");
   const Packed x_rows(tokens, inputs, 0), x_columns(inputs, tokens, 0);
   const Packed w_tiles(outputs, inputs, 1), w_turned(inputs, outputs, 1);
   char* w_at = static_cast<char*>(work) + x_rows.bytes;
@@ -150,6 +152,8 @@ extern "C" int dionw_float8_linear_backward(const void* dy, int dy_dtype, int64_
   if (st != DIONW_OK) return st;
   DIONW_REQUIRE((dx == nullptr || weight_kept != nullptr) && (dw == nullptr || x_kept != nullptr),
                 "float8_linear_backward: a gradient without what the forward pass keeps for it");
+  DIONW_REQUIRE(((dx == nullptr && dw == nullptr) || work != nullptr) && aligned16(work) && aligned16(x_kept) && aligned16(weight_kept),
+                "float8_linear_backward: packed matrices need 16-byte aligned room");
   const Packed rows(tokens, outputs, 0), columns(outputs, tokens, 0);
   const Packed x_columns(inputs, tokens, 0), w_turned(inputs, outputs, 1);
   void* rows_at = dx != nullptr ? work : nullptr;

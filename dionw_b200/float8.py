@@ -12,6 +12,7 @@ There is no counterpart in the reference.
 from __future__ import annotations
 
 import functools
+import math
 from dataclasses import dataclass
 from typing import Any
 
@@ -134,7 +135,7 @@ def quantize_rows(x: Tensor, *, transposed: bool = False) -> Any:
 
     Codes are rounded to nearest even; a scale is the least power of two that keeps its block in range.
     With ``transposed=True`` returns a pair: the matrix and its transpose (scales along ``x``'s columns),
-    from one read.
+    from one read.  No gradient passes through (``float8_linear`` has its own).
 
     Raises:
         ValueError: If ``x`` is not a CUDA matrix.
@@ -153,7 +154,8 @@ def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = No
     """``a @ b.T`` (``a`` ``[m, k]``, ``b`` ``[n, k]``), plus ``bias`` ``[n]``, summed in fp32 and rounded once.
 
     Args:
-        out: ``[m, n]`` result (float32, float16 or bfloat16), rows contiguous; made if None.
+        out: ``[m, n]`` result (float32, float16 or bfloat16), rows contiguous; made if None.  Must not overlap
+            ``a``, ``b`` or ``bias``.
         accumulate: Add to what ``out`` holds.
         out_dtype: Of the result that is made (bfloat16 if None); must be ``out``'s where both are given.
 
@@ -260,7 +262,8 @@ def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tens
 
     ``x`` is ``[..., inputs]``, ``weight`` ``[outputs, inputs]`` (an fp32 master weight, or 2 bytes), the result has
     ``x``'s dtype, and the weight's gradient the weight's.  Activations and output gradients get a scale for each 1 x 128
-    block along the side that is summed over, the weight one for each 128 x 128 tile.
+    block along the side that is summed over, the weight one for each 128 x 128 tile.  Both passes may be captured into
+    a CUDA graph; as with any layer, let no graph of an eager call on the same leaves live on meanwhile.
 
     Raises:
         ValueError: On shapes that do not fit, or tensors off CUDA or on different devices.
@@ -277,7 +280,8 @@ def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tens
         raise ValueError(f"float8_linear: bias {tuple(bias.shape)} does not fit a weight {tuple(weight.shape)}")
     if x.ndim == 2:
         return _Linear.apply(x, weight, bias)
-    return _Linear.apply(x.reshape(-1, x.shape[-1]), weight, bias).view(*x.shape[:-1], weight.shape[0])
+    leading = x.shape[:-1]
+    return _Linear.apply(x.reshape(math.prod(leading), x.shape[-1]), weight, bias).view(*leading, weight.shape[0])
 
 
 class Float8Linear(nn.Linear):

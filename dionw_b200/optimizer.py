@@ -200,7 +200,7 @@ class _DionCore(Optimizer):
         if isinstance(members, set):
             raise TypeError("Dion param group params must be ordered, not a set")
         group = {**param_group, "params": [members] if isinstance(members, Tensor) else list(members)}
-        if self._adamw_state_bits == 8 and group.get(ROUTE_KEY) == RouteKind.ADAMW.value:
+        if self._adamw_state_bits == 8 and group.get(ROUTE_KEY) in (RouteKind.ADAMW, RouteKind.ADAMW.value):
             group.setdefault(ADAMW_STATE_BITS_KEY, 8)
         for param in group["params"]:
             _require_param(param)

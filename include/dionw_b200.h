@@ -283,10 +283,10 @@ int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, 
  * where a_tiles != 0 (b likewise).  out must not overlap an operand.  Results do not depend on
  * anything but the operands: sums are taken in a fixed order.  a_exponents and b_exponents
  * (both or neither, 16-byte aligned): the scales as dionw_float8_quantize wrote them a second
- * time; large products then leave them to the tensor cores and sum in one piece.  Without
- * them, and with a workspace (nullable, 16-byte aligned, of the bytes that the function below
- * says, 0 for small products), a large product first looks whether all scales are powers of two
- * (or NaN) and does the same if so. */
+ * time; a product with m above 64 then leaves them to the tensor cores.  Without them, and with a
+ * workspace (nullable, 16-byte aligned, of the bytes that the function below says, 0 for small
+ * products), a large product first looks whether all scales are powers of two (or NaN) and does
+ * the same if so. */
 int dionw_float8_product(const void* a, int64_t lda, const float* a_scales, int64_t a_row_stride,
                          int64_t a_block_stride, int a_tiles, const void* b, int64_t ldb,
                          const float* b_scales, int64_t b_row_stride, int64_t b_block_stride,

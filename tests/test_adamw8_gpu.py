@@ -40,6 +40,13 @@ def _tensors(sizes: list[int], dtype: torch.dtype = torch.float32, shift: int = 
     return out
 
 
+def _shift_codes(t: dict[str, list[Tensor]], key: str, shift: int) -> None:
+    for i, codes in enumerate(t[key]):
+        room = torch.zeros(codes.numel() + shift, dtype=torch.uint8, device=DEV)
+        room[shift:] = codes.view(torch.uint8)
+        t[key][i] = room[shift:].view(codes.dtype)
+
+
 def _moments(t: dict[str, list[Tensor]], i: int) -> tuple[Tensor, Tensor]:
     return dequantize_moments({"exp_avg": t["m"][i], "exp_avg_sq": t["v"][i], "exp_avg_scale": t["ms"][i],
                                "exp_avg_sq_scale": t["vs"][i]})
@@ -91,6 +98,26 @@ def test_step_of_sizes(sizes) -> None:
 @pytest.mark.parametrize("shift", [0, 1, 2])
 def test_step_of_gradient_types_and_alignments(dtype, shift) -> None:
     _check(_tensors([1000, 4096 + 128], dtype, shift, seed=3))
+
+
+@pytest.mark.parametrize("keys", ["m", "v", "mv"])
+@pytest.mark.parametrize("shift", [1, 2, 3, 4])
+def test_step_of_codes_between_words(keys, shift) -> None:
+    t = _tensors([3000, 129, 1], torch.bfloat16, seed=shift)
+    for key in keys:
+        _shift_codes(t, key, shift)
+    _check(t)
+
+
+def test_what_is_written_twice_is_refused() -> None:
+    for key in ("p", "m", "v", "ms", "vs", "t"):
+        t = _tensors([256, 256])
+        t[key][1] = t[key][0]
+        with pytest.raises(ValueError, match="given twice"):
+            _step(t)
+    t = _tensors([256, 0, 0, 256])
+    t["g"][3] = t["g"][0]     # a gradient may serve two
+    _check(t)
 
 
 @pytest.mark.parametrize("more", [

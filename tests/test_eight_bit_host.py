@@ -236,6 +236,36 @@ def test_dion_state_bits_are_checked() -> None:
             _require_same_structure([{**plain, "adamw_state_bits": old}], [{**plain, "adamw_state_bits": new}])
 
 
+def test_a_step_of_tensors_elsewhere_or_of_other_moments_is_refused() -> None:
+    from dionw_b200._adamw import adamw_step, init_adamw_state
+
+    param = torch.zeros(300, requires_grad=True)
+    param.grad = torch.ones(300)
+    group = {"params": [param], "lr": 1e-3, "betas": (0.9, 0.95), "eps": 1e-8, "weight_decay": 0.0}
+    state: dict = {param: dionw.adamw8_state(param)}
+    with pytest.raises(ValueError, match="one CUDA device"):
+        adamw_step({**group, "adamw_state_bits": 8}, state)
+    with pytest.raises(ValueError, match="cannot change"):
+        adamw_step(group, state)
+    state[param] = {}
+    init_adamw_state(param, state[param])
+    with pytest.raises(ValueError, match="cannot change"):
+        adamw_step({**group, "adamw_state_bits": 8}, state)
+
+
+def test_lists_and_room_that_are_missing_are_refused() -> None:
+    lib = _native.library()
+    at = 1 << 20
+    assert lib.dionw_adamw8_multi(at, at, 0, at, at, at, at, None, at, 1, 1e-3, 0.9, 0.95, 0.0, 1e-8, 0, None, None) == -1
+    assert "null list" in _native.last_error()
+    assert lib.dionw_float8_linear_forward(at, 0, 8, at, 0, 8, None, 0, at, 4, 8, 8, None, None, None, None) == -1
+    assert "room" in _native.last_error()
+    assert lib.dionw_float8_linear_forward(at, 0, 8, at, 0, 8, None, 0, at, 4, 8, 8, at, at + 8, None, None) == -1
+    assert "room" in _native.last_error()
+    assert lib.dionw_float8_linear_backward(at, 0, 8, at, 0, None, 0, None, 4, 8, 8, None, None, at, None) == -1
+    assert "room" in _native.last_error()
+
+
 def test_linear_entries_refuse() -> None:
     lib = _native.library()
     at = 1 << 20

@@ -382,6 +382,11 @@ def test_linear_of_any_leading_shape_and_partial_gradients() -> None:
     assert dx.shape == empty.shape and float(dw.abs().max()) == 0.0
     with torch.autocast("cuda", torch.bfloat16):
         assert layer(x.float()).dtype is torch.bfloat16
+    # no inputs: the bias alone
+    bias = torch.randn(5, device=DEV)
+    nothing = dionw.float8_linear(torch.zeros(2, 3, 0, device=DEV), torch.zeros(5, 0, device=DEV), bias)
+    assert torch.equal(nothing, bias.expand(2, 3, 5))
+    assert dionw.float8_linear(x[0, 0, 0], layer.weight).shape == (48,)
 
 
 def test_linear_forward_and_backward_in_a_graph() -> None:
