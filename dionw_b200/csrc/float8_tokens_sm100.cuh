@@ -4,8 +4,13 @@
 // Bound by the weights' bytes, 16 KB for each block and SM: at 6.5 TB/s and 148 SMs some 700 cycles.  With a barrier for
 // each block, in the ring, to the summing warps and back, the warp that issues the MMAs took 780 cycles a block whatever the
 // ring's depth (1 x 4096 x 14336 45.7 us, without the summing warps' barriers 34, with one MMA of the four 26): so stages and
-// accumulators are of four blocks, with a barrier for all four.  Where tiles are few, a cluster of two to eight CTAs shares
-// a tile, each with a part of the blocks, and adds the parts in the order of their ranks through one another's shared memory.
+// accumulators are of four blocks, with a barrier for all four.  A lane fetches its row's scales of four blocks at once, 16 bytes
+// where they lie so: 4-byte copies of 32 rows are 32 lines each, and 64 x 14336 x 4096 took 23.5 us with them instead of 16.9.
+// Where tiles are few, a cluster of two to eight CTAs shares a tile, each with a part of the blocks, and adds the parts in the
+// order of their ranks through one another's shared memory.
+//
+// 1 x 14336 x 4096 takes 13.0 us, of which 3 are those of a launch that reads next to nothing; without the sums it takes 12.6.
+// More bytes in flight (three stages) and tiles of fewer rows on more SMs changed nothing.
 #pragma once
 
 #include "float8_sm100.cuh"
@@ -24,9 +29,33 @@ struct Shape {
   static constexpr uint32_t kStageBytes = kGroup * kBlockBytes;
   static constexpr int kStages = 2;
   static constexpr uint32_t kTmemCols = kSets * kGroup * kTokens;  // 128, 256 or 512
-  using Queue = ScaleQueue<kRowScales ? kColumns : 0, 8>;
-  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kSumWarps * Queue::kBytes + 256 + 1024;
+  // The tokens' scales of four blocks, block after block, twice, for each summing warp.
+  static constexpr uint32_t kScaleBytes = kRowScales ? 2 * kGroup * kColumns * 4 : 0;
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + kSumWarps * kScaleBytes + 256 + 1024;
   static_assert(kTokens * kBM * 4 <= kStages * kStageBytes, "the parts of a tile lie where the ring was");
+};
+
+// The scales of one row of an operand, four blocks at a time.
+struct RowScales {
+  const float* at;           // nullptr: the row is not there, its scales are zero
+  int64_t block_stride;
+  bool whole;                // four blocks' lie in 16 aligned bytes
+
+  __device__ __forceinline__ RowScales(const Scales& s, int row, int rows, int first_block)
+      : at(row < rows ? s.base + int64_t(row >> s.shift) * s.row_stride + first_block * s.block_stride : nullptr),
+        block_stride(s.block_stride), whole(s.block_stride == 1 && (reinterpret_cast<uintptr_t>(at) & 15u) == 0) {}
+  // Of blocks k0 .. k0 + 3; zero from block `blocks` on.
+  __device__ __forceinline__ float4 four(int k0, int blocks) const {
+    float4 f = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (at == nullptr || k0 >= blocks) return f;
+    const float* from = at + k0 * block_stride;
+    if (whole && k0 + kGroup <= blocks) return __ldg(reinterpret_cast<const float4*>(from));
+    f.x = __ldg(from);
+    if (k0 + 1 < blocks) f.y = __ldg(from + block_stride);
+    if (k0 + 2 < blocks) f.z = __ldg(from + 2 * block_stride);
+    if (k0 + 3 < blocks) f.w = __ldg(from + 3 * block_stride);
+    return f;
+  }
 };
 
 template <typename T, int kTokens, bool kRowScales>
@@ -35,10 +64,11 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   using namespace gemm;
   using S = Shape<kTokens, kRowScales>;
   constexpr int kStages = S::kStages, kColumns = S::kColumns;
+  constexpr int kChunk = kColumns < 16 ? kColumns : 16, kChunks = kColumns / kChunk;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* queues = smem + size_t(kStages) * S::kStageBytes;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(queues + kSumWarps * S::Queue::kBytes);   // a stage's codes are there
+  float* token_scales = reinterpret_cast<float*>(smem + size_t(kStages) * S::kStageBytes);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(token_scales + kSumWarps * S::kScaleBytes / 4);   // a stage's codes are there
   uint64_t* empty_bar = full_bar + kStages;     // its MMAs are done
   uint64_t* acc_full = empty_bar + kStages;     // [kSets] the sums of four blocks are complete
   uint64_t* acc_empty = acc_full + kSets;       // [kSets] they are read
@@ -48,7 +78,7 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // A cluster's CTAs share a tile: CTA `rank` takes the blocks from first_block on.  (One tile a cluster of several CTAs.)
   const int parts = int(cluster_size()), rank = int(cluster_rank());
-  const int all_blocks = (p.k + kBK - 1) / kBK, share = (all_blocks + parts - 1) / parts;
+  const int all_blocks = (p.k + kBK - 1) / kBK, share = ((all_blocks + parts - 1) / parts + kGroup - 1) / kGroup * kGroup;
   const int first_block = min(rank * share, all_blocks), k_blocks = min(share, all_blocks - first_block);
   const int first_tile = int(blockIdx.x) / parts, stride = int(gridDim.x) / parts;
 
@@ -139,30 +169,69 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
     const int sub = warp & 3;
     const int first_token = ((warp - 2) >> 2) * kColumns;
     const uint32_t tmem_mine = tmem_base + uint32_t(first_token) + (uint32_t(sub * 32) << 16);
-    typename S::Queue queue(queues + (warp - 2) * S::Queue::kBytes);
+    float* const scales_here = token_scales + (warp - 2) * (S::kScaleBytes / 4);
     uint32_t it = 0;
     bool ok = true;
     for (int t = first_tile; t < p.tiles_m; t += stride) {
       const int row0 = t * kBM + sub * 32;
-      queue.start(p, row0, first_token, first_block, k_blocks, lane);
+      // Scales are two groups of blocks ahead, in registers: a row's for its lane, and a token's each for the first kColumns lanes.
+      const RowScales weights(p.a, row0 + lane, p.m, first_block);
+      const RowScales tokens(p.b, kRowScales ? first_token + (lane < kColumns ? lane : 0) : 0, p.n, first_block);
+      float4 row_scales[3], token_scales4[3];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        row_scales[i] = weights.four(kGroup * i, k_blocks);
+        token_scales4[i] = tokens.four(kGroup * i, k_blocks);
+      }
       uint64_t sum[kColumns / 2];
 #pragma unroll
       for (int c = 0; c < kColumns / 2; ++c) sum[c] = 0;
       for (int k0 = 0; k0 < k_blocks; k0 += kGroup, ++it) {
         const uint32_t set = it % kSets;
         const int count = min(kGroup, k_blocks - k0);
+        row_scales[2] = weights.four(k0 + 2 * kGroup, k_blocks);
+        token_scales4[2] = tokens.four(k0 + 2 * kGroup, k_blocks);
+        float factor[kGroup] = {row_scales[0].x, row_scales[0].y, row_scales[0].z, row_scales[0].w};
+        const float4 of_token = token_scales4[0];
+        float* const by_block = scales_here + (it & 1u) * (kGroup * kColumns);
+        if constexpr (kRowScales) {
+          if (lane < kColumns) {       // (the other half of the room may still be read)
+            by_block[lane] = of_token.x;
+            by_block[kColumns + lane] = of_token.y;
+            by_block[2 * kColumns + lane] = of_token.z;
+            by_block[3 * kColumns + lane] = of_token.w;
+          }
+        } else {
+          factor[0] *= of_token.x; factor[1] *= of_token.y; factor[2] *= of_token.z; factor[3] *= of_token.w;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          row_scales[i] = row_scales[i + 1];
+          token_scales4[i] = token_scales4[i + 1];
+        }
         if (!warp_wait(&acc_full[set], (it / kSets) & 1u)) { ok = false; break; }
+        __syncwarp();
         tc_fence_after();
-        for (int j = 0; j < count; ++j)
-          add_block<kColumns, kColumns >= 32 ? 16 : kColumns >= 16 ? kColumns / 2 : kColumns, kRowScales>(
-              tmem_mine + (set * kGroup + uint32_t(j)) * kTokens, lane, sum,
-              [&] { return queue.take(p, k_blocks - 1 - k0 - j, lane); },
-              [&] {
-                if (j + 1 < count) return;
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&acc_empty[set]);
-              });
+        // A chunk of a block's sums is on its way from TMEM while the one before is added.
+        const uint32_t accumulators = tmem_mine + set * kGroup * kTokens;
+        uint32_t v[2][kChunk];
+        tmem_load<kChunk>(accumulators, v[0]);
+#pragma unroll
+        for (int i = 0; i < kGroup * kChunks; ++i) {
+          const int j = i / kChunks, c0 = i % kChunks * kChunk, next = i + 1;
+          if (j >= count) break;
+          tmem_wait<kChunk>(v[i & 1]);
+          if (next < count * kChunks) {
+            if (next < kGroup * kChunks)
+              tmem_load<kChunk>(accumulators + uint32_t(next / kChunks * kTokens + next % kChunks * kChunk), v[next & 1]);
+          } else {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[set]);
+          }
+          add_columns<kChunk, kRowScales>(v[i & 1], two(__float_as_uint(factor[j]), __float_as_uint(factor[j])),
+                                          by_block + j * kColumns + c0, sum + c0 / 2);
+        }
       }
       if (!ok) break;
       const int column = row0 + lane;            // of the output: 32 lanes write neighbours
@@ -188,7 +257,6 @@ product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant_
         }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   }
 
   // ------------------------------------------------------------ a tile's parts
