@@ -36,6 +36,12 @@ __device__ __forceinline__ uint32_t peer_address(const void* local, uint32_t ran
   return out;
 }
 
+__device__ __forceinline__ float4 peer_load4(const void* local, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer_address(local, rank)) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t peer_load(const void* local, uint32_t rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(peer_address(local, rank)) : "memory");

@@ -54,12 +54,49 @@ int code_maps(CUtensorMap& map_a, CUtensorMap& map_b, const void* a, int64_t lda
   return st != DIONW_OK ? st : make_byte_map(&map_b, b, p.k, p.n, ldb, float8::kBK, b_rows);
 }
 
-// 128 x 128 tiles.
-template <typename T, bool kRowScales>
-int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, cudaStream_t stream) {
+// Clusters of so many CTAs, one to an SM, that run at once.  (Of 148 SMs the driver counts 74 of two, 33 of four and 15 of eight.)
+long long cluster_slots(unsigned parts) {
+  return parts == 8 ? sm_count() / 8 - 3 : parts == 4 ? sm_count() / 4 - 4 : sm_count() / parts;
+}
+
+// How many CTAs share a tile: what costs least, `round` for a block that SMs go through one after the other and `join` for adding
+// the parts.
+struct Split {
+  unsigned parts;
+  long long cost;
+  Split(long long tiles, long long blocks, int round, int join) : parts(1), cost(0) {
+    for (unsigned p = 1; p <= unsigned(float8::kMaxParts); p *= 2) {
+      const long long slots = cluster_slots(p);
+      if (slots < 1) break;
+      const long long c = (tiles + slots - 1) / slots * ((blocks + p - 1) / p) * round + (p > 1 ? join : 0);
+      if (p == 1 || c < cost) {
+        parts = p;
+        cost = c;
+      }
+    }
+  }
+};
+
+// A product of more than 64 rows whose 256 x 256 tiles would not fill the SM pairs: 128 x 128 tiles, or 256 x 128 ones of pairs where
+// the tensor cores apply the scales.  Costs in 0.14 us: a block takes 0.7 us and 0.28, adding the parts 2.8.  Measured, one CTA to a
+// tile and parts (us): 200 x 200 x 8192 42.7 and 11.4 (eight), 128 x 4096 x 4096 22.5 and 10.2 (four), 1000 x 768 x 2304 14.5 and 10.1
+// (two), 1024^3 6.8 and 8.2 (two: it stays with one).
+struct Shapes {
+  Split own;
+  long long scaled;
+  Shapes(long long m, long long n, long long k)
+      : own(((m + 127) / 128) * ((n + 127) / 128), (k + 127) / 128, 5, 20) {
+    const long long pairs = sm_count() / 2, tiles = ((m + 255) / 256) * ((n + 127) / 128);
+    scaled = (tiles + pairs - 1) / pairs * ((k + 127) / 128) * 2;
+  }
+};
+
+// 128 x 128 tiles, each shared by `parts` CTAs.
+template <typename T, bool kRowScales, bool kSplit>
+int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p, unsigned parts, cudaStream_t stream) {
   using S = float8::Shape<kRowScales>;
   static_assert(S::kSmemBytes <= 227 * 1024, "shared memory of a CTA");
-  auto kernel = float8::product_kernel<T, kRowScales>;
+  auto kernel = float8::product_kernel<T, kRowScales, kSplit>;
   static std::atomic<bool> configured[kMaxDevices];
   int st = allow_shared(kernel, S::kSmemBytes, configured);
   CUtensorMap map_a{}, map_b{};
@@ -69,8 +106,8 @@ int launch_single(const void* a, int64_t lda, const void* b, int64_t ldb, float8
   p.tiles_n = (p.n + float8::kTileN - 1) / float8::kTileN;
   const long long total = (long long)p.tiles_m * p.tiles_n;
   DIONW_REQUIRE(total <= 0x7FFFFFFFll, "float8_product: too many tiles");
-  return launch_in_clusters(kernel, unsigned(total < sm_count() ? total : sm_count()), 1, S::kSmemBytes, float8::kThreads, p,
-                            stream, map_a, map_b);
+  return launch_in_clusters(kernel, kSplit ? parts * unsigned(total) : unsigned(total < sm_count() ? total : sm_count()), parts,
+                            S::kSmemBytes, float8::kThreads, p, stream, map_a, map_b);
 }
 
 // Up to kTokens rows of B, tiles of 128 rows of A.
@@ -86,10 +123,8 @@ int launch_tokens(const void* a, int64_t lda, const void* b, int64_t ldb, float8
   if (st != DIONW_OK) return st;
   p.tiles_m = (p.m + float8::kBM - 1) / float8::kBM;
   p.tiles_n = 1;
-  // A tile's blocks are shared out while that keeps more SMs busy, and each part has two stages at least.
-  const int blocks = (p.k + 127) / 128;
-  unsigned parts = 1;
-  while (parts < 8 && 2 * parts * p.tiles_m <= sm_count() && blocks >= int(4 * parts * float8::tokens::kGroup)) parts *= 2;
+  // A tile's blocks are shared out by groups; adding the parts costs about as much as a group.
+  const unsigned parts = Split(p.tiles_m, ((p.k + 127) / 128 + float8::tokens::kGroup - 1) / float8::tokens::kGroup, 1, 1).parts;
   const unsigned ctas = parts > 1 || p.tiles_m < sm_count() ? parts * p.tiles_m : sm_count();
   return launch_in_clusters(kernel, ctas, parts, S::kSmemBytes, float8::kThreads, p, stream, map_a, map_b);
 }
@@ -195,14 +230,27 @@ exponents_kernel(const ExponentJob a, const ExponentJob b, int* odd) {
 
 long long pair_tiles(long long m, long long n) { return ((m + 255) / 256) * ((n + 255) / 256); }
 
-// Whether a product looks at its scales, to leave them to the tensor cores where they are powers of two: where its SMs would
-// otherwise go through 18 blocks of 128 x 128 tiles or more, one after the other.  The two launches more cost 5 us.
-// Measured, own sums against looking first (us): 6 blocks (1000 x 2304 x 768) 7.2 and 10.7, 8 (1024^3) 7.0 and 9.6, 16 (300 x 700 x
-// 2048) 14.3 and 15.2, 18 (1000 x 768 x 2304) 12.5 and 12.5, 23 (1531 x 1100 x 2927) 25.3 and 20.1, 32 (2048^3) 20.3 and 17.8,
-// 64 (256 x 14336 x 4096) 36 and 27, 112 (512 x 4096 x 14336) 54 and 41.
+bool wide(long long m, long long n) { return pair_tiles(m, n) >= sm_count() / 2; }
+
+// Whether a product looks at its scales, to leave them to the tensor cores where they are powers of two; the two launches more cost 5
+// us.  Measured, own sums against looking first (us): 1000 x 2304 x 768 7.2 and 10.7, 1000 x 768 x 2304 10.1 and 12.8, 1024 x 1024 x 4096
+// 14.0 and 16.2, 1531 x 1100 x 2927 25.3 and 18.1, 2048^3 20.3 and 17.8, 512 x 4096 x 14336 54 and 40.  256 x 256 tiles: from 18 blocks
+// of 128 x 128 on that SMs would go through one after the other.
 bool takes_exponents(long long m, long long n, long long k) {
-  const long long tiles = ((m + 127) / 128) * ((n + 127) / 128);
-  return m > 64 && (tiles + sm_count() - 1) / sm_count() * ((k + 127) / 128) >= 18;
+  if (m <= 64) return false;
+  if (wide(m, n)) return (((m + 127) / 128) * ((n + 127) / 128) + sm_count() - 1) / sm_count() * ((k + 127) / 128) >= 18;
+  const Shapes shapes(m, n, k);
+  return shapes.scaled + 36 < shapes.own.cost;
+}
+
+// Whether a product that is given its exponents uses them: unless it has so few tiles that parts of them, with sums of its own, are
+// faster.  Measured, own sums against tensor cores (us): 65 x 256 x 4096 8.2 and 12.3, 200 x 200 x 8192 11.4 and 21.2, 128 x 4096 x 4096
+// 12.5 and 13.1, 256 x 2048 x 2048 9.7 and 7.9, 512 x 2048 x 4096 17.2 and 12.8, 128 x 1024 x 1024 7.7 and 6.3.
+bool prefers_exponents(long long m, long long n, long long k) {
+  if (m <= 64) return false;
+  if (wide(m, n)) return true;
+  const Shapes shapes(m, n, k);
+  return shapes.scaled <= shapes.own.cost;
 }
 
 // Scratch of a product whose scales are looked at: a word a CTA, and both operands' exponents.
@@ -219,7 +267,7 @@ struct ExponentRoom {
 template <typename T>
 int run_scaled(const void* a, int64_t lda, const void* ea, const void* b, int64_t ldb, const void* eb, const float8::Params& p,
                cudaStream_t stream) {
-  if (pair_tiles(p.m, p.n) >= sm_count() / 2) return launch_scaled<T, 256>(a, lda, ea, b, ldb, eb, p, stream);
+  if (wide(p.m, p.n)) return launch_scaled<T, 256>(a, lda, ea, b, ldb, eb, p, stream);
   return launch_scaled<T, 128>(a, lda, ea, b, ldb, eb, p, stream);
 }
 
@@ -239,9 +287,14 @@ int run(const void* a, int64_t lda, const void* b, int64_t ldb, float8::Params p
     };
     return p.b.shift == 0 ? launch(std::true_type()) : launch(std::false_type());
   }
-  if (pair_tiles(p.m, p.n) >= sm_count() / 2)
+  if (wide(p.m, p.n))
     return p.b.shift != 0 ? launch_pairs<T, false>(a, lda, b, ldb, p, stream) : launch_pairs<T, true>(a, lda, b, ldb, p, stream);
-  return p.b.shift != 0 ? launch_single<T, false>(a, lda, b, ldb, p, stream) : launch_single<T, true>(a, lda, b, ldb, p, stream);
+  const unsigned parts = Shapes(p.m, p.n, p.k).own.parts;
+  if (parts > 1)
+    return p.b.shift != 0 ? launch_single<T, false, true>(a, lda, b, ldb, p, parts, stream)
+                          : launch_single<T, true, true>(a, lda, b, ldb, p, parts, stream);
+  return p.b.shift != 0 ? launch_single<T, false, false>(a, lda, b, ldb, p, 1, stream)
+                        : launch_single<T, true, false>(a, lda, b, ldb, p, 1, stream);
 }
 
 }  // namespace
@@ -293,11 +346,10 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
     if (out_dtype == DIONW_F16) return run_scaled<__half>(a, lda, ea, b, ldb, eb, p, stream);
     return run_scaled<__nv_bfloat16>(a, lda, ea, b, ldb, eb, p, stream);
   };
-  if (a_exponents != nullptr && b_exponents != nullptr && k > 0 && m > 64) {
+  if (a_exponents != nullptr && b_exponents != nullptr) {
     DIONW_REQUIRE(aligned16(a_exponents) && aligned16(b_exponents), "float8_product: exponents must be 16-byte aligned");
-    return scaled(a_exponents, b_exponents);
-  }
-  if (takes_exponents(m, n, k)) {
+    if (k > 0 && prefers_exponents(m, n, k)) return scaled(a_exponents, b_exponents);
+  } else if (takes_exponents(m, n, k)) {
     const ExponentRoom room(m, n, k);
     if (workspace != nullptr) {
       DIONW_REQUIRE(aligned16(workspace), "float8_product: the workspace must be 16-byte aligned");

@@ -152,7 +152,7 @@ def test_product_of_many_tiles(m, n, k, b_tiles) -> None:
     _close(dionw.float8_product(a, b, out=held.to(DEV), accumulate=True), a64, b64, held.double())
 
 
-@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 1153), (300, 260, 2400)])
+@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 1153), (300, 260, 2400), (1300, 1100, 2900)])
 @pytest.mark.parametrize("b_tiles", [False, True])
 @pytest.mark.parametrize("layout", ["rows", "blocks"])
 def test_product_of_many_tiles_and_powers_of_two(m, n, k, b_tiles, layout) -> None:
@@ -167,7 +167,8 @@ def test_product_of_many_tiles_and_powers_of_two(m, n, k, b_tiles, layout) -> No
     def values(x: Float8Matrix) -> Tensor:
         return oracle.spread(x.values.cpu().float(), x.scales.cpu())
 
-    assert _native.float8_product_workspace_bytes(0, m, n, k) > 0
+    # (the few tiles of the third one are shared out instead)
+    assert (_native.float8_product_workspace_bytes(0, m, n, k) > 0) == (m != 300)
     for dtype in DTYPES[:2]:
         _close(dionw.float8_product(a, b, out_dtype=dtype), values(a), values(b))
     for x, at in ((a, (0, 0)), (a, (-1, -1)), (b, (0, 0)), (b, (-1, -1))):
