@@ -420,14 +420,14 @@ def float8_product_workspace_bytes(device: int, m: int, n: int, k: int) -> int:
 
 
 def float8_product(device: int, a: tuple[int, int, int, int, int, bool], b: tuple[int, int, int, int, int, bool],
-                   bias: Tensor | None, out: Tensor, accumulate: bool, m: int, n: int, k: int,
+                   bias: Tensor | None, out: Tensor, ldo: int, accumulate: bool, m: int, n: int, k: int,
                    workspace: Tensor | None) -> None:
     """``a`` and ``b``: address and leading dimension of the codes, address and the two strides of the scales, and
     whether those are tiles'."""
+    room, room_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
     on_device(device, library().dionw_float8_product, *a, *b, None if bias is None else bias.data_ptr(),
-              0 if bias is None else _DTYPE_CODE[bias.dtype], out.data_ptr(), out.stride(0) if m > 1 else n,
-              _DTYPE_CODE[out.dtype], accumulate, m, n, k, None, None,
-              *((None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())))
+              0 if bias is None else _DTYPE_CODE[bias.dtype], out.data_ptr(), ldo, _DTYPE_CODE[out.dtype], accumulate, m, n, k,
+              None, None, room, room_bytes)
 
 
 def float8_packed_bytes(rows: int, cols: int, tiles: bool) -> int:

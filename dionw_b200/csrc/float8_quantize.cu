@@ -10,8 +10,11 @@
 // came in: row maxima are maxima over the 16 lanes of a row, column maxima over the 32 row groups go through shared
 // memory, and so do the codes on their way into the transposed matrix.
 //
-// HBM-bound where enough is in flight.  With eight rows a thread, as fp32, an SM held 16 warps of 104 registers: 8192 x 4096 bf16
-// in both orders 46.8 us, 14336 x 4096 fp32 in tiles 69.6 us.
+// HBM-bound: 14336 x 4096 fp32 in tiles and both orders 61.3 us, 5.7 TB/s; 8192 x 4096 bf16 by rows 17.4 us, 5.8 TB/s.  Both orders
+// of that, with a byte written for each byte read and two scales for each value, take 27.5 us, 4.9 TB/s: two thirds of the issue
+// slots are taken, and three barriers a tile keep the rest from being filled.  With eight rows a thread, as fp32, an SM held 16
+// warps of 104 registers: 46.8 us, and 69.6 for the tiles.  Asynchronous copies a tile ahead changed nothing (27.9), two ahead took
+// 33.6.
 #include <type_traits>
 
 #include "cluster.cuh"

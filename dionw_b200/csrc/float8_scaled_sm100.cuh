@@ -14,6 +14,9 @@
 //
 // A tile's 256 columns are half of TMEM and there is one of them: the eight warps take it into registers at once, and
 // convert and store while the next tile is computed.  Tiles of 256 x 128 are for products that have too few of the wide ones.
+//
+// 8192 x 14336 x 4096 takes 350 us in short runs, 2.75 PFLOP/s; 577 cycles a block where the MMAs alone are 512, at some 1.3 GHz:
+// the power cap sets the clock, and long runs take 420 to 440 us.
 #pragma once
 
 #include "float8_pair_sm100.cuh"

@@ -35,7 +35,7 @@ def _padded(n: int) -> int:
     return (n + 15) // 16 * 16
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, init=False, eq=False)
 class Float8Matrix:
     """A ``[rows, cols]`` matrix of e4m3 codes and its fp32 scales.
 
@@ -51,8 +51,7 @@ class Float8Matrix:
     values: Tensor
     scales: Tensor
 
-    def __post_init__(self) -> None:
-        values, scales = self.values, self.scales
+    def __init__(self, values: Tensor, scales: Tensor) -> None:
         if values.dtype is not CODES or scales.dtype is not torch.float32:
             raise TypeError(f"Float8Matrix needs float8_e4m3fn codes and float32 scales, got {values.dtype}, {scales.dtype}")
         if values.ndim != 2 or scales.ndim != 2 or values.device != scales.device:
@@ -60,11 +59,14 @@ class Float8Matrix:
                 f"Float8Matrix needs two matrices on one device, got shapes {tuple(values.shape)} on {values.device} and "
                 f"{tuple(scales.shape)} on {scales.device}")
         rows, cols = values.shape
-        if scales.shape[1] != _blocks(cols) or scales.shape[0] not in (rows, _blocks(rows)):
+        scale_rows, blocks = scales.shape
+        if blocks != (cols + 127) // BLOCK or (scale_rows != rows and scale_rows != (rows + 127) // BLOCK):
             raise ValueError(f"scales {tuple(scales.shape)} fit neither the rows nor the tiles of {tuple(values.shape)} codes")
-        if rows and cols and ((cols > 1 and values.stride(1) != 1) or values.data_ptr() % 16
-                              or (rows > 1 and (values.stride(0) % 16 or values.stride(0) < cols))):
+        ld, step = values.stride()
+        if ((cols > 1 and step != 1) or values.data_ptr() & 15 or (rows > 1 and (ld & 15 or ld < cols))) and rows and cols:
             raise ValueError(f"rows of codes must start on 16-byte boundaries, got strides {values.stride()}")
+        fields = self.__dict__   # (a frozen dataclass's own way costs a microsecond)
+        fields["values"], fields["scales"] = values, scales
 
     @property
     def shape(self) -> torch.Size:
@@ -163,25 +165,29 @@ def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = No
         ValueError: On shapes, strides or devices that do not fit, or ``accumulate`` without ``out``.
         TypeError: On other dtypes.
     """
-    (m, k), (n, other) = a.shape, b.shape
-    device = a.values.device
+    left, right = a.values, b.values
+    (m, k), (n, other) = left.shape, right.shape
+    number = left.get_device()
     if k != other:
         raise ValueError(f"float8_product: {tuple(a.shape)} and {tuple(b.shape)} differ in their columns")
-    if device.type != "cuda" or b.values.device != device:
-        raise ValueError(f"float8_product needs operands on one CUDA device, got {device} and {b.values.device}")
+    if not left.is_cuda or right.get_device() != number:
+        raise ValueError(f"float8_product needs operands on one CUDA device, got {left.device} and {right.device}")
+    device = left.device
     if out is None:
         if accumulate:
             raise ValueError("float8_product: accumulate needs out")
         out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
         if out_dtype not in _DTYPES:
             raise TypeError(f"float8_product gives float32, float16 or bfloat16, not {out_dtype}")
-        out = torch.empty(m, n, dtype=out_dtype, device=device)
-    if out.dtype not in _DTYPES or out_dtype not in (None, out.dtype):
-        raise TypeError(f"float8_product: out is {out.dtype}, out_dtype {out_dtype}")
-    if out.shape != (m, n) or out.device != device or (m and n and ((n > 1 and out.stride(1) != 1)
-                                                                    or (m > 1 and out.stride(0) < n))):
-        raise ValueError(f"float8_product: out must be a [{m}, {n}] matrix with contiguous rows on {device}, "
-                         f"got {tuple(out.shape)} with strides {out.stride()} on {out.device}")
+        out, ldo = torch.empty(m, n, dtype=out_dtype, device=device), n
+    else:
+        if out.dtype not in _DTYPES or (out_dtype is not None and out_dtype is not out.dtype):
+            raise TypeError(f"float8_product: out is {out.dtype}, out_dtype {out_dtype}")
+        if out.shape != (m, n) or out.get_device() != number or (m and n and ((n > 1 and out.stride(1) != 1)
+                                                                              or (m > 1 and out.stride(0) < n))):
+            raise ValueError(f"float8_product: out must be a [{m}, {n}] matrix with contiguous rows on {device}, "
+                             f"got {tuple(out.shape)} with strides {out.stride()} on {out.device}")
+        ldo = out.stride(0) if m > 1 else n
     if bias is not None:
         if bias.dtype not in _DTYPES:
             raise TypeError(f"float8_product: bias is {bias.dtype}")
@@ -189,10 +195,9 @@ def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = No
             raise ValueError(f"float8_product: bias must have {n} elements on {device}, got {tuple(bias.shape)} on {bias.device}")
         bias = bias.contiguous()
     if m and n:
-        number = out.get_device()
         scratch = _product_scratch(number, m, n, k)
-        _native.float8_product(number, _operand(a), _operand(b), bias, out, accumulate, m, n, k,
-                               torch.empty(scratch, dtype=torch.uint8, device=device) if scratch else None)
+        _native.float8_product(number, _operand(left, a.scales, m, k), _operand(right, b.scales, n, k), bias, out, ldo, accumulate,
+                               m, n, k, torch.empty(scratch, dtype=torch.uint8, device=device) if scratch else None)
     return out
 
 
@@ -201,10 +206,9 @@ def _product_scratch(device: int, m: int, n: int, k: int) -> int:
     return _native.float8_product_workspace_bytes(device, m, n, k)
 
 
-def _operand(x: Float8Matrix) -> tuple[int, int, int, int, int, bool]:
-    values, scales = x.values, x.scales
-    rows, cols = values.shape
-    return (values.data_ptr(), values.stride(0) if rows > 1 else _padded(cols), scales.data_ptr(), *scales.stride(),
+def _operand(values: Tensor, scales: Tensor, rows: int, cols: int) -> tuple[int, int, int, int, int, bool]:
+    row_stride, block_stride = scales.stride()
+    return (values.data_ptr(), values.stride(0) if rows > 1 else _padded(cols), scales.data_ptr(), row_stride, block_stride,
             scales.shape[0] != rows)
 
 
