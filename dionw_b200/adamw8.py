@@ -96,17 +96,18 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         raise TypeError(f"adamw8_step takes float32, float16 or bfloat16 gradients, got {grad_dtype}")
     # Hundreds of tensors a step: each question goes to all of them at once.
     n = len(params)
-    tensors = [*params, *grads, *exp_avg, *exp_avg_sq, *exp_avg_scale, *exp_avg_sq_scale, *steps]
+    arrays = [*params, *grads, *exp_avg, *exp_avg_sq, *exp_avg_scale, *exp_avg_sq_scale]
+    tensors = [*arrays, *steps]
     dtypes = [torch.float32] * n + [grad_dtype] * n + [MEAN_DTYPE] * n + [SQUARE_DTYPE] * n + [torch.float32] * (3 * n)
     if list(map(_dtype_of, tensors)) != dtypes:
         raise TypeError(
             f"adamw8_step needs float32 parameters, scales and step counters, {grad_dtype} gradients, {MEAN_DTYPE} and "
             f"{SQUARE_DTYPE} moments, got {sorted(set(map(str, map(_dtype_of, tensors))))}")
-    if set(map(Tensor.get_device, tensors)) != {device} or not all(map(Tensor.is_contiguous, tensors)):
+    if set(map(Tensor.get_device, tensors)) != {device} or not all(map(Tensor.is_contiguous, arrays)):
         raise ValueError("adamw8_step needs contiguous tensors of one device")
-    numels = list(map(Tensor.numel, params))
-    blocks = [(numel + BLOCK - 1) // BLOCK for numel in numels]
-    if list(map(Tensor.numel, tensors[n:])) != numels * 3 + blocks * 2 + [1] * n:
+    sizes = list(map(Tensor.numel, tensors))
+    numels = sizes[:n]
+    if sizes[n:] != numels * 3 + [(numel + 127) // BLOCK for numel in numels] * 2 + [1] * n:
         raise ValueError("adamw8_step: gradients, moments or scales do not have the sizes that their parameters need")
     addresses = list(map(Tensor.data_ptr, tensors))
     written = addresses[:n] + addresses[2 * n:]
