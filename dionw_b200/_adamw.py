@@ -4,6 +4,7 @@ A group with ``adamw_state_bits = 8`` keeps its moments as 8-bit codes with bloc
 
 from __future__ import annotations
 
+from array import array
 from collections.abc import Callable
 from typing import Any
 
@@ -15,7 +16,7 @@ from dionw_b200._keys import (
     ADAMW_STATE_BITS_KEY, ADAMW_STEP_STATE, EXP_AVG_SCALE_STATE, EXP_AVG_SQ_SCALE_STATE, EXP_AVG_SQ_STATE, EXP_AVG_STATE,
     ParamState,
 )
-from dionw_b200.adamw8 import adamw8_state
+from dionw_b200.adamw8 import adamw8_state, expected_kinds
 
 
 def init_adamw_state(param: Tensor, state: dict[str, Any], bits: int = 32) -> None:
@@ -76,12 +77,15 @@ def adamw_step(group: dict[str, Any], state: ParamState,
                     weight_decay=float(group["weight_decay"]), eps=float(group["eps"]),
                     hyper_device=None if hyper is None else hyper(device))
     if bits == 8:
+        if device.type != "cuda":
+            raise ValueError(f"an AdamW update runs on one CUDA device, not on {device}")
         tensors = [*p_list, *g_list, *m_list, *v_list, *scales[0], *scales[1], *s_list]
-        if device.type != "cuda" or set(map(Tensor.get_device, tensors)) != {p_list[0].get_device()}:
+        addresses, sizes, kinds = _native.tensor_table(tensors)
+        number, n = p_list[0].get_device(), len(p_list)
+        if kinds != array("Q", expected_kinds(number, torch.float32, n)):
             raise ValueError(f"an AdamW update needs its parameters, gradients and moments on one CUDA device, not {device} and "
-                             f"{sorted({str(t.device) for t in tensors})}")
-        _native.adamw8_multi(list(map(Tensor.data_ptr, tensors)), list(map(Tensor.numel, p_list)), torch.float32,
-                             device=p_list[0].get_device(), seed=0, **settings)
+                             f"{sorted({f'{t.dtype} on {t.device}' for t in tensors})}")
+        _native.adamw8_multi(addresses, sizes[:n], torch.float32, device=number, seed=0, **settings)
     else:
         with torch.cuda.device(device):
             _native.adamw_multi(p_list, g_list, m_list, v_list, s_list, **settings)

@@ -12,10 +12,11 @@ The reference keeps its moments in fp32 (src/dionw/_adamw.py:18-61).
 
 from __future__ import annotations
 
+import functools
 import math
+from array import array
 from collections.abc import Sequence
-from operator import attrgetter
-from typing import Any
+from typing import Any, NoReturn
 
 import torch
 from torch import Tensor
@@ -28,7 +29,6 @@ from dionw_b200._keys import (
 BLOCK = 128                        # consecutive elements that share a scale
 MEAN_DTYPE = torch.float8_e4m3fn
 SQUARE_DTYPE = torch.float8_e5m2
-_dtype_of = attrgetter("dtype")
 _GRAD_DTYPES = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -94,25 +94,18 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         raise ValueError(f"adamw8_step runs on CUDA devices, got a parameter on {params[0].device}")
     if grad_dtype not in _GRAD_DTYPES:
         raise TypeError(f"adamw8_step takes float32, float16 or bfloat16 gradients, got {grad_dtype}")
-    # Hundreds of tensors a step: each question goes to all of them at once.
+    # Hundreds of tensors a step: one question to all of them.
     n = len(params)
-    arrays = [*params, *grads, *exp_avg, *exp_avg_sq, *exp_avg_scale, *exp_avg_sq_scale]
-    tensors = [*arrays, *steps]
-    dtypes = [torch.float32] * n + [grad_dtype] * n + [MEAN_DTYPE] * n + [SQUARE_DTYPE] * n + [torch.float32] * (3 * n)
-    if list(map(_dtype_of, tensors)) != dtypes:
-        raise TypeError(
-            f"adamw8_step needs float32 parameters, scales and step counters, {grad_dtype} gradients, {MEAN_DTYPE} and "
-            f"{SQUARE_DTYPE} moments, got {sorted(set(map(str, map(_dtype_of, tensors))))}")
-    if set(map(Tensor.get_device, tensors)) != {device} or not all(map(Tensor.is_contiguous, arrays)):
-        raise ValueError("adamw8_step needs contiguous tensors of one device")
-    sizes = list(map(Tensor.numel, tensors))
+    tensors = [*params, *grads, *exp_avg, *exp_avg_sq, *exp_avg_scale, *exp_avg_sq_scale, *steps]
+    addresses, sizes, kinds = _native.tensor_table(tensors)
+    if kinds != array("Q", expected_kinds(device, grad_dtype, n)):
+        _refuse_kinds(tensors, device, grad_dtype)
     numels = sizes[:n]
-    if sizes[n:] != numels * 3 + [(numel + 127) // BLOCK for numel in numels] * 2 + [1] * n:
+    if sizes.tolist()[n:] != numels.tolist() * 3 + [(numel + 127) // BLOCK for numel in numels] * 2 + [1] * n:
         raise ValueError("adamw8_step: gradients, moments or scales do not have the sizes that their parameters need")
-    addresses = list(map(Tensor.data_ptr, tensors))
     written = addresses[:n] + addresses[2 * n:]
-    if len(set(written)) != 6 * n:   # tensors without elements may share an address
-        written = [a for a, k in zip(written, numels * 5 + [1] * n) if k]
+    if len(set(written)) != 6 * n:   # tensors without elements share the address 0
+        written = [a for a in written if a]
         if len(set(written)) != len(written):
             raise ValueError("adamw8_step: a parameter, a moment, a scale or a step counter is given twice")
     if hyper_device is not None and (hyper_device.get_device() != device or hyper_device.dtype is not torch.float32
@@ -120,6 +113,27 @@ def adamw8_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avg: Sequ
         raise ValueError("adamw8_step: hyper_device must be two contiguous float32 on the parameters' device")
     _native.adamw8_multi(addresses, numels, grad_dtype, device=device, lr=lr, beta1=beta1, beta2=beta2,
                          weight_decay=weight_decay, eps=eps, seed=seed, hyper_device=hyper_device)
+
+
+@functools.lru_cache(maxsize=64)
+def _kinds(device: int, grad_dtype: torch.dtype) -> tuple[int, ...]:
+    return tuple(_native.tensor_kind(t, device) for t in (torch.float32, grad_dtype, MEAN_DTYPE, SQUARE_DTYPE))
+
+
+def expected_kinds(device: int, grad_dtype: torch.dtype, n: int) -> list[int]:
+    """Of parameters, gradients, the two moments, their scales and step counters, n each, as ``_native.tensor_table`` says it."""
+    single, gradient, mean, square = _kinds(device, grad_dtype)
+    return [single] * n + [gradient] * n + [mean] * n + [square] * n + [single] * (3 * n)
+
+
+def _refuse_kinds(tensors: list[Tensor], device: int, grad_dtype: torch.dtype) -> NoReturn:
+    n = len(tensors) // 7
+    dtypes = [torch.float32] * n + [grad_dtype] * n + [MEAN_DTYPE] * n + [SQUARE_DTYPE] * n + [torch.float32] * (3 * n)
+    if [t.dtype for t in tensors] != dtypes:
+        raise TypeError(
+            f"adamw8_step needs float32 parameters, scales and step counters, {grad_dtype} gradients, {MEAN_DTYPE} and "
+            f"{SQUARE_DTYPE} moments, got {sorted({str(t.dtype) for t in tensors})}")
+    raise ValueError(f"adamw8_step needs contiguous tensors of device {device}")
 
 
 def require_adamw8_state(param: Tensor, entry: dict[str, Any]) -> None:

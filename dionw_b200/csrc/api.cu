@@ -47,6 +47,41 @@ extern "C" void dionw_last_error(char* buffer, size_t size) {
   buffer[size - 1] = '\0';
 }
 
+namespace {
+
+// DLPack's view of a tensor (dlpack.h, DLTensor).
+struct DlTensor {
+  void* data;
+  int32_t device_type, device_id;
+  int32_t ndim;
+  uint8_t type_code, bits;
+  uint16_t lanes;
+  int64_t* shape;
+  int64_t* strides;
+  uint64_t byte_offset;
+};
+
+}  // namespace
+
+extern "C" int dionw_tensor_table(int (*from_object)(void*, void*), void* const* objects, int n, uint64_t* address,
+                                  int64_t* numel, uint64_t* kind) {
+  for (int i = 0; i < n; ++i) {
+    DlTensor t;
+    if (from_object(objects[i], &t) != 0) return i + 1;
+    int64_t count = 1;
+    bool contiguous = true;
+    for (int d = t.ndim - 1; d >= 0; --d) {
+      contiguous = contiguous && (t.shape[d] == 1 || t.strides == nullptr || t.strides[d] == count);
+      count *= t.shape[d];
+    }
+    address[i] = count == 0 ? 0 : reinterpret_cast<uint64_t>(t.data) + t.byte_offset;
+    numel[i] = count;
+    kind[i] = uint64_t(t.type_code) | uint64_t(t.bits) << 8 | uint64_t(t.lanes) << 16 | uint64_t(uint8_t(t.device_type)) << 32 |
+              uint64_t(uint8_t(t.device_id)) << 40 | uint64_t(contiguous || count == 0) << 48;
+  }
+  return 0;
+}
+
 extern "C" const char* dionw_version(void) { return "dionw_b200 0.1.0 (sm_100a)"; }
 
 extern "C" int64_t dionw_launch_count(void) { return dionw::g_launches.load(std::memory_order_relaxed); }

@@ -58,6 +58,16 @@ extern "C" {
 void dionw_last_error(char* buffer, size_t size);
 /* Library version string. */
 const char* dionw_version(void);
+
+/* What a binding asks of each of n tensors before a multi-tensor call, in one call: address (0 of
+ * a tensor without elements), number of elements, and kind[i] = type code | bits << 8 | lanes << 16 |
+ * device type << 32 | device number << 40 | contiguous << 48, with DLPack's codes (CUDA is
+ * device type 2; float 2, bfloat 4, float8_e4m3fn 10, float8_e5m2 12).  from_object is the
+ * dltensor_from_py_object_no_sync of the framework's DLPack exchange API (DLPack 1.3), objects
+ * are its tensors; the caller holds what that function needs (the interpreter's lock).  Returns 0, or 1 +
+ * the index of the tensor that from_object refused. */
+int dionw_tensor_table(int (*from_object)(void* object, void* dl_tensor), void* const* objects,
+                       int n, uint64_t* address, int64_t* numel, uint64_t* kind);
 /* Kernels this library has launched in this process so far (all threads). */
 int64_t dionw_launch_count(void);
 /* Reads and clears the device status word (non-zero: a bounded wait inside a

@@ -253,6 +253,23 @@ def test_a_step_of_tensors_elsewhere_or_of_other_moments_is_refused() -> None:
         adamw_step({**group, "adamw_state_bits": 8}, state)
 
 
+def test_tensor_table_is_what_torch_says() -> None:
+    x = torch.randn(6, 50)
+    tensors = [x, torch.nn.Parameter(x), x.to(E4M3), x.to(torch.float8_e5m2), x.half(), x.bfloat16(), x.T, x[1:], x.view(-1)[7:],
+               x[:, :1], x[:, ::2], torch.zeros(()), torch.zeros(0, 5), torch.zeros(1, 4, 1), x.expand(3, 6, 50), x[:, None]]
+    addresses, numels, kinds = _native.tensor_table(tensors)
+    assert list(addresses) == [t.data_ptr() for t in tensors] and list(numels) == [t.numel() for t in tensors]
+    for t, kind in zip(tensors, kinds):
+        assert bool(kind >> 48) == t.is_contiguous(), t.shape
+        # on CPU: device type 1
+        assert kind % 2**32 == _native.tensor_kind(t.dtype, 0) % 2**32 and kind >> 32 & 0xFFFF == 1
+    assert len(set(_native.tensor_kind(t, d) for t in _native._DL_TYPES for d in range(8))) == 8 * len(_native._DL_TYPES)
+    assert all(len(values) == 0 for values in _native.tensor_table([]))
+    for bad in (3, None, x.to_sparse(), torch.zeros(3, device="meta")):
+        with pytest.raises(TypeError, match="memory of their own"):
+            _native.tensor_table([x, bad])
+
+
 def test_lists_and_room_that_are_missing_are_refused() -> None:
     lib = _native.library()
     at = 1 << 20
@@ -271,8 +288,8 @@ def test_linear_entries_refuse() -> None:
     at = 1 << 20
     assert lib.dionw_float8_packed_bytes(-1, 4, 0) == 0 and lib.dionw_float8_packed_bytes(0, 0, 0) == 256
     # codes 130 x 304, scales 3 x 130, exponents 3 x 2 x 128, each from a multiple of 256 bytes on
-    assert lib.dionw_float8_packed_bytes(130, 300, 0) == 39680 + 1792 + 3072
-    assert lib.dionw_float8_packed_bytes(130, 300, 1) == 39680 + 256 + 3072
+    assert lib.dionw_float8_packed_bytes(130, 300, 0) == 39680 + 1792 + 6 * 512
+    assert lib.dionw_float8_packed_bytes(130, 300, 1) == 39680 + 256 + 6 * 512
     assert lib.dionw_float8_linear_forward(at, 0, 8, at, 0, 8, None, 0, at, -1, 8, 8, at, None, None, None) == -1
     assert "bad shape" in _native.last_error()
     assert lib.dionw_float8_linear_backward(at, 0, 8, at, 0, None, 0, None, 4, 8, 8, at, None, None, None) == -1
