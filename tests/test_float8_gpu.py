@@ -152,7 +152,7 @@ def test_product_of_many_tiles(m, n, k, b_tiles) -> None:
     _close(dionw.float8_product(a, b, out=held.to(DEV), accumulate=True), a64, b64, held.double())
 
 
-@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 1153), (300, 260, 2400), (1300, 1100, 2900)])
+@pytest.mark.parametrize("m,n,k", [(2500, 1900, 1153), (513, 9500, 1153), (300, 260, 2400), (1300, 1100, 2900), (200, 4000, 6900)])
 @pytest.mark.parametrize("b_tiles", [False, True])
 @pytest.mark.parametrize("layout", ["rows", "blocks"])
 def test_product_of_many_tiles_and_powers_of_two(m, n, k, b_tiles, layout) -> None:
@@ -204,6 +204,25 @@ def test_product_adds_bias_and_what_is_there(m, n, dtype) -> None:
     room = torch.full((m, n + 9), 5.0, dtype=dtype, device=DEV)
     _close(dionw.float8_product(a, b, out=room[:, 3:n + 3]), a64, b64)
     assert bool((room[:, :3] == 5).all()) and bool((room[:, n + 3:] == 5).all())
+
+
+@pytest.mark.parametrize("m,n,k", [(200, 333, 3001), (66, 1030, 5000), (300, 700, 2048)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_product_in_parts_adds_bias_and_what_is_there(m, n, k, dtype) -> None:
+    """Few tiles with long sums: the CTAs of a cluster share them."""
+    a, a64 = _operand(m, k, False, 5, "rows")
+    b, b64 = _operand(n, k, False, 6)
+    gen = torch.Generator().manual_seed(7)
+    bias = (torch.randn(n, generator=gen) * 30).to(dtype)
+    held = (torch.randn(m, n, generator=gen) * 30).to(dtype)
+    out = held.to(DEV)
+    dionw.float8_product(a, b, bias=bias.to(DEV), out=out, accumulate=True)
+    _close(out, a64, b64, bias.double() + held.double())
+    room = torch.full((m + 2, n + 9), 5.0, dtype=dtype, device=DEV)
+    _close(dionw.float8_product(a, b, out=room[1:-1, 3:n + 3]), a64, b64)
+    assert bool((room[:, :3] == 5).all()) and bool((room[:, n + 3:] == 5).all()) and bool((room[[0, -1]] == 5).all())
+    again = [dionw.float8_product(a, b, out_dtype=torch.float32) for _ in range(3)]
+    assert torch.equal(again[0], again[1]) and torch.equal(again[0], again[2])
 
 
 def test_product_of_nothing() -> None:
