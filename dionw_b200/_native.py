@@ -491,20 +491,20 @@ def float8_packed_bytes(rows: int, cols: int, tiles: bool) -> int:
     return int(library().dionw_float8_packed_bytes(rows, cols, tiles))
 
 
-def float8_linear_forward(x: Tensor, ldx: int, weight: Tensor, ldw: int, bias: Tensor | None, y: Tensor, inputs: int,
-                          work: Tensor, x_kept: Tensor | None, weight_kept: Tensor | None) -> None:
-    tokens, outputs = y.shape
+def float8_linear_forward(x: Tensor, ldx: int, weight: Tensor, ldw: int, bias: Tensor | None, y: Tensor, tokens: int,
+                          inputs: int, outputs: int, work: Tensor, x_kept: int | None, weight_kept: int | None) -> None:
+    """What is kept is given by address."""
     on_device(y.get_device(), library().dionw_float8_linear_forward, x.data_ptr(), _DTYPE_CODE[x.dtype], ldx,
               weight.data_ptr(), _DTYPE_CODE[weight.dtype], ldw, _ptr(bias), 0 if bias is None else _DTYPE_CODE[bias.dtype],
-              y.data_ptr(), tokens, inputs, outputs, work.data_ptr(), _ptr(x_kept), _ptr(weight_kept))
+              y.data_ptr(), tokens, inputs, outputs, work.data_ptr(), x_kept, weight_kept)
 
 
 def float8_linear_backward(dy: Tensor, ldy: int, dx: Tensor | None, dw: Tensor | None, db: Tensor | None, tokens: int,
-                           inputs: int, outputs: int, work: Tensor | None, x_kept: Tensor | None,
-                           weight_kept: Tensor | None) -> None:
+                           inputs: int, outputs: int, work: Tensor | None, x_kept: int | None,
+                           weight_kept: int | None) -> None:
     on_device(dy.get_device(), library().dionw_float8_linear_backward, dy.data_ptr(), _DTYPE_CODE[dy.dtype], ldy, _ptr(dx),
               0 if dx is None else _DTYPE_CODE[dx.dtype], _ptr(dw), 0 if dw is None else _DTYPE_CODE[dw.dtype], _ptr(db),
-              tokens, inputs, outputs, _ptr(work), _ptr(x_kept), _ptr(weight_kept))
+              tokens, inputs, outputs, _ptr(work), x_kept, weight_kept)
 
 
 # ---------------------------------------------------------------------------

@@ -217,6 +217,14 @@ def _packed_bytes(rows: int, cols: int, tiles: bool) -> int:
     return _native.float8_packed_bytes(rows, cols, tiles)
 
 
+def _kept_at(kept: Tensor | None, x_bytes: int, need_x: bool, need_w: bool) -> tuple[int | None, int | None]:
+    """Addresses of the packed transposes of a layer's input and weight."""
+    if kept is None:
+        return None, None
+    at = kept.data_ptr()
+    return at if need_w else None, at + x_bytes if need_x else None
+
+
 class _Linear(torch.autograd.Function):
     """``x @ weight.T`` on 8-bit products; every operand is quantized along the side that is summed over.
 
@@ -229,27 +237,27 @@ class _Linear(torch.autograd.Function):
         (tokens, inputs), outputs, device = x.shape, weight.shape[0], x.device
         x_rows, ldx = _with_rows(x)
         w_rows, ldw = _with_rows(weight)
-
-        def room(nbytes: int) -> Tensor:
-            return torch.empty(nbytes, dtype=torch.uint8, device=device)
-
-        # What the backward pass needs, a byte an element: the packed transposes of both.
-        x_kept = room(_packed_bytes(inputs, tokens, False)) if need_w else None
-        w_kept = room(_packed_bytes(inputs, outputs, True)) if need_x else None
-        work = room(_packed_bytes(tokens, inputs, False) + _packed_bytes(outputs, inputs, True))
+        # What the backward pass needs, a byte an element: the packed transposes of both, x's first.
+        x_bytes = _packed_bytes(inputs, tokens, False) if need_w else 0
+        kept_bytes = x_bytes + (_packed_bytes(inputs, outputs, True) if need_x else 0)
+        kept = torch.empty(kept_bytes, dtype=torch.uint8, device=device) if kept_bytes else None
+        x_kept, w_kept = _kept_at(kept, x_bytes, need_x, need_w)
+        work = torch.empty(_packed_bytes(tokens, inputs, False) + _packed_bytes(outputs, inputs, True), dtype=torch.uint8,
+                           device=device)
         y = torch.empty(tokens, outputs, dtype=x.dtype, device=device)
-        _native.float8_linear_forward(x_rows, ldx, w_rows, ldw, None if bias is None else bias.contiguous(), y, inputs, work,
-                                      x_kept, w_kept)
-        ctx.save_for_backward(x_kept, w_kept)
-        ctx.made_of = (tokens, inputs, outputs, x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        _native.float8_linear_forward(x_rows, ldx, w_rows, ldw, None if bias is None else bias.contiguous(), y, tokens, inputs,
+                                      outputs, work, x_kept, w_kept)
+        ctx.save_for_backward(kept)
+        ctx.made_of = (tokens, inputs, outputs, x.dtype, weight.dtype, None if bias is None else bias.dtype, x_bytes)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad: Tensor) -> tuple[Tensor | None, ...]:
         need_x, need_w, need_b = ctx.needs_input_grad
-        tokens, inputs, outputs, x_dtype, w_dtype, b_dtype = ctx.made_of
-        x_kept, w_kept = ctx.saved_tensors
+        tokens, inputs, outputs, x_dtype, w_dtype, b_dtype, x_bytes = ctx.made_of
+        kept, = ctx.saved_tensors
+        x_kept, w_kept = _kept_at(kept, x_bytes, need_x, need_w)
         device = grad.device
         dx = torch.empty(tokens, inputs, dtype=x_dtype, device=device) if need_x else None
         dw = torch.empty(outputs, inputs, dtype=w_dtype, device=device) if need_w else None
@@ -275,10 +283,11 @@ def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tens
     """
     if weight.ndim != 2 or x.ndim < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"float8_linear: x {tuple(x.shape)} does not fit a weight {tuple(weight.shape)}")
-    for name, t in (("x", x), ("weight", weight), ("bias", bias)):
-        if t is not None and t.dtype not in _DTYPES:
+    number = x.get_device()
+    for name, t in (("x", x), ("weight", weight)) if bias is None else (("x", x), ("weight", weight), ("bias", bias)):
+        if t.dtype not in _DTYPES:
             raise TypeError(f"float8_linear takes float32, float16 and bfloat16, {name} is {t.dtype}")
-        if t is not None and (not t.is_cuda or t.device != x.device):
+        if not t.is_cuda or t.get_device() != number:
             raise ValueError(f"float8_linear needs its tensors on one CUDA device, {name} is on {t.device}")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"float8_linear: bias {tuple(bias.shape)} does not fit a weight {tuple(weight.shape)}")
