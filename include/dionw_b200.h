@@ -293,7 +293,7 @@ int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, 
  * where a_tiles != 0 (b likewise).  out must not overlap an operand.  Results do not depend on
  * anything but the operands: sums are taken in a fixed order.  a_exponents and b_exponents
  * (both or neither, 16-byte aligned): the scales as dionw_float8_quantize wrote them a second
- * time; a product with m above 64 then leaves them to the tensor cores.  Without them, and with a
+ * time; the tensor cores then apply them where that is the faster way.  Without them, and with a
  * workspace (nullable, 16-byte aligned, of the bytes that the function below says, 0 for small
  * products), a large product first looks whether all scales are powers of two (or NaN) and does
  * the same if so. */
