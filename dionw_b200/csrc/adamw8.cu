@@ -22,11 +22,17 @@ namespace {
 
 constexpr int kBlock = 128;          // elements of a scale: four for each lane of a warp
 constexpr int kTable = 96;
-constexpr int kUnroll = 2;           // blocks of a warp
-// Threads of a CTA.  Many small ones where SMs are full of them; large ones, that take a whole tensor each and count its step
-// themselves, where no tensor is larger than that: a launch less for the vectors of a model, which are a group of their own.
-constexpr int kThreads = 128, kVectorThreads = 512;
-constexpr int elements_of(int threads) { return threads / 32 * kUnroll * kBlock; }
+// Threads of a CTA, CTAs of an SM and blocks of a warp.  Whole accesses, eight rounds of CTAs and more: six of 128 threads with four blocks, so that what a tensor's
+// elements share is worked out half as often as with two (39.4 M elements with fp32 gradients 103.7 us against 105.1, 39.0 M with bf16
+// ones 94 against 98, 1051 M 2.76 ms against 2.92; three blocks 110, five 117, four with seven CTAs 118).  Otherwise eight with two
+// blocks (4.8 M elements between 16-byte boundaries 21.7 us, with four 23.5; 5 M aligned ones 16.2 and 17.1, 1 M 4.8 and 6.0, 5000
+// 3.6 and 6.3).  Where no tensor is larger than 4096 elements, 512
+// threads take a whole one and count its step themselves: a launch less for the vectors of a model, which are a group of their own.
+struct Aligned { static constexpr int kThreads = 128, kCtas = 6, kUnroll = 4; static constexpr bool kWhole = false; };
+struct Any { static constexpr int kThreads = 128, kCtas = 8, kUnroll = 2; static constexpr bool kWhole = false; };
+struct Vectors { static constexpr int kThreads = 512, kCtas = 2, kUnroll = 2; static constexpr bool kWhole = true; };
+template <typename Form>
+constexpr int elements_of = Form::kThreads / 32 * Form::kUnroll * kBlock;
 constexpr float kMeanMax = 448.0f, kSquareMax = 57344.0f;
 constexpr float kSmallestScale = 1.17549435e-38f;          // 2^-126: its reciprocal is finite
 
@@ -153,11 +159,11 @@ struct Factors {
 // scale of piece j's first moment, lane 2j + 1 with that of the second.
 //
 // What bounds it: at 16 bytes an element and 6.5 TB/s an SM has about 85 instructions a lane and element, so that both the
-// memory and the issue slots are nearly full.  39.4 M elements with fp32 gradients take 105 us, 6.0 TB/s.  The first version took
+// memory and the issue slots are nearly full.  39.4 M elements with fp32 gradients take 104 us, 6.1 TB/s.  The first version took
 // 141 us: each lane worked out each scale and its reciprocal, and each code went through the form that holds for the smallest
 // numbers too.  Those are now left to the pieces that have any (1 of 100 where gradients are normal), and the scales to a
 // lane each.  Noise that a byte permutation puts where the code wants it, instead of a shift and a mask, was 3 us.
-template <typename G, typename Words>
+template <int kUnroll, typename G, typename Words>
 __device__ __forceinline__ float update(Piece<G> (&x)[kUnroll], const Factors& f, int lane, Words&& words) {
   float m[kUnroll][4], v[kUnroll][4];
   float largest = 0.0f;
@@ -226,10 +232,12 @@ __device__ __forceinline__ float update(Piece<G> (&x)[kUnroll], const Factors& f
 // at most is one of a third and less.
 __device__ __forceinline__ float correction(float x) { return x < -1.0f ? 1.0f - __expf(x) : -expm1f(x); }
 
-// kWhole: a CTA takes all of a tensor, and its step has not been counted yet.
-template <typename G, int kCtaThreads, bool kWhole>
-__global__ void __launch_bounds__(kCtaThreads, 1024 / kCtaThreads)
+// Form::kWhole: a CTA takes all of a tensor, and its step has not been counted yet.
+template <typename G, typename Form>
+__global__ void __launch_bounds__(Form::kThreads, Form::kCtas)
 adamw8_kernel(const Table tab, const Hyper hyper) {
+  constexpr int kUnroll = Form::kUnroll;
+  constexpr bool kWhole = Form::kWhole;
   after_previous();
   const float lr = hyper.device != nullptr ? hyper.device[0] : hyper.lr;
   const float weight_decay = hyper.device != nullptr ? hyper.device[1] : hyper.weight_decay;
@@ -240,7 +248,7 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   }
   const unsigned first_cta = lo == 0 ? 0u : tab.block_end[lo - 1];
   const int lane = threadIdx.x & 31;
-  const long long first = ((long long)(blockIdx.x - first_cta) * (kCtaThreads / 32) + (threadIdx.x >> 5)) * kUnroll;
+  const long long first = ((long long)(blockIdx.x - first_cta) * (Form::kThreads / 32) + (threadIdx.x >> 5)) * kUnroll;
   const long long n = tab.numel[lo];
   const float step = kWhole ? *tab.step[lo] + 1.0f : *tab.step[lo];
   if constexpr (kWhole) {
@@ -277,7 +285,7 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
 #pragma unroll
     for (int i = 0; i < 4; ++i, h += apart) w[i] = mix(h);
   };
-  // lane 2j, 2j + 1 of the warp: the scales of block first + j
+  // lanes 2j, 2j + 1 of the warp: the scales of block first + j
   float* const scale_at = ((lane & 1) != 0 ? v_scale : m_scale) + first + (lane >> 1);
   if (all_fours) {
 #pragma unroll
@@ -290,7 +298,7 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
       x[j].m_scale = m_scale[first + j];
       x[j].v_scale = v_scale[first + j];
     }
-    const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) { words((first + j) * kBlock + 4 * lane, 0x9E3779B1u, w); });
+    const float scale = update<kUnroll>(x, f, lane, [&](int j, uint32_t (&w)[4]) { words((first + j) * kBlock + 4 * lane, 0x9E3779B1u, w); });
 #pragma unroll
     for (int j = 0; j < kUnroll; ++j) {
       const long long e = (first + j) * kBlock + 4 * lane;
@@ -329,7 +337,7 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
       }
     }
   }
-  const float scale = update(x, f, lane, [&](int j, uint32_t (&w)[4]) {
+  const float scale = update<kUnroll>(x, f, lane, [&](int j, uint32_t (&w)[4]) {
     words((first + j) * kBlock + (codes_fours ? 4 * lane : lane), codes_fours ? 0x9E3779B1u : 32u * 0x9E3779B1u, w);
   });
 #pragma unroll
@@ -355,17 +363,47 @@ adamw8_kernel(const Table tab, const Hyper hyper) {
   if (lane < 2 * kUnroll && (first + (lane >> 1)) * kBlock < n) *scale_at = scale;
 }
 
-template <typename G>
-int launch(const Table& tab, unsigned ctas, bool whole, const Hyper& hyper, cudaStream_t stream) {
-  if (whole) {
-    launch_dependent(adamw8_kernel<G, kVectorThreads, true>, ctas, kVectorThreads, stream, tab, hyper);
-    return launch_status("adamw8_kernel");
+// Launches one form of the kernel over the first `count` tensors of the table, or as many as a grid takes: -> `count`.
+template <typename G, typename Form>
+int launch(Table& tab, int& count, const Hyper& hyper, cudaStream_t stream) {
+  unsigned long long ctas = 0;
+  for (int i = 0; i < count; ++i) {
+    const unsigned long long need =
+        Form::kWhole ? 1 : (unsigned long long)((tab.numel[i] + elements_of<Form> - 1) / elements_of<Form>);
+    if (ctas + need > 0x7FFFFFFFull) {
+      if (i == 0) {
+        set_error("adamw8_multi: a tensor of %lld elements is too large for one launch", (long long)tab.numel[i]);
+        return DIONW_ERR_UNSUPPORTED;
+      }
+      count = i;
+      break;
+    }
+    ctas += need;
+    tab.block_end[i] = unsigned(ctas);
   }
-  launch_dependent(adamw8_bump_steps_kernel, 1, kTable, stream, tab);
-  const int st = launch_status("adamw8_bump_steps_kernel");
-  if (st != DIONW_OK || ctas == 0) return st;   // empty tensors still count the step
-  launch_dependent(adamw8_kernel<G, kThreads, false>, ctas, kThreads, stream, tab, hyper);
+  tab.n = count;
+  if (!Form::kWhole) {
+    launch_dependent(adamw8_bump_steps_kernel, 1, kTable, stream, tab);
+    const int st = launch_status("adamw8_bump_steps_kernel");
+    if (st != DIONW_OK || ctas == 0) return st;   // empty tensors still count the step
+  }
+  launch_dependent(adamw8_kernel<G, Form>, unsigned(ctas), Form::kThreads, stream, tab, hyper);
   return launch_status("adamw8_kernel");
+}
+
+template <typename G>
+int launch(Table& tab, int& count, const Hyper& hyper, cudaStream_t stream) {
+  bool vectors = true, aligned = true;
+  long long all = 0;
+  for (int i = 0; i < count; ++i) {
+    all += tab.numel[i];
+    vectors = vectors && tab.numel[i] <= elements_of<Vectors>;
+    aligned = aligned && aligned16(tab.p[i]) && reinterpret_cast<uintptr_t>(tab.g[i]) % (4 * sizeof(G)) == 0 &&
+              (reinterpret_cast<uintptr_t>(tab.m[i]) | reinterpret_cast<uintptr_t>(tab.v[i])) % 4 == 0;
+  }
+  if (vectors) return launch<G, Vectors>(tab, count, hyper, stream);
+  aligned = aligned && all >= 8ll * sm_count() * Aligned::kCtas * elements_of<Aligned>;
+  return aligned ? launch<G, Aligned>(tab, count, hyper, stream) : launch<G, Any>(tab, count, hyper, stream);
 }
 
 }  // namespace
@@ -399,11 +437,9 @@ extern "C" int dionw_adamw8_multi(void* const* params, const void* const* grads,
   for (int start = 0; start < n_tensors;) {
     Table tab;
     int count = 0;
-    bool whole = true;
     for (; start + count < n_tensors && count < kTable; ++count) {
       const int i = start + count;
       DIONW_REQUIRE(numels[i] >= 0, "adamw8_multi: tensor %d has %lld elements", i, (long long)numels[i]);
-      whole = whole && numels[i] <= elements_of(kVectorThreads);
       tab.p[count] = static_cast<float*>(params[i]);
       tab.g[count] = grads[i];
       tab.m[count] = static_cast<uint8_t*>(exp_avg[i]);
@@ -413,26 +449,11 @@ extern "C" int dionw_adamw8_multi(void* const* params, const void* const* grads,
       tab.step[count] = static_cast<float*>(steps[i]);
       tab.numel[count] = numels[i];
     }
-    unsigned long long ctas = 0;
-    for (int i = 0; i < count; ++i) {
-      const unsigned long long need = whole ? 1 : (unsigned long long)((tab.numel[i] + elements_of(kThreads) - 1) / elements_of(kThreads));
-      if (ctas + need > 0x7FFFFFFFull) {
-        if (i == 0) {
-          set_error("adamw8_multi: a tensor of %lld elements is too large for one launch", (long long)tab.numel[i]);
-          return DIONW_ERR_UNSUPPORTED;
-        }
-        count = i;
-        break;
-      }
-      ctas += need;
-      tab.block_end[i] = unsigned(ctas);
-    }
-    tab.n = count;
-    start += count;
-    const int st = grad_dtype == DIONW_F32   ? launch<float>(tab, unsigned(ctas), whole, hyper, stream)
-                   : grad_dtype == DIONW_F16 ? launch<__half>(tab, unsigned(ctas), whole, hyper, stream)
-                                             : launch<__nv_bfloat16>(tab, unsigned(ctas), whole, hyper, stream);
+    const int st = grad_dtype == DIONW_F32   ? launch<float>(tab, count, hyper, stream)
+                   : grad_dtype == DIONW_F16 ? launch<__half>(tab, count, hyper, stream)
+                                             : launch<__nv_bfloat16>(tab, count, hyper, stream);
     if (st != DIONW_OK) return st;
+    start += count;
   }
   return DIONW_OK;
 }

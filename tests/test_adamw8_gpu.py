@@ -109,6 +109,34 @@ def test_step_of_codes_between_words(keys, shift) -> None:
     _check(t)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_many_elements_give_the_bits_of_a_call_each(dtype) -> None:
+    """Whole accesses with more blocks to a warp, from 14.6 M elements on, against tensors between 16-byte boundaries."""
+    sizes = [14_600_003, 300, 2048 * 127 + 1, 0, 4096]
+
+    def tensors(shift: int) -> dict[str, list[Tensor]]:
+        gen = torch.Generator(device=DEV).manual_seed(3)
+        out: dict[str, list[Tensor]] = {key: [] for key in ("p", "g", "m", "v", "ms", "vs", "t")}
+        for n in sizes:
+            p = torch.empty(n + shift, device=DEV)[shift:].copy_(torch.randn(n, device=DEV, generator=gen) * 0.02)
+            g = torch.empty(n + shift, dtype=dtype, device=DEV)[shift:].copy_(torch.randn(n, device=DEV, generator=gen) * 1e-3)
+            state = dionw.adamw8_state(p)
+            for key, value in zip(out, (p, g, *state.values())):
+                out[key].append(value)
+        return out
+
+    together, apart = tensors(0), tensors(1)
+    for _ in range(3):
+        _step(together)
+        for i in range(len(sizes)):
+            _step({key: values[i:i + 1] for key, values in apart.items()})
+    for key in together:
+        for a, b in zip(together[key], apart[key]):
+            assert torch.equal(a.reshape(-1).view(torch.uint8), b.clone().reshape(-1).view(torch.uint8)), key
+    assert [float(t) for t in together["t"]] == [3.0] * len(sizes)
+    assert float(together["m"][0].float().abs().max()) == 448.0
+
+
 def test_what_is_written_twice_is_refused() -> None:
     for key in ("p", "m", "v", "ms", "vs", "t"):
         t = _tensors([256, 256])
