@@ -177,7 +177,10 @@ def _tensor_exchange() -> tuple[Any, int]:
         entry.restype, entry.argtypes = SIGNATURES["dionw_tensor_table"]
         pointer = ctypes.pythonapi.PyCapsule_GetPointer
         pointer.restype, pointer.argtypes = c_void_p, (ctypes.py_object, c_char_p)
-        api = pointer(torch.Tensor.__dlpack_c_exchange_api__, b"dlpack_exchange_api")
+        capsule = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+        if capsule is None:
+            raise RuntimeError("dionw_b200 needs a torch with the DLPack exchange API")
+        api = pointer(capsule, b"dlpack_exchange_api")
         # two words of version, a pointer to another version's, then the functions: the fourth of them
         major = ctypes.c_uint32.from_address(api).value
         function = ctypes.c_uint64.from_address(api + 40).value
