@@ -158,9 +158,9 @@ struct Factors {
 // Updates a warp's pieces.  words(j, w) gives the noise of piece j's four elements.  Lane 2j of the warp is left with the
 // scale of piece j's first moment, lane 2j + 1 with that of the second.
 //
-// What bounds it: at 16 bytes an element and 6.5 TB/s an SM has about 85 instructions a lane and element, so that both the
-// memory and the issue slots are nearly full.  39.4 M elements with fp32 gradients take 104 us, 6.1 TB/s.  The first version took
-// 141 us: each lane worked out each scale and its reciprocal, and each code went through the form that holds for the smallest
+// What bounds it: the memory, as long as an element takes clearly fewer than the 85 instructions that an SM has time for at 16 bytes
+// an element and 6.5 TB/s.  It takes 58 (71 with two blocks a warp), and 39.4 M elements with fp32 gradients 104 us, 6.1 TB/s.  The
+// first version took 100 and 141 us: each lane worked out each scale and its reciprocal, and each code went through the form that holds for the smallest
 // numbers too.  Those are now left to the pieces that have any (1 of 100 where gradients are normal), and the scales to a
 // lane each.  Noise that a byte permutation puts where the code wants it, instead of a shift and a mask, was 3 us.
 template <int kUnroll, typename G, typename Words>
