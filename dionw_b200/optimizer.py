@@ -263,7 +263,9 @@ class _DionCore(Optimizer):
 
     def _restore_adamw8_state(self) -> None:
         """torch's loader casts floating state to the parameter's dtype: 8-bit moments come back as the fp32 values of
-        their codes, which turn into the same codes again."""
+        their codes, which turn into the same codes again.  What it has not cast are the tensors of the state that was
+        loaded: scales and step counters are copied as the codes are, or another optimizer's step would change them
+        under codes that belong to others."""
         for group in self.param_groups:
             if group.get(ADAMW_STATE_BITS_KEY, 32) != 8:
                 continue
@@ -272,6 +274,9 @@ class _DionCore(Optimizer):
                 for key, dtype in ((EXP_AVG_STATE, MEAN_DTYPE), (EXP_AVG_SQ_STATE, SQUARE_DTYPE)):
                     if key in entry:
                         entry[key] = entry[key].to(dtype).contiguous()
+                for key in (EXP_AVG_SCALE_STATE, EXP_AVG_SQ_SCALE_STATE, ADAMW_STEP_STATE):
+                    if key in entry:
+                        entry[key] = entry[key].clone(memory_format=torch.contiguous_format)
 
     @torch.no_grad()
     def step(self, closure: Callable[[], float] | None = None) -> float | None:
