@@ -16,7 +16,8 @@ a CUDA device.
 from __future__ import annotations
 
 import warnings
-from collections.abc import Callable, Iterable
+from collections.abc import Callable, Iterable, Iterator
+from contextlib import contextmanager
 from typing import Any
 
 import torch
@@ -45,6 +46,12 @@ __all__ = ["MAX_RUN_ELEMENTS", "NEWTON_SCHULZ_KEY", "Dion", "step_run"]
 # ``step_run`` is a module attribute so that it can be replaced; the overlapped step only
 # takes over while it is still this function.
 _sequential_step_run = step_run
+
+# What an AdamW state entry with 8-bit moments holds.
+_ADAMW8_DTYPES = {
+    EXP_AVG_STATE: MEAN_DTYPE, EXP_AVG_SQ_STATE: SQUARE_DTYPE, EXP_AVG_SCALE_STATE: torch.float32,
+    EXP_AVG_SQ_SCALE_STATE: torch.float32, ADAMW_STEP_STATE: torch.float32,
+}
 
 
 def _require_param(param: Tensor) -> None:
@@ -256,27 +263,45 @@ class _DionCore(Optimizer):
                     entry = state_dict["state"].get(index)
                     if entry:
                         require_adamw8_state(param, entry)
-        super().load_state_dict({**state_dict, "param_groups": saved})
-        self._restore_adamw8_state()
+        with self._adamw8_state_aside():
+            super().load_state_dict({**state_dict, "param_groups": saved})
         self._buckets = None
         self._graph = self._graph_warm = None
 
-    def _restore_adamw8_state(self) -> None:
-        """torch's loader casts floating state to the parameter's dtype: 8-bit moments come back as the fp32 values of
-        their codes, which turn into the same codes again.  What it has not cast are the tensors of the state that was
-        loaded: scales and step counters are copied as the codes are, or another optimizer's step would change them
-        under codes that belong to others."""
-        for group in self.param_groups:
-            if group.get(ADAMW_STATE_BITS_KEY, 32) != 8:
-                continue
-            for param in group["params"]:
-                entry = self.state.get(param) or {}
-                for key, dtype in ((EXP_AVG_STATE, MEAN_DTYPE), (EXP_AVG_SQ_STATE, SQUARE_DTYPE)):
-                    if key in entry:
-                        entry[key] = entry[key].to(dtype).contiguous()
-                for key in (EXP_AVG_SCALE_STATE, EXP_AVG_SQ_SCALE_STATE, ADAMW_STEP_STATE):
-                    if key in entry:
-                        entry[key] = entry[key].clone(memory_format=torch.contiguous_format)
+    @contextmanager
+    def _adamw8_state_aside(self) -> Iterator[None]:
+        """Keeps 8-bit AdamW state from torch's loader, which casts floating state to the parameter's dtype (eight bytes an
+        element at once) and takes over a tensor that needs no cast (scales of a living optimizer, whose step would
+        change them under codes that belong to others).  It is taken out behind the caller's pre-hooks and put in as
+        copies before the caller's post-hooks: both see the codes."""
+        aside: dict[Tensor, dict[str, Tensor]] = {}
+
+        def take_out(_: Optimizer, loading: dict[str, Any]) -> dict[str, Any]:
+            state = dict(loading["state"])
+            for saved, group in zip(loading["param_groups"], self.param_groups):
+                if group.get(ADAMW_STATE_BITS_KEY, 32) != 8:
+                    continue
+                for index, param in zip(saved["params"], group["params"]):
+                    entry = state.get(index) or {}
+                    aside[param] = {key: value for key, value in entry.items() if key in _ADAMW8_DTYPES}
+                    if index in state:
+                        state[index] = {key: value for key, value in entry.items() if key not in _ADAMW8_DTYPES}
+            return {**loading, "state": state}
+
+        def put_in(_: Optimizer) -> None:
+            while aside:
+                param, entry = aside.popitem()
+                for key, value in entry.items():
+                    self.state[param][key] = value.to(device=param.device, dtype=_ADAMW8_DTYPES[key], copy=True,
+                                                      memory_format=torch.contiguous_format)
+
+        hooks = (self.register_load_state_dict_pre_hook(take_out),
+                 self.register_load_state_dict_post_hook(put_in, prepend=True))
+        try:
+            yield
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     @torch.no_grad()
     def step(self, closure: Callable[[], float] | None = None) -> float | None:

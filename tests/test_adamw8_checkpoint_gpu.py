@@ -1,6 +1,8 @@
-"""Loading 8-bit AdamW moments: each optimizer has a state of its own."""
+"""Loading 8-bit AdamW moments: each optimizer has a state of its own, and the load takes no more room than it."""
 
 from __future__ import annotations
+
+import copy
 
 import pytest
 import torch
@@ -52,3 +54,60 @@ def test_a_state_loaded_from_a_living_optimizer_is_a_copy() -> None:
     moved = _state(first)
     _step(second, 2)
     assert _same(_state(second), moved) and _same(_state(first), moved)
+
+
+def test_loading_takes_the_room_of_the_codes() -> None:
+    """Two bytes an element and the scales, beside what the optimizer holds already: no fp32 copies on the way."""
+    n = 1 << 24
+    optimizer = _optimizer([n, n])
+    _step(optimizer, 0)
+    saved = copy.deepcopy(optimizer.state_dict())
+    for entry in saved["state"].values():
+        for key, value in entry.items():
+            entry[key] = value.cpu() if isinstance(value, Tensor) else value
+    expect = _state(optimizer)
+    _step(optimizer, 1)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    optimizer.load_state_dict(saved)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - before <= 2 * n * (2 + 8 / 128) + (1 << 20)
+    assert _same(_state(optimizer), expect)
+
+
+def test_loading_hooks_see_the_moments() -> None:
+    optimizer = _optimizer([300])
+    _step(optimizer, 0)
+    saved = copy.deepcopy(optimizer.state_dict())
+    expect = _state(optimizer)
+    seen = []
+
+    def before(opt: dionw.Dion, loading: dict) -> dict:
+        seen.append({key: value.dtype for key, value in loading["state"][0].items()})
+        return loading
+
+    def after(opt: dionw.Dion) -> None:
+        entry = opt.state[opt.param_groups[0]["params"][0]]
+        seen.append({key: entry[key].dtype for key in KEYS})
+
+    fresh = _optimizer([300], seed=1)
+    fresh.register_load_state_dict_pre_hook(before)
+    fresh.register_load_state_dict_post_hook(after)
+    for _ in range(2):   # what one load sets up is gone before the next
+        fresh.load_state_dict(saved)
+    dtypes = dict(zip(KEYS, (torch.float8_e4m3fn, torch.float8_e5m2, torch.float32, torch.float32, torch.float32)))
+    assert seen == [dtypes] * 4
+    assert _same(_state(fresh), expect)
+
+
+def test_a_checkpoint_that_does_not_fit_leaves_the_loader_as_it_was() -> None:
+    optimizer = _optimizer([300])
+    _step(optimizer, 0)
+    saved, expect = copy.deepcopy(optimizer.state_dict()), _state(optimizer)
+    broken = {**saved, "param_groups": [{**saved["param_groups"][0], "params": [0, 1]}]}
+    with pytest.raises(ValueError):
+        optimizer.load_state_dict(broken)
+    assert _same(_state(optimizer), expect)
+    optimizer.load_state_dict(saved)
+    assert _same(_state(optimizer), expect)
