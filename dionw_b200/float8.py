@@ -232,8 +232,9 @@ class _Linear(torch.autograd.Function):
     """
 
     @staticmethod
-    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None) -> Tensor:
-        need_x, need_w, _ = ctx.needs_input_grad
+    def forward(ctx: Any, x: Tensor, weight: Tensor, bias: Tensor | None, recorded: bool) -> Tensor:
+        # needs_input_grad says which inputs require gradients; that none is wanted of this call, only its caller knows
+        need_x, need_w = (need and recorded for need in ctx.needs_input_grad[:2])
         (tokens, inputs), outputs, device = x.shape, weight.shape[0], x.device
         x_rows, ldx = _with_rows(x)
         w_rows, ldw = _with_rows(weight)
@@ -254,7 +255,7 @@ class _Linear(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx: Any, grad: Tensor) -> tuple[Tensor | None, ...]:
-        need_x, need_w, need_b = ctx.needs_input_grad
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
         tokens, inputs, outputs, x_dtype, w_dtype, b_dtype, x_bytes = ctx.made_of
         kept, = ctx.saved_tensors
         x_kept, w_kept = _kept_at(kept, x_bytes, need_x, need_w)
@@ -266,7 +267,7 @@ class _Linear(torch.autograd.Function):
                            + (_packed_bytes(outputs, tokens, False) if need_w else 0), dtype=torch.uint8, device=device)
         dy, ldy = _with_rows(grad)
         _native.float8_linear_backward(dy, ldy, dx, dw, db, tokens, inputs, outputs, work, x_kept, w_kept)
-        return dx, dw, db if db is None or b_dtype is torch.float32 else db.to(b_dtype)
+        return dx, dw, db if db is None or b_dtype is torch.float32 else db.to(b_dtype), None
 
 
 def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
@@ -291,10 +292,11 @@ def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tens
             raise ValueError(f"float8_linear needs its tensors on one CUDA device, {name} is on {t.device}")
     if bias is not None and bias.shape != weight.shape[:1]:
         raise ValueError(f"float8_linear: bias {tuple(bias.shape)} does not fit a weight {tuple(weight.shape)}")
+    recorded = torch.is_grad_enabled()   # (never so inside a function's forward)
     if x.ndim == 2:
-        return _Linear.apply(x, weight, bias)
+        return _Linear.apply(x, weight, bias, recorded)
     leading = x.shape[:-1]
-    return _Linear.apply(x.reshape(math.prod(leading), x.shape[-1]), weight, bias).view(*leading, weight.shape[0])
+    return _Linear.apply(x.reshape(math.prod(leading), x.shape[-1]), weight, bias, recorded).view(*leading, weight.shape[0])
 
 
 class Float8Linear(nn.Linear):
