@@ -318,6 +318,7 @@ extern "C" int dionw_float8_product(const void* a, int64_t lda, const float* a_s
                 "float8_product: bad shape %lld x %lld x %lld", (long long)m, (long long)n, (long long)k);
   DIONW_REQUIRE(out_dtype >= DIONW_F32 && out_dtype <= DIONW_BF16, "float8_product: bad output dtype");
   DIONW_REQUIRE(bias == nullptr || (bias_dtype >= DIONW_F32 && bias_dtype <= DIONW_BF16), "float8_product: bad bias dtype");
+  DIONW_REQUIRE((a_exponents == nullptr) == (b_exponents == nullptr), "float8_product: exponents of one operand only");
   if (m == 0 || n == 0) return DIONW_OK;
   DIONW_REQUIRE(out != nullptr && ldo >= n, "float8_product: leading dimension %lld of %lld columns", (long long)ldo,
                 (long long)n);
