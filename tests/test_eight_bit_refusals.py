@@ -2,7 +2,14 @@
 
 from __future__ import annotations
 
+import contextlib
+
+import pytest
+import torch
+import torch.distributed as dist
+
 from dionw_b200 import _native
+from dionw_b200.distributed import ShardedDion
 
 
 def test_exponents_of_one_operand_are_refused() -> None:
@@ -19,3 +26,42 @@ def test_exponents_of_one_operand_are_refused() -> None:
             assert call(m, *one) == -1
             assert "one operand" in _native.last_error()
     assert call(0, at, at) == 0 and call(0, None, None) == 0
+
+
+def test_sharded_dion_refuses_moments_in_8_bits(tmp_path) -> None:
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        group = {"params": [], "dion_route": "adamw"}
+        with pytest.raises(ValueError, match="trainable"):   # 32 is not what is refused
+            ShardedDion([{**group, "adamw_state_bits": 32}], lr=1e-3)
+        with pytest.raises(NotImplementedError, match="float32"):
+            ShardedDion([{**group, "adamw_state_bits": 8}], lr=1e-3)
+        with pytest.raises(TypeError, match="adamw_state_bits"):
+            ShardedDion([group], lr=1e-3, adamw_state_bits=8)
+    finally:
+        dist.destroy_process_group()
+
+
+def test_a_call_runs_on_its_tensors_device(monkeypatch) -> None:
+    """The device is made current for the call, where it is not, and the stream is that device's."""
+    events: list = []
+
+    @contextlib.contextmanager
+    def device(number: int):
+        events.append(("enter", number))
+        yield
+        events.append(("leave", number))
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda number: 1000 + number, raising=False)
+
+    def entry(*args: int) -> int:
+        events.append(args)
+        return 0
+
+    _native.on_device(1, entry, 5, 6)
+    assert events == [(5, 6, 1001)]
+    events.clear()
+    _native.on_device(3, entry, 5)
+    assert events == [("enter", 3), (5, 1003), ("leave", 3)]

@@ -42,3 +42,57 @@ def test_a_pass_without_gradients_keeps_nothing(monkeypatch) -> None:
     results += [dionw.float8_linear(x, layer.weight.detach(), layer.bias.detach())]
     assert kept == [(False, False)] * 5
     assert all(torch.equal(r, with_gradients) and not r.requires_grad for r in results)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_a_checkpointed_layer_has_the_layers_gradients(reentrant) -> None:
+    from torch.utils.checkpoint import checkpoint
+
+    x, layer = _case()
+    dy = torch.randn(70, 192, device=DEV).bfloat16()
+    found = []
+    for run in (layer, lambda t: checkpoint(layer, t, use_reentrant=reentrant)):
+        leaf = x.clone().requires_grad_()
+        layer.zero_grad()
+        y = run(leaf)
+        y.backward(dy)
+        found.append((y.detach(), leaf.grad, layer.weight.grad, layer.bias.grad))
+    assert all(torch.equal(a, b) for a, b in zip(*found))
+
+
+def test_passes_of_several_batches_add_their_gradients() -> None:
+    """Each batch's gradient, added to the one before by autograd: one fp32 rounding each."""
+    x, layer = _case(tokens=200)
+    dy = torch.randn(200, 192, device=DEV).bfloat16()
+    parts = []
+    for at in (slice(0, 70), slice(70, 71), slice(71, 200)):
+        layer.zero_grad()
+        layer(x[at]).backward(dy[at])
+        parts.append([p.grad for p in layer.parameters()])
+    layer.zero_grad()
+    for at in (slice(0, 70), slice(70, 71), slice(71, 200)):
+        layer(x[at]).backward(dy[at])
+    for i, p in enumerate(layer.parameters()):
+        assert torch.equal(p.grad, parts[0][i] + parts[1][i] + parts[2][i])
+    # and of one graph twice
+    layer.zero_grad()
+    y = layer(x)
+    y.backward(dy, retain_graph=True)
+    once = layer.weight.grad.clone()
+    y.backward(dy)
+    assert torch.equal(layer.weight.grad, once + once)
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs 2 GPUs")
+def test_tensors_of_a_device_that_is_not_current() -> None:
+    x, layer = _case()
+    dy = torch.randn(70, 192, device=DEV).bfloat16()
+    other = torch.device("cuda", 1)
+    moved = dionw.Float8Linear(256, 192, device=other)
+    moved.load_state_dict(layer.state_dict())
+    assert torch.cuda.current_device() == 0
+    layer(x).backward(dy)
+    y = moved(x.to(other))
+    y.backward(dy.to(other))
+    assert y.device == other and torch.cuda.current_device() == 0
+    assert all(torch.equal(p.grad, q.grad.to(DEV)) for p, q in zip(layer.parameters(), moved.parameters()))
