@@ -625,7 +625,8 @@ class _ShardedCore(_DionCore):
 class ShardedDion(IntegratedEMAOptimizer, _ShardedCore):
     """``Dion`` with work and state sharded over the ranks of ``process_group``.
 
-    Same arguments as ``Dion``.  Every rank must hold identical parameters and, at
+    Same arguments as ``Dion``, but ``adamw_state_bits``: AdamW moments are held in float32, and a group that
+    asks for other bits is refused.  Every rank must hold identical parameters and, at
     each step, identical gradients; after the step the parameters are again
     identical on every rank, and equal bit for bit to what a single-GPU ``Dion``
     computes.  ``state_dict()`` returns the single-GPU layout on every rank (it
