@@ -4,7 +4,8 @@ The moments of a parameter are an e4m3 and an e5m2 tensor of its shape, and a
 fp32 scale for every 128 consecutive elements of each: 2.1 bytes per element
 where fp32 moments take 8, and 16.1 bytes of memory traffic a step instead of 28.
 They are updated in fp32 and rounded stochastically for the next step, by a hash
-of the seed, the step and the element's place: the same call gives the same bits.
+of the seed, the step and the element's place in its tensor: the same call gives the same
+bits.  Tensors of one call, element by element, share their draws.
 ``Dion(..., adamw_state_bits=8)`` uses it for every AdamW-routed parameter.
 
 The reference keeps its moments in fp32 (src/dionw/_adamw.py:18-61).

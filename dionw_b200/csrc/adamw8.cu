@@ -9,8 +9,10 @@
 // That rounding is stochastic: to the code below or above, with the probability of the distance to the other.  An
 // average moves by (1 - beta) of its distance per step; where that is less than half a step of the format (6 to 12 % of
 // the value in e4m3, 12 to 25 % in e5m2), rounding to nearest would keep it where it is for ever.  Its noise is a hash of the
-// seed, the step and the element's index in its tensor: the same on every replay and whatever the launch looks
-// like.  A second moment that is not zero is not rounded to zero: the weight's step divides by its root.
+// seed, the step and the element's index in its tensor: the same on every replay and whatever the launch looks like, and the same
+// for element i of every tensor of a call.  It has 16 bits: the probability is that of the distance, to 2^-16 below it, which leaves a
+// slow average low by at most 2^-16 / (1 - beta) of a step of the format (0.015 of one for beta = 0.999).
+// A second moment that is not zero is not rounded to zero: the weight's step divides by its root.
 #include <cmath>
 #include <type_traits>
 
@@ -22,12 +24,13 @@ namespace {
 
 constexpr int kBlock = 128;          // elements of a scale: four for each lane of a warp
 constexpr int kTable = 96;
-// Threads of a CTA, CTAs of an SM and blocks of a warp.  Whole accesses, eight rounds of CTAs and more: six of 128 threads with four blocks, so that what a tensor's
-// elements share is worked out half as often as with two (39.4 M elements with fp32 gradients 103.7 us against 105.1, 39.0 M with bf16
-// ones 94 against 98, 1051 M 2.76 ms against 2.92; three blocks 110, five 117, four with seven CTAs 118).  Otherwise eight with two
-// blocks (4.8 M elements between 16-byte boundaries 21.7 us, with four 23.5; 5 M aligned ones 16.2 and 17.1, 1 M 4.8 and 6.0, 5000
-// 3.6 and 6.3).  Where no tensor is larger than 4096 elements, 512
-// threads take a whole one and count its step themselves: a launch less for the vectors of a model, which are a group of their own.
+// Threads of a CTA, CTAs of an SM and blocks of a warp, in three forms.
+// Aligned: whole accesses throughout, and at least eight rounds of CTAs.  A warp with four blocks works out what a tensor's elements
+//   share half as often as one with two: 39.4 M elements with fp32 gradients take 103.7 us against 105.1, 39.0 M with bf16 ones 94
+//   against 98, 1051 M 2.76 ms against 2.92.  (Three blocks 110 us, five 117, four with seven CTAs 118.)
+// Any: everything else.  Two blocks against four: 4.8 M elements between 16-byte boundaries 21.7 us and 23.5, 5 M aligned ones 16.2
+//   and 17.1, 1 M 4.8 and 6.0, 5000 3.6 and 6.3.
+// Vectors: no tensor above 4096 elements.  512 threads take a whole one and count its step themselves, which saves a launch.
 struct Aligned { static constexpr int kThreads = 128, kCtas = 6, kUnroll = 4; static constexpr bool kWhole = false; };
 struct Any { static constexpr int kThreads = 128, kCtas = 8, kUnroll = 2; static constexpr bool kWhole = false; };
 struct Vectors { static constexpr int kThreads = 512, kCtas = 2, kUnroll = 2; static constexpr bool kWhole = true; };

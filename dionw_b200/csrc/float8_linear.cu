@@ -49,7 +49,8 @@ int multiply(const Packed& x, const void* a, const Packed& y, const void* b, con
 // ---------------------------------------------------------------------------
 // A CTA takes 32 columns: eight lanes of a warp four columns each, four rows at a time, 64 rows with its 16 warps; the 64
 // partial sums of a column are added in a fixed order.  Eight rows are under way for each thread: with four, and half the
-// warps, 1000 x 2304 took 12.6 us.
+// warps, 1000 x 2304 took 12.6 us.  Bound by the few CTAs where a matrix is narrow and long: 768 columns of bf16 are 24 of them, and
+// take 11.4 us for 8192 rows, 217 us (0.5 TB/s) for 65536.
 constexpr int kSumColumns = 32, kSumThreads = 512;
 
 template <typename T>

@@ -5,8 +5,9 @@
 // The bound: a block of 128 is 512 cycles of MMA for 32 KB of codes a CTA.  In that time its eight summing warps read 128 x
 // 256 accumulators from TMEM (128 bytes each cycle and sub-partition: 256 cycles) and add them (64 packed
 // multiply-adds a thread, 128 issue cycles; twice that where each row of B has a scale of its own).  Two
-// accumulators of 256 columns are all of TMEM, so the warps give one back as soon as it is in registers.  Measured with a
-// scale for each row of both: 8192 x 14336 x 4096 826 us (the tensor cores apply powers of two in 350, float8_scaled_sm100.cuh).
+// accumulators of 256 columns are all of TMEM, so the warps give one back as soon as it is in registers.  Measured with scales
+// that are no powers of two: 8192 x 14336 x 4096 490 us with B's in tiles, 826 to 880 with a scale for each row of both, the look at
+// them included (the tensor cores apply powers of two in 350, float8_scaled_sm100.cuh).  What takes the rest of the time has not been found.
 #pragma once
 
 #include "float8_sm100.cuh"

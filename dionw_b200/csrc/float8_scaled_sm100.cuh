@@ -8,9 +8,11 @@
 // into each CTA with the codes of a block, tcgen05.cp from there into TMEM, where each 32 lanes get a copy.  The hardware takes
 // one scale for 32 codes of a row; the four MMAs of a block use the same ones.
 //
-// The tensor cores cut off what an addition to their fp32 sums leaves behind the last place, so that sums of one sign fall behind
-// by up to 2^-24 each 32 products: 4e-6 of a sum of 8192, 1e-3 of one of half a million.  After kPiece blocks the sums are therefore
-// taken into registers, where the pieces are added to nearest: 1.5e-6 at most, at any length.
+// The tensor cores cut off what an addition to their fp32 sums leaves behind the last place, up to 2^-23 of the sum for each 32
+// products, so that sums of one sign fall behind: 1e-3 of one of half a million.  After kPiece blocks the sums are therefore taken into
+// registers, where the pieces are added to nearest: at most 128 * 2^-23 = 1.5e-5 for a piece, and 2^-24 for each addition of one.
+// Measured on positive values of a wide range, 2304 x 2304 sums of 4096 to 131072 products: 1.35e-6 on average, 2.4e-6 at most (sums in
+// registers block by block, as float8_sm100.cuh does: 7e-8 to 3.7e-7 on average, 2.4e-6 at most).
 //
 // A tile's 256 columns are half of TMEM and there is one of them: the eight warps take it into registers at once, and
 // convert and store while the next tile is computed.  Tiles of 256 x 128 are for products that have too few of the wide ones.

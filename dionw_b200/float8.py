@@ -155,6 +155,10 @@ def float8_product(a: Float8Matrix, b: Float8Matrix, *, bias: Tensor | None = No
                    accumulate: bool = False, out_dtype: torch.dtype | None = None) -> Tensor:
     """``a @ b.T`` (``a`` ``[m, k]``, ``b`` ``[n, k]``), plus ``bias`` ``[n]``, summed in fp32 and rounded once.
 
+    Scales may have any value, as long as products of a row's and a column's stay within fp32's range; powers of two, as
+    the quantizers make them, are the fast ones for large products (the tensor cores apply them).  The same call gives the
+    same bits on the same kind of device.
+
     Args:
         out: ``[m, n]`` result (float32, float16 or bfloat16), rows contiguous; made if None.  Must not overlap
             ``a``, ``b`` or ``bias``.
@@ -275,8 +279,10 @@ def float8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tens
 
     ``x`` is ``[..., inputs]``, ``weight`` ``[outputs, inputs]`` (an fp32 master weight, or 2 bytes), the result has
     ``x``'s dtype, and the weight's gradient the weight's.  Activations and output gradients get a scale for each 1 x 128
-    block along the side that is summed over, the weight one for each 128 x 128 tile.  Both passes may be captured into
-    a CUDA graph; as with any layer, let no graph of an eager call on the same leaves live on meanwhile.
+    block along the side that is summed over, the weight one for each 128 x 128 tile.  A pass without gradients keeps
+    nothing.  Both passes may be captured into a CUDA graph; as with any layer, let no graph of an eager call on the same
+    leaves live on meanwhile.  Second derivatives, forward-mode derivatives, ``vmap`` and tracing by ``torch.compile`` are
+    not supported.
 
     Raises:
         ValueError: On shapes that do not fit, or tensors off CUDA or on different devices.

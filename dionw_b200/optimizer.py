@@ -573,7 +573,8 @@ class Dion(IntegratedEMAOptimizer, _DionCore):
         profile_region: Named profiling region entered around EMA work.
         adamw_state_bits: 32, or 8 to hold the moments of AdamW-routed parameters as 8-bit codes with a scale for
             each 128 elements (``adamw8_step``): 2.1 bytes an element instead of 8.  A group may have its own
-            ``"adamw_state_bits"``.
+            ``"adamw_state_bits"``.  Rounding uses seed 0: its draws depend on the step and the element's place in its
+            tensor alone.
 
     Raises:
         TypeError: For groups without a route or non-float32 parameters.

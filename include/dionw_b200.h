@@ -290,8 +290,10 @@ int dionw_float8_quantize(const void* x, int dtype, int64_t rows, int64_t cols, 
  * + bias[j] (nullable), + out[i, j] (accumulate != 0); sums in fp32, rounded once to out_dtype.
  * a [m, lda] and b [n, ldb] are e4m3 codes, rows on 16-byte boundaries; the scale of row i in
  * block b is a_scales[i * a_row_stride + b * a_block_stride], with i / 128 in the place of i
- * where a_tiles != 0 (b likewise).  out must not overlap an operand.  Results do not depend on
- * anything but the operands: sums are taken in a fixed order.  a_exponents and b_exponents
+ * where a_tiles != 0 (b likewise); products of a row's and a column's scale should lie within
+ * fp32's range.  out must not overlap an operand.  The same call gives the same bits: sums are
+ * taken in an order that the shape, the device's SM count and whether exponents or a workspace
+ * are given decide.  Without those two, low bits may be others.  a_exponents and b_exponents
  * (both or neither, 16-byte aligned): the scales as dionw_float8_quantize wrote them a second
  * time; the tensor cores then apply them where that is the faster way.  Without them, and with a
  * workspace (nullable, 16-byte aligned, of the bytes that the function below says, 0 for small
@@ -440,7 +442,8 @@ int dionw_adamw_multi(void* const* params, const void* const* grads, void* const
  * code times its scale; zeros everywhere are the state before the first step.  Moments are
  * updated in fp32 and rounded, for the next step, to a code below or above with the
  * probability of the distance to the other: by a hash of `seed`, the step and the element's
- * index, so that the same call gives the same bits.  A second moment that is not zero keeps
+ * index in its tensor, so that the same call gives the same bits (and element i of every
+ * tensor the same draw).  A second moment that is not zero keeps
  * a code that is not zero.  A block in which a moment becomes infinite or NaN gets the scale
  * NaN.  grads are of any of the three dtypes, params fp32; any alignment (16 bytes, and 4 of
  * the codes, are the fast ones).  The reference keeps moments in fp32 (src/dionw/_adamw.py:18-61). */
